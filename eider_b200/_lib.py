@@ -173,6 +173,28 @@ SIGNATURES = {
     "infer_nvfp4_w4a16_top1_f32_on_stream": (_I, [_P, _P, _P, _P, _P, _U32, _P, _P, _U32, _U32, _F, _U32, _P]),
     "infer_deepseek4_block_fp8_linear_f32_on_stream": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _P]),
     "infer_block_fp8_f32_scale_linear_f32_on_stream": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _P]),
+    "eider_b200_mxfp4_scale_layout_len": (_SZ, [_SZ, _SZ]),
+    "eider_b200_quantize_mxfp4_on_stream": (_I, [_P, _I, _SZ, _P, _P, _U32, _U32, _P]),
+    "eider_b200_quantize_mxfp4_weight_on_stream": (_I, [_P, _I, _P, _P, _U32, _U32, _P]),
+    "eider_b200_silu_mul_halves_quantize_mxfp4_on_stream": (_I, [_P, _P, _P, _U32, _U32, _P]),
+    "eider_b200_dequantize_mxfp4_on_stream": (_I, [_P, _P, _P, _I, _U32, _U32, _P]),
+    "eider_b200_mxfp4_scales_to_tiled_on_stream": (_I, [_P, _P, _U32, _U32, _U32, _P]),
+    "eider_b200_mxfp4_gemm_tn_supported": (_I, [_U32, _U32, _U32]),
+    "eider_b200_mxfp4_gemm_tn_create": (_P, [_U32, _U32, _U32]),
+    "eider_b200_mxfp4_gemm_tn_destroy": (None, [_P]),
+    "eider_b200_mxfp4_gemm_tn_on_stream": (_I, [_P, _P, _P, _P, _P, _P, _P, _F, _F, _I, _P]),
+    "eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream": (_I, [_P, _P, _P, _P, _P, _F, _P, _P, _P]),
+    "eider_b200_mxfp4_decode_create": (_P, [_U32, _U32, _U32]),
+    "eider_b200_mxfp4_decode_destroy": (None, [_P]),
+    "eider_b200_mxfp4_decode_status": (_I, [_P, _P]),
+    "eider_b200_mxfp4_w4a16_gemv_on_stream": (_I, [_P, _P, _I, _U32, _P, _P, _U32, _P, _P, _F, _I, _P]),
+    "eider_b200_moe_quantize_routes_mxfp4_on_stream": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _P]),
+    "eider_b200_mxfp4_grouped_gemm_supported": (_I, [_U32, _U32, _U32, _U32]),
+    "eider_b200_mxfp4_grouped_gemm_create": (_P, [_U32, _U32, _U32, _U32]),
+    "eider_b200_mxfp4_grouped_gemm_destroy": (None, [_P]),
+    "eider_b200_mxfp4_grouped_gemm_on_stream": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _U32, _P]),
+    "eider_b200_mxfp4_grouped_gemm_silu_quantize_on_stream": (_I, [_P, _P, _P, _P, _P, _P, _P, _U32, _P, _P, _U32, _P]),
+    "eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _P]),
     "eider_b200_peer_barrier_on_stream": (_I, [_P, _U32, _U32, _U32, _P, C.c_uint64, _P]),
 }
 

@@ -16,8 +16,13 @@ inline bool is_pair_code(uint32_t block_n) { return block_n == kPairBlockCode ||
 // Dense GEMMs (row-major output): picks the kernel for the tile code and the kind of output and fills in the column tiles.
 // `p.row_tiles` and `p.splits` are set by the caller.
 cudaError_t launch_dense(int kind, uint32_t block_n, const CUtensorMap& map_rows, const CUtensorMap& map_cols, Params p, cudaStream_t stream);
-// The gate/up GEMM with the SiLU * up -> NVFP4 quantizer in its epilogue.
-cudaError_t launch_gated(const CUtensorMap& map_rows, const CUtensorMap& map_cols, Params p, cudaStream_t stream);
+// The gate/up GEMM with the SiLU * up -> FP4 quantizer in its epilogue.
+cudaError_t launch_gated(int kind, const CUtensorMap& map_rows, const CUtensorMap& map_cols, Params p, cudaStream_t stream);
+// The MXFP4 kernels of the two above, and the grouped GEMM over MXFP4 experts (`p.act_packed`: SiLU * up -> MXFP4 in its epilogue).
+cudaError_t launch_dense_mxf4(uint32_t block_n, const CUtensorMap& map_rows, const CUtensorMap& map_cols, Params p, cudaStream_t stream);
+cudaError_t launch_gated_mxf4(const CUtensorMap& map_rows, const CUtensorMap& map_cols, Params p, cudaStream_t stream);
+cudaError_t launch_grouped_mxf4(const CUtensorMap& map_rows, const CUtensorMap& map_cols, Params p, uint32_t max_row_tiles, cudaStream_t stream,
+                                const ShortRowMaps& short_rows);
 
 namespace {
 
@@ -118,6 +123,27 @@ cudaError_t launch_pair(const CUtensorMap& map_rows, const CUtensorMap& map_cols
     cfg.gridDim = dim3(grid_pairs * 2);
     cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, map_rows, map_cols, p);
+}
+
+template <int KIND, bool ANY_OUTPUT>
+cudaError_t dispatch_dense(uint32_t block_n, const CUtensorMap& map_rows, const CUtensorMap& map_cols, Params& p, cudaStream_t stream) {
+    const uint32_t tile_n = block_n == kPairBlockCode ? kPairN : block_n == kPairNarrowBlockCode ? kPairNarrowN : block_n;
+    p.col_tiles = (p.cols + tile_n - 1) / tile_n;
+    const uint32_t pair_items = ((p.row_tiles + 1) / 2) * p.col_tiles * p.splits;
+    const uint32_t items = p.row_tiles * p.col_tiles * p.splits;
+    switch (block_n) {
+        case kPairBlockCode: return launch_pair<KIND, kPairN, false, ANY_OUTPUT>(map_rows, map_cols, p, pair_items, stream);
+        case kPairNarrowBlockCode: return launch_pair<KIND, kPairNarrowN, false, ANY_OUTPUT>(map_rows, map_cols, p, pair_items, stream);
+        case 256: return launch<KIND, 256, false, 1, false, 4, ANY_OUTPUT>(map_rows, map_cols, p, items, stream);
+        case 192: return launch<KIND, 192, false, 1, false, 4, ANY_OUTPUT>(map_rows, map_cols, p, items, stream);
+        case 128: return launch<KIND, 128, false, 1, false, 4, ANY_OUTPUT>(map_rows, map_cols, p, items, stream);
+        default: return launch<KIND, 64, false, 1, false, 4, ANY_OUTPUT>(map_rows, map_cols, p, items, stream);
+    }
+}
+template <int KIND>
+cudaError_t dispatch_gated(const CUtensorMap& map_rows, const CUtensorMap& map_cols, Params& p, cudaStream_t stream) {
+    p.col_tiles = p.gate_rows / kGatedFeatures;
+    return launch_pair<KIND, kPairN, true, false>(map_rows, map_cols, p, ((p.row_tiles + 1) / 2) * p.col_tiles, stream);
 }
 
 }  // namespace

@@ -28,11 +28,10 @@ constexpr uint32_t kPairHalfN = 128;  // of which each CTA loads half
 constexpr uint32_t kPairNarrowN = 192;
 
 template <int KIND, uint32_t PAIR_N = kPairN> struct PairSmem {
-    static constexpr bool kNv = KIND == kNvf4;
     static constexpr uint32_t kA = kTileRows * kStageBytesK;          // this CTA's 128 rows
     static constexpr uint32_t kB = (PAIR_N / 2) * kStageBytesK;       // this CTA's half of the weight rows
-    static constexpr uint32_t kSfA = kNv ? 4 * kScaleTileBytes : 0;   // scales of this CTA's rows
-    static constexpr uint32_t kSfB = kNv ? 8 * kScaleTileBytes : 0;   // scales of all 256 weight rows
+    static constexpr uint32_t kSfA = scale_tiles(KIND) * kScaleTileBytes;  // scales of this CTA's rows
+    static constexpr uint32_t kSfB = 2 * kSfA;                             // scales of all 256 weight rows
     static constexpr uint32_t kStage = kA + kB + kSfA + kSfB;
     // epilogue staging for TMA stores: per epilogue warp two buffers of 32 rows x 128 bytes (64 bf16 columns)
     static constexpr uint32_t kStoreBuf = 32 * 128;
@@ -84,6 +83,21 @@ __device__ __forceinline__ void gated_quantize_store32(const Params& p, uint32_t
         *reinterpret_cast<uint16_t*>(p.act_scales + tiled_scale_offset(row, feature / 16, p.gate_rows)) = static_cast<uint16_t>(scale_pair);
 }
 
+// The same in MXFP4, whose block is the 32 features.
+__device__ __forceinline__ void mx_gated_quantize_store32(const Params& p, uint32_t row, uint32_t feature, const uint32_t (&gate)[32],
+                                                          const uint32_t (&up)[32], float rs, bool row_ok, bool pad_ok) {
+    uint32_t code = 0;
+    if (row_ok) {
+        float v[32];
+        uint32_t words[4];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = mx::silu_mul(__uint_as_float(gate[i]) * rs, __uint_as_float(up[i]) * rs);
+        code = mx::quantize_block(v, words);
+        *reinterpret_cast<uint4*>(p.act_packed + static_cast<size_t>(row) * (p.gate_rows / 2) + feature / 2) = make_uint4(words[0], words[1], words[2], words[3]);
+    }
+    if (row_ok || pad_ok) p.act_scales[mx::tiled_offset(row, feature / mx::kBlock, p.gate_rows / mx::kBlock)] = static_cast<uint8_t>(code);
+}
+
 template <uint32_t COL_STEP>
 __device__ __forceinline__ bool pair_tile(const Params& p, uint32_t item, uint32_t rank, PairTile& t) {
     const uint32_t row_pairs = (p.row_tiles + 1) / 2;
@@ -105,12 +119,14 @@ template <int KIND, uint32_t PAIR_N = kPairN, bool GATED = false, bool ANY_OUTPU
 __global__ void __launch_bounds__(GATED ? 64 + 32 * kGatedEpilogueWarps : kNumThreads, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_cols, const Params p) {
     static_assert(PAIR_N == kPairN || PAIR_N == kPairNarrowN, "pair tiles are 256 or 192 weight rows wide");
-    static_assert(!GATED || (KIND == kNvf4 && PAIR_N == kPairN), "gated tiles are 128 gate and 128 up rows in NVFP4");
+    static_assert(!GATED || (KIND != kFp8 && PAIR_N == kPairN), "gated tiles are 128 gate and 128 up rows in FP4");
     constexpr uint32_t kColStep = GATED ? kGatedFeatures : PAIR_N;      // weight rows (gate rows) from one tile to the next
     constexpr uint32_t kEpiWarps = GATED ? kGatedEpilogueWarps : 4;     // epilogue warps per CTA
     using L = PairSmem<KIND, PAIR_N>;
     using T = TmemPlan<KIND, PAIR_N>;
-    constexpr bool kNv = KIND == kNvf4;
+    constexpr bool kNv = KIND != kFp8;                    // block-scaled FP4
+    constexpr uint32_t kSfTiles = scale_tiles(KIND);      // scale tiles per stage and 128 rows
+    constexpr uint32_t kSfStep = KIND == kMxf4 ? 2 : 1;   // MMAs that share a scale tile
     constexpr int STAGES = L::kStages;
     constexpr uint32_t kAcc = T::kAccStages;
 
@@ -176,20 +192,21 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_cons
             auto expect = [&](uint32_t s, uint32_t stage) {
                 const uint32_t kb = min(4u, (p.k_bytes - s * kStageBytesK + 31) / 32);  // MMAs in this stage
                 uint32_t bytes = L::kA + L::kB;
-                if (kNv) bytes += kb * kScaleTileBytes * ((row_sf ? 1 : 0) + 1 + (second_sf ? 1 : 0));
+                if (kNv) bytes += scale_tiles_of<KIND>(kb) * kScaleTileBytes * ((row_sf ? 1 : 0) + 1 + (second_sf ? 1 : 0));
                 umma::mbar_arrive_expect_tx(&full[stage], bytes);
                 return kb;
             };
             auto load_weights = [&](uint32_t s, uint32_t stage, uint32_t kb) {
-                const size_t k_off = static_cast<size_t>(s) * 4 * kScaleTileBytes;
+                const size_t k_off = static_cast<size_t>(s) * kSfTiles * kScaleTileBytes;
+                const uint32_t sf_bytes = scale_tiles_of<KIND>(kb) * kScaleTileBytes;
                 umma::tma_load_2d(smem_b + stage * L::kB, &map_cols, &full[stage], static_cast<int32_t>(s * kStageBytesK), static_cast<int32_t>(w_row0));
                 if (kNv) {
                     umma::bulk_load_1d(smem_sfb + stage * L::kSfB, p.sf_cols + static_cast<size_t>(sf_col_tile0) * p.sf_tile_stride + k_off,
-                                       kb * kScaleTileBytes, &full[stage]);
+                                       sf_bytes, &full[stage]);
                     if (second_sf)
-                        umma::bulk_load_1d(smem_sfb + stage * L::kSfB + 4 * kScaleTileBytes,
+                        umma::bulk_load_1d(smem_sfb + stage * L::kSfB + kSfTiles * kScaleTileBytes,
                                            p.sf_cols + static_cast<size_t>(sf_col_tile1) * p.sf_tile_stride + k_off,
-                                           kb * kScaleTileBytes, &full[stage]);
+                                           sf_bytes, &full[stage]);
                 }
             };
             auto load_rows = [&](uint32_t s, uint32_t stage, uint32_t kb) {
@@ -197,8 +214,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_cons
                                   static_cast<int32_t>(t.row0));
                 if (row_sf)
                     umma::bulk_load_1d(smem_sfa + stage * L::kSfA,
-                                       p.sf_rows + static_cast<size_t>(t.row_tile) * p.sf_tile_stride + static_cast<size_t>(s) * 4 * kScaleTileBytes,
-                                       kb * kScaleTileBytes, &full[stage]);
+                                       p.sf_rows + static_cast<size_t>(t.row_tile) * p.sf_tile_stride + static_cast<size_t>(s) * kSfTiles * kScaleTileBytes,
+                                       scale_tiles_of<KIND>(kb) * kScaleTileBytes, &full[stage]);
             };
             uint32_t s = t.k0;
             if (!dep_waited) {
@@ -244,7 +261,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_cons
     } else if (warp == 1) {
         // ------------------------------------------------------------------ even CTA: MMA issuer for the pair
         const bool leader = umma::elect_one();
-        constexpr uint32_t idesc = kNv ? umma::idesc_nvf4_pair(PAIR_N) : umma::idesc_f8_pair(PAIR_N);
+        constexpr uint32_t idesc = KIND == kNvf4 ? umma::idesc_nvf4_pair(PAIR_N) : umma::idesc_f8_pair(PAIR_N);
         const uint32_t a_lo0 = umma::desc_lo_sw128(umma::smem_u32(smem_a));
         const uint32_t b_lo0 = umma::desc_lo_sw128(umma::smem_u32(smem_b));
         const uint32_t sfa_lo0 = umma::desc_lo_scales(umma::smem_u32(smem_sfa));
@@ -276,37 +293,36 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_cons
                     const uint32_t sfa_lo = sfa_lo0 + stage * (L::kSfA >> 4);
                     const uint32_t sfb_lo = sfb_lo0 + stage * (L::kSfB >> 4);
                     const uint32_t nkb = (s + 1 < p.k_stages) ? 4u : tail_kb;
+                    // scale tile i of the stage into its tensor-memory columns
+                    auto copy_scales = [&](uint32_t i) {
+                        umma::tc_copy_scales_pair(sfa_tmem + i * 4, umma::make_desc(sfa_lo + i * 32, umma::kDescHiScales));
+                        umma::tc_copy_scales_pair(sfb_tmem + i * 8, umma::make_desc(sfb_lo + i * 32, umma::kDescHiScales));
+                        umma::tc_copy_scales_pair(sfb_tmem + i * 8 + 4, umma::make_desc(sfb_lo + (kSfTiles + i) * 32, umma::kDescHiScales));
+                    };
+                    auto mma = [&](uint32_t j, uint32_t accumulate) {
+                        const uint64_t a_desc = umma::make_desc(a_lo + j * 2, umma::kDescHiSw128);
+                        const uint64_t b_desc = umma::make_desc(b_lo + j * 2, umma::kDescHiSw128);
+                        const uint32_t sf = j / kSfStep;
+                        if constexpr (KIND == kNvf4)
+                            umma::mma_nvf4_pair(d_tmem, a_desc, b_desc, idesc, sfa_tmem + sf * 4, sfb_tmem + sf * 8 + sfb_sub, accumulate);
+                        else if constexpr (KIND == kMxf4)
+                            umma::mma_mxf4_pair(d_tmem, a_desc, b_desc, umma::idesc_mxf4(PAIR_N, j % kSfStep, 256), sfa_tmem + sf * 4,
+                                                sfb_tmem + sf * 8 + sfb_sub, accumulate);
+                        else
+                            umma::mma_f8_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
+                    };
                     if (nkb == 4) {
                         // the scale copies of a 64-element step right in front of its MMA: the copies of step j + 1 then run
                         // under the MMA of step j (measured 1.2 us of 33.9 against all twelve copies first)
 #pragma unroll
                         for (uint32_t j = 0; j < 4; ++j) {
-                            if (kNv) {
-                                umma::tc_copy_scales_pair(sfa_tmem + j * 4, umma::make_desc(sfa_lo + j * 32, umma::kDescHiScales));
-                                umma::tc_copy_scales_pair(sfb_tmem + j * 8, umma::make_desc(sfb_lo + j * 32, umma::kDescHiScales));
-                                umma::tc_copy_scales_pair(sfb_tmem + j * 8 + 4, umma::make_desc(sfb_lo + (4 + j) * 32, umma::kDescHiScales));
-                            }
-                            const uint64_t a_desc = umma::make_desc(a_lo + j * 2, umma::kDescHiSw128);
-                            const uint64_t b_desc = umma::make_desc(b_lo + j * 2, umma::kDescHiSw128);
-                            const uint32_t accumulate = (s > t.k0 || j > 0) ? 1u : 0u;
-                            if (kNv) umma::mma_nvf4_pair(d_tmem, a_desc, b_desc, idesc, sfa_tmem + j * 4, sfb_tmem + j * 8 + sfb_sub, accumulate);
-                            else umma::mma_f8_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
+                            if (kNv && j % kSfStep == 0) copy_scales(j / kSfStep);
+                            mma(j, (s > t.k0 || j > 0) ? 1u : 0u);
                         }
                     } else {
-                        for (uint32_t j = 0; j < nkb; ++j) {
-                            if (kNv) {
-                                umma::tc_copy_scales_pair(sfa_tmem + j * 4, umma::make_desc(sfa_lo + j * 32, umma::kDescHiScales));
-                                umma::tc_copy_scales_pair(sfb_tmem + j * 8, umma::make_desc(sfb_lo + j * 32, umma::kDescHiScales));
-                                umma::tc_copy_scales_pair(sfb_tmem + j * 8 + 4, umma::make_desc(sfb_lo + (4 + j) * 32, umma::kDescHiScales));
-                            }
-                        }
-                        for (uint32_t j = 0; j < nkb; ++j) {
-                            const uint64_t a_desc = umma::make_desc(a_lo + j * 2, umma::kDescHiSw128);
-                            const uint64_t b_desc = umma::make_desc(b_lo + j * 2, umma::kDescHiSw128);
-                            const uint32_t accumulate = (s > t.k0 || j > 0) ? 1u : 0u;
-                            if (kNv) umma::mma_nvf4_pair(d_tmem, a_desc, b_desc, idesc, sfa_tmem + j * 4, sfb_tmem + j * 8 + sfb_sub, accumulate);
-                            else umma::mma_f8_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
-                        }
+                        if (kNv)
+                            for (uint32_t i = 0; i < scale_tiles_of<KIND>(nkb); ++i) copy_scales(i);
+                        for (uint32_t j = 0; j < nkb; ++j) mma(j, (s > t.k0 || j > 0) ? 1u : 0u);
                     }
                     // the stage is free in both CTAs once these MMAs (and scale copies) retire
                     umma::tc_commit_pair_both(empty0_local + stage * 8);
@@ -347,7 +363,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_cons
                 umma::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) umma::mbar_arrive_cluster(accempty0_remote + acc * 8);
-                gated_quantize_store32(p, row, t.col0 + c, gate, up, rs, row_ok, t.row_tile < p.row_tiles);
+                if constexpr (KIND == kMxf4) mx_gated_quantize_store32(p, row, t.col0 + c, gate, up, rs, row_ok, t.row_tile < p.row_tiles);
+                else gated_quantize_store32(p, row, t.col0 + c, gate, up, rs, row_ok, t.row_tile < p.row_tiles);
             }
         } else {
         auto epilogue = [&](auto kind) {

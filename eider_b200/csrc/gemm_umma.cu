@@ -6,13 +6,14 @@
 #include "decode_umma.cuh"
 #include "decode_fp8_umma.cuh"
 #include "gemv_stream.cuh"
-#include "map_cache.h"
+#include "tensor_maps.cuh"
 
 #include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "eider_b200.h"
@@ -21,49 +22,6 @@ namespace eider {
 namespace gemm {
 namespace {
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The driver entry point is looked up at run time so the library loads on machines without a driver.
-EncodeTiled encode_fn() {
-    static EncodeTiled fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult res;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &res) == cudaSuccess &&
-            res == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiled>(ptr);
-    });
-    return fn;
-}
-
-// 2-D byte matrix [rows][row_bytes] with pitch `pitch_bytes`, box = 128 bytes x box_rows, 128-byte swizzle.
-cudaError_t make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_bytes, uint64_t pitch_bytes,
-                     uint32_t box_rows) {
-    EncodeTiled enc = encode_fn();
-    if (!enc) return cudaErrorNotSupported;
-    if ((reinterpret_cast<uintptr_t>(base) & 15) != 0 || pitch_bytes % 16 != 0) return cudaErrorInvalidValue;
-    cuuint64_t dims[2] = {row_bytes, rows};
-    cuuint64_t strides[1] = {pitch_bytes};
-    cuuint32_t box[2] = {kStageBytesK, box_rows};
-    cuuint32_t elem[2] = {1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
-// Tensor maps a plan has already encoded: encoding costs a driver call of a microsecond or two, which is a visible part of a 9 us
-// decode launch.
-struct MapCache {
-    FifoCache<CUtensorMap> maps;
-    cudaError_t get(const CUtensorMap** out, const void* base, uint64_t rows, uint64_t row_bytes, uint64_t pitch, uint32_t box_rows) {
-        return maps.get(out, MapKey{base, rows, row_bytes, pitch, box_rows},
-                        [&](CUtensorMap* map) { return make_map(map, base, rows, row_bytes, pitch, box_rows); });
-    }
-};
 // The row operand of the grouped GEMM in its three box heights.
 struct GroupedRowMaps {
     CUtensorMap rows128;
@@ -221,6 +179,7 @@ struct DecodeOperand {
 };
 
 struct GroupedPlan {
+    int kind;
     uint32_t m, max_n, k, groups;  // reference naming: m = out features per expert, max_n = max tokens per expert
     uint32_t* status;
     GroupedRowMapCache maps_a;
@@ -234,6 +193,9 @@ struct GroupedPlan {
 
 namespace {
 
+// Bytes from one 128-row scale tile of an FP4 matrix to the next: four-block groups of 512 bytes.
+uint32_t scale_tile_stride(int kind, uint32_t k) { return (k / (kind == kMxf4 ? mx::kBlock : 16) + 3) / 4 * 4 * 128; }
+
 cudaError_t alloc_status(uint32_t** status) {
     cudaError_t st = cudaMalloc(reinterpret_cast<void**>(status), sizeof(uint32_t));
     if (st != cudaSuccess) return st;
@@ -242,7 +204,7 @@ cudaError_t alloc_status(uint32_t** status) {
 
 bool dense_shape_ok(int kind, uint32_t m, uint32_t n, uint32_t k) {
     if (m == 0 || n == 0 || k == 0) return false;
-    if (kind == kNvf4) return k % 32 == 0;  // TMA pitch (K/2 bytes) must be a multiple of 16
+    if (kind != kFp8) return k % 32 == 0;  // TMA pitch (K/2 bytes) must be a multiple of 16; an MXFP4 block is 32 elements
     return k % 16 == 0;
 }
 
@@ -293,7 +255,7 @@ uint32_t pick_block_n(uint32_t m, uint32_t n, uint32_t sms) {
 uint32_t pick_k_splits(int kind, uint32_t m, uint32_t n, uint32_t k, uint32_t block_n, uint32_t sms) {
     const uint32_t row_tiles = (m + kTileRows - 1) / kTileRows;
     if (row_tiles > 1) return 1;
-    const uint32_t stages = ((kind == kNvf4 ? k / 2 : k) + kStageBytesK - 1) / kStageBytesK;
+    const uint32_t stages = ((kind != kFp8 ? k / 2 : k) + kStageBytesK - 1) / kStageBytesK;
     if (stages < 32) return 1;  // (a short K: the second launch costs what the split saves; the measured gains are at 54 stages)
     const bool pair = is_pair_code(block_n);
     const uint32_t slots = pair ? sms / 2 : sms;
@@ -323,7 +285,7 @@ uint32_t pick_k_splits(int kind, uint32_t m, uint32_t n, uint32_t k, uint32_t bl
 
 // Sets the plan's split count and makes sure the workspace can hold the partial sums (nothing changes on failure).
 cudaError_t set_k_splits(DensePlan& plan, uint32_t splits) {
-    const uint32_t stages = ((plan.kind == kNvf4 ? plan.k / 2 : plan.k) + kStageBytesK - 1) / kStageBytesK;
+    const uint32_t stages = ((plan.kind != kFp8 ? plan.k / 2 : plan.k) + kStageBytesK - 1) / kStageBytesK;
     if (splits == 0 || splits > 16) return cudaErrorInvalidValue;
     if (splits > 1 && (splits - 1) * ((stages + splits - 1) / splits) >= stages) return cudaErrorInvalidValue;  // an empty split
     const size_t need = splits > 1 ? static_cast<size_t>(splits) * plan.m * plan.n : 0;
@@ -344,7 +306,7 @@ cudaError_t set_k_splits(DensePlan& plan, uint32_t splits) {
 cudaError_t run_dense(DensePlan& plan, const uint8_t* x_values, const uint8_t* x_scales, const uint8_t* w_values,
                       const uint8_t* w_scales, const void* c, void* d, float alpha, float beta, const float* token_scale,
                       const float* channel_scale, int out_is_bf16, cudaStream_t stream) {
-    const bool nv = plan.kind == kNvf4;
+    const bool nv = plan.kind != kFp8;
     if (!x_values || !w_values || !d || (nv && (!x_scales || !w_scales))) return cudaErrorInvalidValue;
     if (beta != 0.0f && !c) return cudaErrorInvalidValue;
     const uint32_t k_bytes = nv ? plan.k / 2 : plan.k;
@@ -364,7 +326,7 @@ cudaError_t run_dense(DensePlan& plan, const uint8_t* x_values, const uint8_t* x
     p.k_stages = (k_bytes + kStageBytesK - 1) / kStageBytesK;
     p.sf_rows = x_scales;
     p.sf_cols = w_scales;
-    p.sf_tile_stride = ((plan.k / 16 + 3) / 4 * 4) * 128;
+    p.sf_tile_stride = scale_tile_stride(plan.kind, plan.k);
     p.out = d;
     p.c_in = c;
     p.ld_out = plan.n;
@@ -459,7 +421,7 @@ cudaError_t run_gated(DensePlan& plan, const uint8_t* x_values, const uint8_t* x
     p.k_stages = (k_bytes + kStageBytesK - 1) / kStageBytesK;
     p.sf_rows = x_scales;
     p.sf_cols = w_scales;
-    p.sf_tile_stride = ((plan.k / 16 + 3) / 4 * 4) * 128;
+    p.sf_tile_stride = scale_tile_stride(plan.kind, plan.k);
     p.alpha = alpha;
     p.row_scale = token_scale;
     p.splits = 1;
@@ -467,7 +429,7 @@ cudaError_t run_gated(DensePlan& plan, const uint8_t* x_values, const uint8_t* x
     p.act_packed = act_packed;
     p.act_scales = act_scales;
     p.act_input_scale = act_input_scale;
-    return launch_gated(*map_rows, *map_cols, p, stream);
+    return launch_gated(plan.kind, *map_rows, *map_cols, p, stream);
 }
 
 // Decode orientation: weights are the row operand (128 output features per tile on the tensor-memory
@@ -663,7 +625,7 @@ cudaError_t run_grouped(GroupedPlan& plan, const uint8_t* a_values, const uint8_
     cudaError_t st = plan.maps_a.get(&row_maps, a_values, total_routes, k_bytes);
     if (st != cudaSuccess) return st;
     st = plan.maps_w.get(&map_cols_p, w_values, static_cast<uint64_t>(plan.groups) * plan.m, k_bytes, k_bytes,
-                         plan.m % 256 == 0 ? 256 : 128);
+                         plan.kind == kMxf4 || plan.m % 256 == 0 ? 256 : 128);
     if (st != cudaSuccess) return st;
     const CUtensorMap& map_rows = row_maps->rows128;
     const ShortRowMaps& short_rows = row_maps->short_rows;
@@ -676,7 +638,7 @@ cudaError_t run_grouped(GroupedPlan& plan, const uint8_t* a_values, const uint8_
     p.k_stages = (k_bytes + kStageBytesK - 1) / kStageBytesK;
     p.sf_rows = a_scales;
     p.sf_cols = w_scales;
-    p.sf_tile_stride = ((plan.k / 16 + 3) / 4 * 4) * 128;
+    p.sf_tile_stride = scale_tile_stride(plan.kind, plan.k);
     p.out = output;
     p.ld_out = plan.m;
     p.out_is_bf16 = 1;
@@ -694,6 +656,7 @@ cudaError_t run_grouped(GroupedPlan& plan, const uint8_t* a_values, const uint8_
     p.act_tile_bytes = act_tile_bytes;
     // upper bound on work items: every expert may add one partial row tile
     const uint32_t max_row_tiles = (total_routes + kTileRows - 1) / kTileRows + plan.groups;
+    if (plan.kind == kMxf4) return launch_grouped_mxf4(map_rows, map_cols, p, max_row_tiles, stream, short_rows);
     if (plan.m % 256 == 0) {
         p.col_tiles = plan.m / 256;
         // sixteen epilogue warps: one 64-column step of the SiLU * up quantizer per warp (measured 98 us against 108 us with
@@ -835,6 +798,42 @@ cudaError_t eider_b200_gemm_plan_status(void* raw, uint32_t* host_status) {
     auto* plan = static_cast<DensePlan*>(raw);
     if (!plan || !host_status) return cudaErrorInvalidValue;
     return cudaMemcpy(host_status, plan->status, sizeof(uint32_t), cudaMemcpyDeviceToHost);
+}
+
+// ---- dense MXFP4 W4A4 GEMM -----------------------------------------------------------------
+// (No split K: its partial sums would live in the plan, and two captured graphs of one plan would share them.)
+int eider_b200_mxfp4_gemm_tn_supported(uint32_t m, uint32_t n, uint32_t k) { return dense_shape_ok(kMxf4, m, n, k) ? 1 : 0; }
+
+void* eider_b200_mxfp4_gemm_tn_create(uint32_t m, uint32_t n, uint32_t k) {
+    if (!dense_shape_ok(kMxf4, m, n, k)) return nullptr;
+    auto* plan = new (std::nothrow) DensePlan{kMxf4, m, n, k, pick_block_n(m, n, static_cast<uint32_t>(sm_count())), nullptr};
+    if (!plan) return nullptr;
+    if (alloc_status(&plan->status) != cudaSuccess) {
+        delete plan;
+        return nullptr;
+    }
+    plan->splits = 1;
+    return plan;
+}
+
+void eider_b200_mxfp4_gemm_tn_destroy(void* raw) { eider_b200_nvfp4_gemm_tn_destroy(raw); }
+
+cudaError_t eider_b200_mxfp4_gemm_tn_on_stream(void* raw, const uint8_t* x_values, const uint8_t* x_scales, const uint8_t* w_values,
+                                               const uint8_t* w_scales, const void* c, void* d, float alpha, float beta, int out_is_bf16,
+                                               cudaStream_t stream) {
+    auto* plan = static_cast<DensePlan*>(raw);
+    if (!plan || plan->kind != kMxf4) return cudaErrorInvalidValue;
+    if (((reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales)) & 15) != 0) return cudaErrorInvalidValue;
+    return run_dense(*plan, x_values, x_scales, w_values, w_scales, c, d, alpha, beta, nullptr, nullptr, out_is_bf16, stream);
+}
+
+cudaError_t eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream(void* raw, const uint8_t* x_values, const uint8_t* x_scales,
+                                                             const uint8_t* w_values, const uint8_t* w_scales, float alpha, uint8_t* packed,
+                                                             uint8_t* scales, cudaStream_t stream) {
+    auto* plan = static_cast<DensePlan*>(raw);
+    if (!plan || plan->kind != kMxf4) return cudaErrorInvalidValue;
+    if (((reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales)) & 15) != 0) return cudaErrorInvalidValue;
+    return run_gated(*plan, x_values, x_scales, w_values, w_scales, alpha, nullptr, packed, scales, 1.0f, stream);
 }
 
 // ---- dense FP8 E4M3 GEMM ---------------------------------------------------------------------
@@ -1478,7 +1477,7 @@ int eider_b200_nvfp4_grouped_gemm_supported(uint32_t m, uint32_t max_n, uint32_t
 
 void* eider_b200_nvfp4_grouped_gemm_create(uint32_t m, uint32_t max_n, uint32_t k, uint32_t groups) {
     if (!eider_b200_nvfp4_grouped_gemm_supported(m, max_n, k, groups)) return nullptr;
-    auto* plan = new GroupedPlan{m, max_n, k, groups, nullptr, {}, {}, nullptr, nullptr, nullptr, {}};
+    auto* plan = new GroupedPlan{kNvf4, m, max_n, k, groups, nullptr, {}, {}, nullptr, nullptr, nullptr, {}};
     if (alloc_status(&plan->status) != cudaSuccess) {
         delete plan;
         return nullptr;
@@ -1519,7 +1518,7 @@ cudaError_t infer_cutlass_fp4_grouped_gemm_on_stream(void* raw, const uint8_t* c
                                                      uint16_t* const* output, float* const* alpha, const uint32_t* tokens_per_expert,
                                                      cudaStream_t stream) {
     auto* plan = static_cast<GroupedPlan*>(raw);
-    if (!plan) return cudaErrorInvalidValue;
+    if (!plan || plan->kind != kNvf4) return cudaErrorInvalidValue;
     return run_grouped_tables(*plan, a_values, a_scales, b_values, b_scales, output, const_cast<const float* const*>(alpha),
                               tokens_per_expert, stream);
 }
@@ -1539,7 +1538,7 @@ cudaError_t eider_b200_nvfp4_grouped_gemm_on_stream(void* raw, const uint8_t* a_
                                                     const float* alpha, const uint32_t* expert_offsets, uint32_t total_routes,
                                                     cudaStream_t stream) {
     auto* plan = static_cast<GroupedPlan*>(raw);
-    if (!plan) return cudaErrorInvalidValue;
+    if (!plan || plan->kind != kNvf4) return cudaErrorInvalidValue;
     return run_grouped(*plan, a_values, a_scales, w_values, w_scales_tiled, output, alpha, expert_offsets, total_routes, stream);
 }
 
@@ -1552,9 +1551,51 @@ cudaError_t eider_b200_nvfp4_grouped_gemm_silu_quantize_on_stream(void* raw, con
     auto* plan = static_cast<GroupedPlan*>(raw);
     // m = 2 * intermediate: 32 interleaved weight rows give one 16-feature block, and the 16-byte packed stores of two blocks
     // need whole 64-column steps
-    if (!plan || !packed || !scales || scale_tile_bytes == 0 || plan->m % 128 != 0 || (reinterpret_cast<uintptr_t>(packed) & 15) != 0 ||
+    if (!plan || plan->kind != kNvf4 || !packed || !scales || scale_tile_bytes == 0 || plan->m % 128 != 0 || (reinterpret_cast<uintptr_t>(packed) & 15) != 0 ||
         (plan->m / 4) % 16 != 0 || (reinterpret_cast<uintptr_t>(scales) & 1) != 0)
         return cudaErrorInvalidValue;
+    return run_grouped(*plan, a_values, a_scales, w_values_interleaved, w_scales_tiled_interleaved, nullptr, alpha, expert_offsets,
+                       total_routes, stream, packed, scales, scale_tile_bytes);
+}
+
+// Experts in MXFP4: any number of output features in whole blocks of 32 (each expert's scales start on a 128-row tile of their own).
+int eider_b200_mxfp4_grouped_gemm_supported(uint32_t m, uint32_t max_n, uint32_t k, uint32_t groups) {
+    return (m > 0 && max_n > 0 && k > 0 && groups > 0 && m % 32 == 0 && k % 32 == 0 && static_cast<uint64_t>(m) * groups < (1ull << 31)) ? 1 : 0;
+}
+
+void* eider_b200_mxfp4_grouped_gemm_create(uint32_t m, uint32_t max_n, uint32_t k, uint32_t groups) {
+    if (!eider_b200_mxfp4_grouped_gemm_supported(m, max_n, k, groups)) return nullptr;
+    auto* plan = new (std::nothrow) GroupedPlan{kMxf4, m, max_n, k, groups, nullptr, {}, {}, nullptr, nullptr, nullptr, {}};
+    if (!plan) return nullptr;
+    if (alloc_status(&plan->status) != cudaSuccess) {
+        delete plan;
+        return nullptr;
+    }
+    return plan;
+}
+
+void eider_b200_mxfp4_grouped_gemm_destroy(void* raw) { eider_b200_nvfp4_grouped_gemm_destroy(raw); }
+
+cudaError_t eider_b200_mxfp4_grouped_gemm_on_stream(void* raw, const uint8_t* a_values, const uint8_t* a_scales, const uint8_t* w_values,
+                                                    const uint8_t* w_scales_tiled, uint16_t* output, const float* alpha,
+                                                    const uint32_t* expert_offsets, uint32_t total_routes, cudaStream_t stream) {
+    auto* plan = static_cast<GroupedPlan*>(raw);
+    if (!plan || plan->kind != kMxf4 || !output) return cudaErrorInvalidValue;
+    if (((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(w_scales_tiled)) & 15) != 0) return cudaErrorInvalidValue;
+    return run_grouped(*plan, a_values, a_scales, w_values, w_scales_tiled, output, alpha, expert_offsets, total_routes, stream);
+}
+
+cudaError_t eider_b200_mxfp4_grouped_gemm_silu_quantize_on_stream(void* raw, const uint8_t* a_values, const uint8_t* a_scales,
+                                                                  const uint8_t* w_values_interleaved, const uint8_t* w_scales_tiled_interleaved,
+                                                                  const float* alpha, const uint32_t* expert_offsets, uint32_t total_routes,
+                                                                  uint8_t* packed, uint8_t* scales, uint32_t scale_tile_bytes,
+                                                                  cudaStream_t stream) {
+    auto* plan = static_cast<GroupedPlan*>(raw);
+    // 64 interleaved weight rows, [32 gate, 32 up], give one 32-feature block
+    if (!plan || plan->kind != kMxf4 || !packed || !scales || plan->m % 64 != 0 || (reinterpret_cast<uintptr_t>(packed) & 15) != 0 ||
+        scale_tile_bytes != scale_tile_stride(kMxf4, plan->m / 2))
+        return cudaErrorInvalidValue;
+    if (((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(w_scales_tiled_interleaved)) & 15) != 0) return cudaErrorInvalidValue;
     return run_grouped(*plan, a_values, a_scales, w_values_interleaved, w_scales_tiled_interleaved, nullptr, alpha, expert_offsets,
                        total_routes, stream, packed, scales, scale_tile_bytes);
 }

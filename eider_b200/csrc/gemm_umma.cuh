@@ -19,12 +19,19 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "mx_block.cuh"
 #include "umma.cuh"
 
 namespace eider {
 namespace gemm {
 
-enum Kind { kNvf4 = 0, kFp8 = 1 };
+enum Kind { kNvf4 = 0, kFp8 = 1, kMxf4 = 2 };
+
+// 128-row scale tiles (four blocks of K, 512 bytes) that a stage's 256 FP4 elements take: a block is 16 elements in NVFP4 and 32
+// in MXFP4, whose scale copies are half as many for the same MMAs.  FP8 has none.
+__host__ __device__ constexpr uint32_t scale_tiles(int kind) { return kind == kNvf4 ? 4 : kind == kMxf4 ? 2 : 0; }
+// ... that `mmas` 64-element steps take
+template <int KIND> __device__ __forceinline__ uint32_t scale_tiles_of(uint32_t mmas) { return KIND == kMxf4 ? (mmas + 1) / 2 : mmas; }
 
 constexpr uint32_t kTileRows = 128;       // MMA M
 constexpr uint32_t kStageBytesK = 128;    // bytes of K per row per stage (one swizzle row)
@@ -111,28 +118,28 @@ template <typename F> __device__ __forceinline__ void for_each_out(const Params&
     for (uint32_t q = 0; q < p.n_peers; ++q) f(p.out_peers[q]);
 }
 
-template <int BLOCK_N> struct SmemLayout {
+template <int KIND, int BLOCK_N> struct SmemLayout {
     static constexpr uint32_t kA = kTileRows * kStageBytesK;                 // 16 KB
     static constexpr uint32_t kB = BLOCK_N * kStageBytesK;
-    static constexpr uint32_t kSfA = 4 * kScaleTileBytes;                    // 2 KB
-    static constexpr uint32_t kSfB = (BLOCK_N > 128 ? 2 : 1) * 4 * kScaleTileBytes;
-    __host__ __device__ static constexpr uint32_t stage_bytes(bool nvf4) { return kA + kB + (nvf4 ? kSfA + kSfB : 0); }
+    static constexpr uint32_t kSfA = scale_tiles(KIND) * kScaleTileBytes;    // 2 KB (NVFP4), 1 KB (MXFP4)
+    static constexpr uint32_t kSfB = (BLOCK_N > 128 ? 2 : 1) * kSfA;
+    static constexpr uint32_t kStage = kA + kB + kSfA + kSfB;
 };
 
 template <int KIND, int BLOCK_N> constexpr int default_stages() {
-    constexpr uint32_t per = SmemLayout<BLOCK_N>::stage_bytes(KIND == kNvf4);
+    constexpr uint32_t per = SmemLayout<KIND, BLOCK_N>::kStage;
     constexpr int s = static_cast<int>((220u * 1024u) / per);
     return s > 8 ? 8 : s;
 }
 
 template <int KIND, int BLOCK_N, int STAGES> constexpr uint32_t smem_bytes() {
-    return SmemLayout<BLOCK_N>::stage_bytes(KIND == kNvf4) * STAGES + 1024 /*alignment slack*/ + 256 /*barriers*/;
+    return SmemLayout<KIND, BLOCK_N>::kStage * STAGES + 1024 /*alignment slack*/ + 256 /*barriers*/;
 }
 
-// Tensor-memory columns: accumulator stages + (NVFP4) one stage of scale columns.
+// Tensor-memory columns: accumulator stages + (NVFP4, MXFP4) one stage of scale columns, four per scale tile.
 template <int KIND, int BLOCK_N> struct TmemPlan {
-    static constexpr uint32_t kSfACols = KIND == kNvf4 ? 16 : 0;                        // 4 MMAs x 4 columns
-    static constexpr uint32_t kSfBCols = KIND == kNvf4 ? (BLOCK_N > 128 ? 32 : 16) : 0;
+    static constexpr uint32_t kSfACols = 4 * scale_tiles(KIND);
+    static constexpr uint32_t kSfBCols = (BLOCK_N > 128 ? 2 : 1) * kSfACols;
     static constexpr uint32_t kAccStages = (2 * BLOCK_N + kSfACols + kSfBCols <= 512) ? 2 : 1;
     // When two full accumulators do not fit beside the scale columns, two buffers that share their last /
     // first kOverlapCols columns are used: buffer 0 = [0, N), buffer 1 = [N - 64, 2N - 64).  The epilogue
@@ -421,6 +428,22 @@ __device__ __forceinline__ void silu_quantize_store64(const Params& p, const Til
     *reinterpret_cast<uint16_t*>(p.act_scales + base + tiled_scale_offset(row - t.group_row0, kb0, features)) = static_cast<uint16_t>(scale_pair);
 }
 
+// The same epilogue in MXFP4: 64 accumulator columns of one row are one 32-feature block, [32 gate, 32 up].  The f32 accumulators go
+// into SiLU as they are.
+__device__ __forceinline__ void mx_silu_quantize_store64(const Params& p, const TileCoord& t, uint32_t row, uint32_t c, const uint32_t* raw,
+                                                         float rs) {
+    const uint32_t features = p.group_cols / 2;
+    const uint32_t block = (t.out_col0 + c) / 64;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = mx::silu_mul(__uint_as_float(raw[i]) * rs, __uint_as_float(raw[32 + i]) * rs);
+    uint32_t words[4];
+    const uint32_t code = mx::quantize_block(v, words);
+    *reinterpret_cast<uint4*>(p.act_packed + static_cast<size_t>(row) * (features / 2) + block * 16) = make_uint4(words[0], words[1], words[2], words[3]);
+    const size_t base = ((static_cast<size_t>(t.group_row0) + 127) / 128 + t.group) * p.act_tile_bytes;
+    p.act_scales[base + mx::tiled_offset(row - t.group_row0, block, features / mx::kBlock)] = static_cast<uint8_t>(code);
+}
+
 // KIND: operand format.  BLOCK_N: column-operand rows per tile.  TRANSPOSED: output is
 // [col][row] (decode: rows are output features, columns are tokens).  TERMS: consecutive columns that
 // are summed (with their column scales) into one output column.  GROUPED: MoE schedule.
@@ -439,11 +462,13 @@ template <int KIND, int BLOCK_N, int STAGES, bool TRANSPOSED, int TERMS, bool GR
 __global__ void __launch_bounds__(64 + 32 * EPI_WARPS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_cols, const Params p,
             const __grid_constant__ ShortRows<GROUPED> short_rows) {
-    using L = SmemLayout<BLOCK_N>;
+    using L = SmemLayout<KIND, BLOCK_N>;
     using T = TmemPlan<KIND, BLOCK_N>;
-    constexpr bool kNv = KIND == kNvf4;
+    constexpr bool kNv = KIND != kFp8;                    // block-scaled FP4
+    constexpr uint32_t kSfTiles = scale_tiles(KIND);      // scale tiles per stage and 128 rows
+    constexpr uint32_t kSfStep = KIND == kMxf4 ? 2 : 1;   // MMAs that share a scale tile
     constexpr bool kActOnly = GROUPED && EPI_WARPS > 4;  // the kernels with the SiLU * up -> NVFP4 epilogue have no other
-    constexpr uint32_t kStage = L::stage_bytes(kNv);
+    constexpr uint32_t kStage = L::kStage;
     constexpr uint32_t kAcc = T::kAccStages;
     static_assert(BLOCK_N == 16 || BLOCK_N == 32 || BLOCK_N == 64 || BLOCK_N == 128 || BLOCK_N == 192 || BLOCK_N == 256, "BLOCK_N");
     static_assert(BLOCK_N % TERMS == 0, "TERMS must divide BLOCK_N");
@@ -510,8 +535,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant_
             for (uint32_t item = blockIdx.x; ok && get_tile<BLOCK_N, TERMS, GROUPED>(p, item, walker, t); item += gridDim.x) {
                 // scale tiles past the end of the column operand do not exist in memory: their rows are
                 // zero-filled by the TMA and their outputs are never stored, so the copy is skipped
-                const uint32_t sf_col_tiles = (p.cols + kTileRows - 1) / kTileRows;
-                const uint32_t sf_col_tile0 = t.col0 / kTileRows;
+                // (MXFP4 experts start on a scale tile of their own, whatever their number of rows; NVFP4's are multiples of 128)
+                constexpr bool kGroupTiles = GROUPED && KIND == kMxf4;
+                const uint32_t group_tiles = (p.group_cols + kTileRows - 1) / kTileRows;
+                const uint32_t sf_col_tiles = kGroupTiles ? p.groups * group_tiles : (p.cols + kTileRows - 1) / kTileRows;
+                const uint32_t sf_col_tile0 = kGroupTiles ? t.group * group_tiles + t.out_col0 / kTileRows : t.col0 / kTileRows;
                 bool second_sf = BLOCK_N > 128 && (sf_col_tile0 + 1 < sf_col_tiles);
                 const CUtensorMap* mrow = &map_rows;
                 const CUtensorMap* mcol = &map_cols;
@@ -550,24 +578,25 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant_
                 auto expect = [&](uint32_t s, uint32_t stage) {
                     const uint32_t kb = min(4u, (p.k_bytes - s * kStageBytesK + 31) / 32);  // MMAs in this stage
                     uint32_t bytes = row_bytes + L::kB;
-                    if (kNv) bytes += kb * kScaleTileBytes * (2 + (second_sf ? 1 : 0));
+                    if (kNv) bytes += scale_tiles_of<KIND>(kb) * kScaleTileBytes * (2 + (second_sf ? 1 : 0));
                     umma::mbar_arrive_expect_tx(&full[stage], bytes);
                     return kb;
                 };
                 auto load_rows = [&](uint32_t s, uint32_t stage, uint32_t kb) {
                     umma::tma_load_2d(smem_a + stage * L::kA, mrow, &full[stage], static_cast<int32_t>(s * kStageBytesK), row_coord);
                     if (kNv)
-                        umma::bulk_load_1d(smem_sfa + stage * L::kSfA, sf_row_ptr + static_cast<size_t>(s) * 4 * kScaleTileBytes, kb * kScaleTileBytes,
-                                           &full[stage]);
+                        umma::bulk_load_1d(smem_sfa + stage * L::kSfA, sf_row_ptr + static_cast<size_t>(s) * kSfTiles * kScaleTileBytes,
+                                           scale_tiles_of<KIND>(kb) * kScaleTileBytes, &full[stage]);
                 };
                 auto load_cols = [&](uint32_t s, uint32_t stage, uint32_t kb) {
-                    const size_t k_off = static_cast<size_t>(s) * 4 * kScaleTileBytes;
+                    const size_t k_off = static_cast<size_t>(s) * kSfTiles * kScaleTileBytes;
+                    const uint32_t sf_bytes = scale_tiles_of<KIND>(kb) * kScaleTileBytes;
                     umma::tma_load_2d(smem_b + stage * L::kB, mcol, &full[stage], static_cast<int32_t>(s * kStageBytesK), col_coord);
                     if (kNv) {
-                        umma::bulk_load_1d(smem_sfb + stage * L::kSfB, sf_col_ptr + k_off, kb * kScaleTileBytes, &full[stage]);
+                        umma::bulk_load_1d(smem_sfb + stage * L::kSfB, sf_col_ptr + k_off, sf_bytes, &full[stage]);
                         if (second_sf)
-                            umma::bulk_load_1d(smem_sfb + stage * L::kSfB + 4 * kScaleTileBytes, sf_col_ptr + p.sf_tile_stride + k_off,
-                                               kb * kScaleTileBytes, &full[stage]);
+                            umma::bulk_load_1d(smem_sfb + stage * L::kSfB + kSfTiles * kScaleTileBytes, sf_col_ptr + p.sf_tile_stride + k_off,
+                                               sf_bytes, &full[stage]);
                     }
                 };
                 uint32_t s = t.k_stage0;
@@ -605,7 +634,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant_
         // one elected lane issues the tcgen05 instructions.
         {
             const bool leader = umma::elect_one();
-            constexpr uint32_t idesc = kNv ? umma::idesc_nvf4(BLOCK_N) : umma::idesc_f8(BLOCK_N);
+            constexpr uint32_t idesc = KIND == kNvf4 ? umma::idesc_nvf4(BLOCK_N) : umma::idesc_f8(BLOCK_N);
             constexpr uint32_t kSfbStep = BLOCK_N > 128 ? 8 : 4;  // tensor-memory columns of column-operand scales per MMA
             const uint32_t a_lo0 = umma::desc_lo_sw128(umma::smem_u32(smem_a));
             const uint32_t b_lo0 = umma::desc_lo_sw128(umma::smem_u32(smem_b));
@@ -636,48 +665,38 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant_
                     const uint32_t sfa_lo = sfa_lo0 + stage * (L::kSfA >> 4);
                     const uint32_t sfb_lo = sfb_lo0 + stage * (L::kSfB >> 4);
                     const uint32_t first = (s > t.k_stage0) ? 1u : 0u;
+                    // scale tile i of the stage into its tensor-memory columns
+                    auto copy_scales = [&](uint32_t i) {
+                        umma::tc_copy_scales(sfa_tmem + i * 4, umma::make_desc(sfa_lo + i * 32, umma::kDescHiScales));
+                        umma::tc_copy_scales(sfb_tmem + i * kSfbStep, umma::make_desc(sfb_lo + i * 32, umma::kDescHiScales));
+                        if (BLOCK_N > 128)
+                            umma::tc_copy_scales(sfb_tmem + i * kSfbStep + 4, umma::make_desc(sfb_lo + (kSfTiles + i) * 32, umma::kDescHiScales));
+                    };
+                    auto mma = [&](uint32_t j, uint32_t accumulate) {
+                        const uint64_t a_desc = umma::make_desc(a_lo + j * 2, umma::kDescHiSw128);
+                        const uint64_t b_desc = umma::make_desc(b_lo + j * 2, umma::kDescHiSw128);
+                        const uint32_t sf = j / kSfStep;
+                        if constexpr (KIND == kNvf4)
+                            umma::mma_nvf4(d_tmem, a_desc, b_desc, idesc, sfa_tmem + sf * 4, sfb_tmem + sf * kSfbStep + sfb_sub, accumulate);
+                        else if constexpr (KIND == kMxf4)
+                            umma::mma_mxf4(d_tmem, a_desc, b_desc, umma::idesc_mxf4(BLOCK_N, j % kSfStep), sfa_tmem + sf * 4,
+                                           sfb_tmem + sf * kSfbStep + sfb_sub, accumulate);
+                        else
+                            umma::mma_f8(d_tmem, a_desc, b_desc, idesc, accumulate);
+                    };
                     if (!leader) {
                         // nothing to issue
                     } else if (s + 1 < p.k_stages || tail_kb == 4) {
                         if (kNv) {
 #pragma unroll
-                            for (uint32_t j = 0; j < 4; ++j) {
-                                umma::tc_copy_scales(sfa_tmem + j * 4, umma::make_desc(sfa_lo + j * 32, umma::kDescHiScales));
-                                umma::tc_copy_scales(sfb_tmem + j * kSfbStep, umma::make_desc(sfb_lo + j * 32, umma::kDescHiScales));
-                                if (BLOCK_N > 128)
-                                    umma::tc_copy_scales(sfb_tmem + j * kSfbStep + 4,
-                                                         umma::make_desc(sfb_lo + (4 + j) * 32, umma::kDescHiScales));
-                            }
+                            for (uint32_t i = 0; i < kSfTiles; ++i) copy_scales(i);
                         }
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) {
-                            const uint64_t a_desc = umma::make_desc(a_lo + j * 2, umma::kDescHiSw128);
-                            const uint64_t b_desc = umma::make_desc(b_lo + j * 2, umma::kDescHiSw128);
-                            if (kNv)
-                                umma::mma_nvf4(d_tmem, a_desc, b_desc, idesc, sfa_tmem + j * 4, sfb_tmem + j * kSfbStep + sfb_sub,
-                                               j == 0 ? first : 1u);
-                            else
-                                umma::mma_f8(d_tmem, a_desc, b_desc, idesc, j == 0 ? first : 1u);
-                        }
+                        for (uint32_t j = 0; j < 4; ++j) mma(j, j == 0 ? first : 1u);
                     } else {  // last stage of a K that is not a multiple of the stage depth
-                        for (uint32_t j = 0; j < tail_kb; ++j) {
-                            if (kNv) {
-                                umma::tc_copy_scales(sfa_tmem + j * 4, umma::make_desc(sfa_lo + j * 32, umma::kDescHiScales));
-                                umma::tc_copy_scales(sfb_tmem + j * kSfbStep, umma::make_desc(sfb_lo + j * 32, umma::kDescHiScales));
-                                if (BLOCK_N > 128)
-                                    umma::tc_copy_scales(sfb_tmem + j * kSfbStep + 4,
-                                                         umma::make_desc(sfb_lo + (4 + j) * 32, umma::kDescHiScales));
-                            }
-                        }
-                        for (uint32_t j = 0; j < tail_kb; ++j) {
-                            const uint64_t a_desc = umma::make_desc(a_lo + j * 2, umma::kDescHiSw128);
-                            const uint64_t b_desc = umma::make_desc(b_lo + j * 2, umma::kDescHiSw128);
-                            if (kNv)
-                                umma::mma_nvf4(d_tmem, a_desc, b_desc, idesc, sfa_tmem + j * 4, sfb_tmem + j * kSfbStep + sfb_sub,
-                                               j == 0 ? first : 1u);
-                            else
-                                umma::mma_f8(d_tmem, a_desc, b_desc, idesc, j == 0 ? first : 1u);
-                        }
+                        if (kNv)
+                            for (uint32_t i = 0; i < scale_tiles_of<KIND>(tail_kb); ++i) copy_scales(i);
+                        for (uint32_t j = 0; j < tail_kb; ++j) mma(j, j == 0 ? first : 1u);
                     }
                     if (leader) umma::tc_commit(&empty[stage]);  // frees the stage once these MMAs (and scale copies) retire
                     __syncwarp();
@@ -749,7 +768,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant_
                         __syncwarp();
                         if (lane == 0) umma::mbar_arrive(&acc_empty[acc]);
                     }
-                    if (row_ok && !empty_tile) silu_quantize_store64(p, t, row, c, raw, rs);
+                    if constexpr (KIND == kMxf4) {
+                        // (a tile may hang over the expert's last weight row, by whole blocks)
+                        if (row_ok && t.out_col0 + c < p.group_cols) mx_silu_quantize_store64(p, t, row, c, raw, rs);
+                    } else {
+                        if (row_ok && !empty_tile) silu_quantize_store64(p, t, row, c, raw, rs);
+                    }
                 }
             } else {
                 if constexpr (kWide) if (wide) {

@@ -559,10 +559,11 @@ __global__ void moe_pointer_tables_kernel(const uint32_t* __restrict__ offsets, 
 // at once and added in slot order; AHEAD divides the slot count, as a test per slot keeps the loads apart, and few slots need the
 // registers for more CTAs instead.  4096 rows of 2048: 4 slots 13.9 us = 6.0 TB/s, 8 slots 26.4 us; a CTA per row with eight slots
 // ahead whatever their count took 17.8 and 27.5 us, and 4.7 us for rows of 128 (now 2.1 to 2.4).
-template <uint32_t AHEAD>
+// T: f32 sums as they are, or rounded once to bf16 (uint16_t).
+template <uint32_t AHEAD, typename T>
 __global__ void __launch_bounds__(256, AHEAD <= 3 ? 8 : AHEAD <= 5 ? 6 : AHEAD <= 7 ? 5 : 4)
 moe_combine_kernel(const uint32_t* __restrict__ route_to_sorted, const float* __restrict__ route_weights,
-                   const uint16_t* __restrict__ sorted_inputs, float* __restrict__ output, uint32_t rows, uint32_t len,
+                   const uint16_t* __restrict__ sorted_inputs, T* __restrict__ output, uint32_t rows, uint32_t len,
                    uint32_t routes_per_row) {
     griddep_begin();
     const uint32_t vec_per_row = len / 8;
@@ -589,15 +590,25 @@ moe_combine_kernel(const uint32_t* __restrict__ route_to_sorted, const float* __
             }
         }
     }
-    float4* dst = reinterpret_cast<float4*>(output + static_cast<size_t>(row) * len + v * 8);
-    dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    T* out = output + static_cast<size_t>(row) * len + v * 8;
+    if constexpr (sizeof(T) == 4) {
+        float4* dst = reinterpret_cast<float4*>(out);
+        dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    } else {
+        uint32_t words[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            words[j] = float_to_bf16_bits(acc[2 * j]) | static_cast<uint32_t>(float_to_bf16_bits(acc[2 * j + 1])) << 16;
+        *reinterpret_cast<uint4*>(out) = make_uint4(words[0], words[1], words[2], words[3]);
+    }
 }
 
+template <typename T>
 __global__ void __launch_bounds__(256) moe_combine_scalar_kernel(const uint32_t* __restrict__ route_to_sorted,
                                                                  const float* __restrict__ route_weights,
                                                                  const uint16_t* __restrict__ sorted_inputs,
-                                                                 float* __restrict__ output, uint32_t rows, uint32_t len,
+                                                                 T* __restrict__ output, uint32_t rows, uint32_t len,
                                                                  uint32_t routes_per_row) {
     griddep_begin();
     const size_t idx = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -609,7 +620,35 @@ __global__ void __launch_bounds__(256) moe_combine_scalar_kernel(const uint32_t*
         sum = fmaf(bf16_bits_to_float(sorted_inputs[static_cast<size_t>(route_to_sorted[route]) * len + col]),
                    route_weights[route], sum);
     }
-    output[idx] = sum;
+    if constexpr (sizeof(T) == 4) output[idx] = sum;
+    else output[idx] = float_to_bf16_bits(sum);
+}
+
+template <typename T>
+cudaError_t combine(const uint32_t* route_to_sorted, const float* route_weights, const uint16_t* sorted_inputs, T* output, uint32_t rows, uint32_t len,
+                    uint32_t routes_per_row, cudaStream_t stream) {
+    if (!route_to_sorted || !route_weights || !sorted_inputs || !output || rows == 0 || len == 0 || routes_per_row == 0)
+        return cudaErrorInvalidValue;
+    const bool vec = len % 8 == 0 && (reinterpret_cast<uintptr_t>(sorted_inputs) & 15) == 0 &&
+                     (reinterpret_cast<uintptr_t>(output) & 15) == 0;
+    const uint64_t units = static_cast<uint64_t>(rows) * (len / 8);
+    if (vec && units <= 0xffffff00u) {
+        uint32_t ahead = 8;
+        while (routes_per_row % ahead != 0) --ahead;
+        auto kernel = ahead == 8   ? moe_combine_kernel<8, T>
+                      : ahead == 7 ? moe_combine_kernel<7, T>
+                      : ahead == 6 ? moe_combine_kernel<6, T>
+                      : ahead == 5 ? moe_combine_kernel<5, T>
+                      : ahead == 4 ? moe_combine_kernel<4, T>
+                      : ahead == 3 ? moe_combine_kernel<3, T>
+                      : ahead == 2 ? moe_combine_kernel<2, T>
+                                   : moe_combine_kernel<1, T>;
+        return launch_dependent(kernel, dim3(static_cast<uint32_t>((units + 255) / 256)), 256, 0, stream, route_to_sorted, route_weights,
+                                sorted_inputs, output, rows, len, routes_per_row);
+    }
+    const size_t total = static_cast<size_t>(rows) * len;
+    return launch_dependent(moe_combine_scalar_kernel<T>, dim3(static_cast<uint32_t>((total + 255) / 256)), 256, 0, stream, route_to_sorted,
+                            route_weights, sorted_inputs, output, rows, len, routes_per_row);
 }
 
 }  // namespace
@@ -898,28 +937,13 @@ cudaError_t infer_moe_weighted_accumulate_sorted_bf16_batch_on_stream(const uint
                                                                       const uint16_t* sorted_inputs, float* output,
                                                                       uint32_t rows, uint32_t len, uint32_t routes_per_row,
                                                                       cudaStream_t stream) {
-    if (!route_to_sorted || !route_weights || !sorted_inputs || !output || rows == 0 || len == 0 || routes_per_row == 0)
-        return cudaErrorInvalidValue;
-    const bool vec = len % 8 == 0 && (reinterpret_cast<uintptr_t>(sorted_inputs) & 15) == 0 &&
-                     (reinterpret_cast<uintptr_t>(output) & 15) == 0;
-    const uint64_t units = static_cast<uint64_t>(rows) * (len / 8);
-    if (vec && units <= 0xffffff00u) {
-        uint32_t ahead = 8;
-        while (routes_per_row % ahead != 0) --ahead;
-        auto kernel = ahead == 8   ? moe_combine_kernel<8>
-                      : ahead == 7 ? moe_combine_kernel<7>
-                      : ahead == 6 ? moe_combine_kernel<6>
-                      : ahead == 5 ? moe_combine_kernel<5>
-                      : ahead == 4 ? moe_combine_kernel<4>
-                      : ahead == 3 ? moe_combine_kernel<3>
-                      : ahead == 2 ? moe_combine_kernel<2>
-                                   : moe_combine_kernel<1>;
-        return launch_dependent(kernel, dim3(static_cast<uint32_t>((units + 255) / 256)), 256, 0, stream, route_to_sorted, route_weights,
-                                sorted_inputs, output, rows, len, routes_per_row);
-    }
-    const size_t total = static_cast<size_t>(rows) * len;
-    return launch_dependent(moe_combine_scalar_kernel, dim3(static_cast<uint32_t>((total + 255) / 256)), 256, 0, stream, route_to_sorted,
-                            route_weights, sorted_inputs, output, rows, len, routes_per_row);
+    return combine(route_to_sorted, route_weights, sorted_inputs, output, rows, len, routes_per_row, stream);
+}
+
+cudaError_t eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream(const uint32_t* route_to_sorted, const float* route_weights,
+                                                                        const uint16_t* sorted_inputs, uint16_t* output, uint32_t rows,
+                                                                        uint32_t len, uint32_t routes_per_row, cudaStream_t stream) {
+    return combine(route_to_sorted, route_weights, sorted_inputs, output, rows, len, routes_per_row, stream);
 }
 
 cudaError_t eider_b200_moe_quantize_routes_on_stream(const void* input, int input_is_bf16, const uint32_t* route_to_sorted,

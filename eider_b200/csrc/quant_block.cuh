@@ -1,4 +1,5 @@
-// A 16-element block of a row in registers and its quotients: shared by the activation quantizers and the routed-MoE ones.
+// A 16-element block of a row in registers and its quotients, and the padding of the scales: shared by the activation quantizers and
+// the routed-MoE ones.
 #pragma once
 
 #include "common.cuh"
@@ -134,6 +135,29 @@ template <typename T> __device__ __forceinline__ uint8_t quantize_unit_block(con
         for (int j = 0; j < 8; ++j) w[j / 4] |= e2m1_byte(div2_negated(v.minus_pair(j), d2, r2)) << ((j % 4) * 8);
     }
     return sc;
+}
+
+// PADDING of the tiled scale layout: a GEMM copies whole tiles, so the rows behind the last one up to a whole 128-row tile and
+// the blocks of a row behind its last one up to a group of four have to be zero.  The quantizers write it only where they are
+// told to (`pad`, the *_padded_on_stream entry points): to the others a scale buffer is the caller's, who may keep other rows
+// of the same tile in it.  The blocks are zeroed by the row's own CTA, the rows by all `threads` threads of the grid here, in the
+// 16-byte units of the layout (the four bytes of rows l, l + 32, l + 64 and l + 96): one row of 5120 elements leaves 39 KB to
+// zero, which took its single CTA 12 us byte by byte and takes it less than 1 us so.
+__device__ __forceinline__ void zero_padding_rows(uint8_t* scales, uint32_t rows, uint32_t k, uint32_t thread, uint32_t threads) {
+    const uint32_t first = rows % 128;
+    if (first == 0) return;
+    const uint32_t units = (k + 63) / 64 * 32;
+    uint4* tile = reinterpret_cast<uint4*>(scales + static_cast<size_t>(rows / 128) * units * 16);
+    for (uint32_t u = thread; u < units; u += threads) {
+        const uint32_t l = u & 31;
+        if (l >= first) {
+            tile[u] = make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (uint32_t q = 1; q < 4; ++q)
+                if (q * 32 + l >= first) reinterpret_cast<uint32_t*>(tile + u)[q] = 0;
+        }
+    }
 }
 
 // A kernel that starts with griddepcontrol.wait, launched so that its prologue overlaps the kernel before it.

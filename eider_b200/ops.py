@@ -352,6 +352,261 @@ class Fp8TnMatmulPlan:
             pass
 
 
+# ---- MXFP4 ------------------------------------------------------------------------------------------
+def _call(device: torch.device, name: str, *args) -> None:
+    """One entry point on the current stream of `device` (the device of its tensors, whichever is current)."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == device.index:
+        check(name, fn(*args, _stream()))
+    else:
+        with torch.cuda.device(device):
+            check(name, fn(*args, _stream()))
+
+
+def _need_floats(t: torch.Tensor, label: str) -> None:
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise ShapeError(f"{label} must be f32 or bf16, got {t.dtype}")
+    _need(t, t.dtype, label)
+
+
+def _need_device(device: torch.device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ShapeError(f"operands are on {t.device} and {device}")
+
+
+def _aligned16(t: torch.Tensor) -> torch.Tensor:
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def mxfp4_scale_layout_len(outer: int, inner: int) -> int:
+    """Bytes of the tiled E8M0 scales of an [outer, inner] matrix: 128-row x 4-block tiles, a block being 32 elements."""
+    return (outer + 127) // 128 * 128 * (((inner + 31) // 32 + 3) // 4 * 4)
+
+
+@dataclass
+class Mxfp4Matrix:
+    """Device MXFP4 matrix: packed E2M1 [rows, K/2] + tiled E8M0 scales, one per 32 elements."""
+    packed: torch.Tensor
+    scales: torch.Tensor
+    rows: int
+    k: int
+
+    @staticmethod
+    def _unwritten(rows: int, k: int, device) -> "Mxfp4Matrix":
+        """Storage for a quantizer, which writes all of it (zero scales for padding rows and blocks included)."""
+        if k % 32 != 0 or k == 0 or rows == 0:
+            raise ShapeError(f"MXFP4 needs rows of whole 32-element blocks, got [{rows}, {k}]")
+        return Mxfp4Matrix(torch.empty(rows, k // 2, dtype=torch.uint8, device=device),
+                           torch.empty(mxfp4_scale_layout_len(rows, k), dtype=torch.uint8, device=device), rows, k)
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The values the codes stand for, [rows, K] f32 or bf16 (both hold every E2M1 multiple of a block scale exactly)."""
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ShapeError(f"values are f32 or bf16, got {dtype}")
+        out = torch.empty(self.rows, self.k, dtype=dtype, device=self.packed.device)
+        _call(out.device, "eider_b200_dequantize_mxfp4_on_stream", self.packed.data_ptr(), self.scales.data_ptr(), out.data_ptr(),
+              int(dtype == torch.bfloat16), self.rows, self.k)
+        return out
+
+
+def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Matrix:
+    """Activation rows [tokens, K] (f32 or bf16; rows may be apart, elements not) -> MXFP4: per block of 32 the scale
+    2^(floor(log2 amax) - 2), codes to nearest even, saturating at 6.  A block with a NaN or an infinity stands for NaN."""
+    if x.dim() != 2 or not x.is_cuda or x.dtype not in (torch.float32, torch.bfloat16) or x.stride(1) != 1:
+        raise ShapeError("activation must be a CUDA matrix of f32 or bf16 with contiguous rows")
+    tokens, k = x.shape
+    stride = x.stride(0) if tokens > 1 else k
+    if stride < k:
+        raise ShapeError("activation rows overlap")
+    out = Mxfp4Matrix._unwritten(tokens, k, x.device)
+    _call(x.device, "eider_b200_quantize_mxfp4_on_stream", x.data_ptr(), int(x.dtype == torch.bfloat16), stride, out.packed.data_ptr(),
+          out.scales.data_ptr(), tokens, k)
+    return out
+
+
+def silu_mul_halves_quantize_mxfp4(gate_up: torch.Tensor) -> Mxfp4Matrix:
+    """Fused SiLU(gate) * up -> MXFP4 of [tokens, 2K] f32 rows (gate half first)."""
+    if gate_up.dim() != 2 or gate_up.shape[1] % 64 != 0:
+        raise ShapeError("gate_up must be [tokens, 2 * intermediate] with an intermediate size in multiples of 32")
+    _need(gate_up, torch.float32, "gate_up")
+    gate_up = _aligned16(gate_up)
+    out = Mxfp4Matrix._unwritten(gate_up.shape[0], gate_up.shape[1] // 2, gate_up.device)
+    _call(gate_up.device, "eider_b200_silu_mul_halves_quantize_mxfp4_on_stream", gate_up.data_ptr(), out.packed.data_ptr(), out.scales.data_ptr(),
+          out.rows, out.k)
+    return out
+
+
+def _mxfp4_tiled(scales_row_major: torch.Tensor, groups: int, rows: int, k: int) -> torch.Tensor:
+    tiled = torch.empty(groups * mxfp4_scale_layout_len(rows, k), dtype=torch.uint8, device=scales_row_major.device)
+    _call(tiled.device, "eider_b200_mxfp4_scales_to_tiled_on_stream", scales_row_major.data_ptr(), tiled.data_ptr(), groups, rows, k)
+    return tiled
+
+
+@dataclass
+class Mxfp4Weight:
+    """Device MXFP4 weight: the checkpoint's packed bytes as they are, its E8M0 scales in tiles for the tensor-core GEMM and in
+    rows padded to 16 bytes for the decode product."""
+    packed: torch.Tensor            # [N, K/2] u8
+    scales_row_major: torch.Tensor  # [N, K/32] u8 (checkpoint layout)
+    scales_tiled: torch.Tensor
+    scales_rows: torch.Tensor       # [N, K/32 up to a multiple of 16], zeros behind the blocks
+    out_features: int
+    in_features: int
+
+    @staticmethod
+    def from_checkpoint(packed: torch.Tensor, scales_row_major: torch.Tensor) -> "Mxfp4Weight":
+        if packed.dim() != 2 or packed.shape[1] % 16 != 0 or packed.numel() == 0:
+            raise ShapeError(f"MXFP4 weight bytes must be [out, in / 2] with in % 32 == 0, got {tuple(packed.shape)}")
+        n, k = packed.shape[0], packed.shape[1] * 2
+        if scales_row_major.shape != (n, k // 32):
+            raise ShapeError(f"MXFP4 scales must be [{n}, {k // 32}], got {tuple(scales_row_major.shape)}")
+        _need(packed, torch.uint8, "weight")
+        _need(scales_row_major, torch.uint8, "weight scales")
+        _need_device(packed.device, scales_row_major)
+        rows = torch.zeros(n, (k // 32 + 15) // 16 * 16, dtype=torch.uint8, device=packed.device)
+        rows[:, : k // 32] = scales_row_major
+        return Mxfp4Weight(_aligned16(packed), scales_row_major, _mxfp4_tiled(scales_row_major, 1, n, k), rows, n, k)
+
+    @staticmethod
+    def quantize(weight: torch.Tensor) -> "Mxfp4Weight":
+        """Quantize a dense [N, K] f32/bf16 weight, block by block as quantize_mxfp4 does."""
+        if weight.dim() != 2 or weight.shape[1] % 32 != 0 or weight.numel() == 0:
+            raise ShapeError(f"MXFP4 needs [N, K] with K % 32 == 0, got {tuple(weight.shape)}")
+        _need_floats(weight, "weight")
+        n, k = weight.shape
+        packed = torch.empty(n, k // 2, dtype=torch.uint8, device=weight.device)
+        scales = torch.empty(n, k // 32, dtype=torch.uint8, device=weight.device)
+        _call(weight.device, "eider_b200_quantize_mxfp4_weight_on_stream", weight.data_ptr(), int(weight.dtype == torch.bfloat16),
+              packed.data_ptr(), scales.data_ptr(), n, k)
+        return Mxfp4Weight.from_checkpoint(packed, scales)
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        return Mxfp4Matrix(self.packed, self.scales_tiled, self.out_features, self.in_features).dequantize(dtype)
+
+
+class _DevicePlan:
+    """A plan handle of the library and the device it was made on."""
+    _destroy = ""
+
+    def _make(self, create: str, what: str, *shape) -> None:
+        self._lib = _lib.load()
+        self._plan = None
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._plan = getattr(self._lib, create)(*shape)
+        if not self._plan:
+            raise ShapeError(f"unsupported {what}")
+
+    def _output(self, out: torch.Tensor | None, shape, dtype, beta: float, c: torch.Tensor | None):
+        """The output and C, checked: C has the output's shape and type, and is the output itself unless given."""
+        if out is None:
+            if dtype not in (torch.float32, torch.bfloat16):
+                raise ShapeError(f"output must be f32 or bf16, got {dtype}")
+            out = torch.empty(shape, dtype=dtype, device=self.device)
+        elif tuple(out.shape) != tuple(shape):
+            raise ShapeError(f"output must be {tuple(shape)}, got {tuple(out.shape)}")
+        _need_floats(out, "output")
+        if beta != 0.0:
+            c = out if c is None else c
+            if c.shape != out.shape or c.dtype != out.dtype:
+                raise ShapeError("C must have the output's shape and type")
+            _need(c, c.dtype, "C")
+        else:
+            c = None
+        _need_device(self.device, out, c)
+        return out, c
+
+    def close(self) -> None:
+        if self._plan:
+            getattr(self._lib, self._destroy)(self._plan)
+            self._plan = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Mxfp4MatmulPlan(_DevicePlan):
+    """Dense MXFP4 W4A4 GEMM: D = alpha * X . W^T + beta * C with fp32 accumulation, bf16 or f32 output [tokens, out_features]."""
+    _destroy = "eider_b200_mxfp4_gemm_tn_destroy"
+
+    def __init__(self, tokens: int, out_features: int, in_features: int):
+        self.m, self.n, self.k = tokens, out_features, in_features
+        self._make("eider_b200_mxfp4_gemm_tn_create", f"MXFP4 GEMM shape m={tokens} n={out_features} k={in_features}", tokens, out_features,
+                   in_features)
+
+    @property
+    def block_n(self) -> int:
+        """Tile code in use, as for Fp4TnMatmulPlan."""
+        return int(self._lib.eider_b200_gemm_plan_block_n(self._plan))
+
+    def set_block_n(self, block_n: int) -> None:
+        if not self._lib.eider_b200_gemm_plan_set_block_n(self._plan, block_n):
+            raise ShapeError(f"block_n must be 64, 128, 192, 256, 512 (CTA pairs, 256 x 256) or 384 (CTA pairs, 256 x 192), got {block_n}")
+
+    def _operands(self, x: Mxfp4Matrix, w: Mxfp4Weight) -> None:
+        if x.rows != self.m or x.k != self.k or w.out_features != self.n or w.in_features != self.k:
+            raise ShapeError("operand shapes do not match the plan")
+        _need_device(self.device, x.packed, w.packed)
+
+    def run(self, x: Mxfp4Matrix, w: Mxfp4Weight, out: torch.Tensor | None = None, alpha: float = 1.0, beta: float = 0.0,
+            c: torch.Tensor | None = None, out_dtype=torch.bfloat16) -> torch.Tensor:
+        self._operands(x, w)
+        out, c = self._output(out, (self.m, self.n), out_dtype, beta, c)
+        _call(self.device, "eider_b200_mxfp4_gemm_tn_on_stream", self._plan, x.packed.data_ptr(), x.scales.data_ptr(), w.packed.data_ptr(),
+              w.scales_tiled.data_ptr(), _ptr(c), out.data_ptr(), alpha, beta, int(out.dtype == torch.bfloat16))
+        return out
+
+    def run_silu_quantize(self, x: Mxfp4Matrix, w: Mxfp4Weight, alpha: float = 1.0) -> Mxfp4Matrix:
+        """Gate/up GEMM with SiLU(gate) * up -> MXFP4 in its epilogue: `w` is [2 * intermediate, in_features], gate rows first,
+        intermediate a multiple of 128; the result is the down projection's input [tokens, intermediate]."""
+        self._operands(x, w)
+        if self.n % 256 != 0:
+            raise ShapeError("the intermediate size must be a multiple of 128")
+        out = Mxfp4Matrix._unwritten(self.m, self.n // 2, self.device)
+        _call(self.device, "eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream", self._plan, x.packed.data_ptr(), x.scales.data_ptr(),
+              w.packed.data_ptr(), w.scales_tiled.data_ptr(), alpha, out.packed.data_ptr(), out.scales.data_ptr())
+        return out
+
+    def status(self) -> int:
+        v = C.c_uint32(0)
+        check("eider_b200_gemm_plan_status", self._lib.eider_b200_gemm_plan_status(self._plan, C.byref(v)))
+        return v.value
+
+
+class Mxfp4DecodePlan(_DevicePlan):
+    """W4A16 decode linear over MXFP4 weights: y[t] = W . x[t] for up to 64 tokens, the weights streamed once, x as it is (bf16 or
+    f32).  The plan keeps nothing between calls: calls on several streams and captured graphs may overlap."""
+    _destroy = "eider_b200_mxfp4_decode_destroy"
+
+    def __init__(self, max_tokens: int, out_features: int, in_features: int):
+        self.max_tokens, self.n, self.k = max_tokens, out_features, in_features
+        self._make("eider_b200_mxfp4_decode_create", f"decode shape tokens<={max_tokens} n={out_features} k={in_features}", max_tokens,
+                   out_features, in_features)
+
+    def run(self, x: torch.Tensor, w: Mxfp4Weight, out: torch.Tensor | None = None, beta: float = 0.0, c: torch.Tensor | None = None,
+            out_dtype=torch.bfloat16) -> torch.Tensor:
+        if x.dim() == 1:
+            x = x.unsqueeze(0)
+        if x.dim() != 2 or x.shape[1] != self.k or w.in_features != self.k or w.out_features != self.n or not 0 < x.shape[0] <= self.max_tokens:
+            raise ShapeError("operand shapes do not match the plan")
+        _need_floats(x, "activation")
+        x = _aligned16(x)
+        _need_device(self.device, x, w.packed)
+        out, c = self._output(out, (x.shape[0], self.n), out_dtype, beta, c)
+        _call(self.device, "eider_b200_mxfp4_w4a16_gemv_on_stream", self._plan, x.data_ptr(), int(x.dtype == torch.bfloat16), x.shape[0],
+              w.packed.data_ptr(), w.scales_rows.data_ptr(), w.scales_rows.shape[1], _ptr(c), out.data_ptr(), beta,
+              int(out.dtype == torch.bfloat16))
+        return out
+
+    def status(self) -> int:
+        v = C.c_uint32(0)
+        check("eider_b200_mxfp4_decode_status", self._lib.eider_b200_mxfp4_decode_status(self._plan, C.byref(v)))
+        return v.value
+
+
 # ---- FP8 quantizers ---------------------------------------------------------------------------------
 def quantize_fp8_dynamic(x: torch.Tensor):
     """Per-token dynamic E4M3: returns (codes [rows, cols] u8, scales [rows] f32)."""
@@ -882,15 +1137,134 @@ class Fp4GroupedGemmPlan:
             pass
 
 
+@dataclass
+class GroupedMxfp4Weights:
+    """Stacked per-expert MXFP4 weights [E, N, K/2] with every expert's scales on 128-row tiles of their own."""
+    packed: torch.Tensor
+    scales_row_major: torch.Tensor  # [E, N, K/32]
+    scales_tiled: torch.Tensor
+    alpha: torch.Tensor             # [E] f32, what an expert's results are multiplied by
+    experts: int
+    out_features: int
+    in_features: int
+
+    @staticmethod
+    def from_checkpoint(packed: torch.Tensor, scales_row_major: torch.Tensor, alpha: torch.Tensor | None = None) -> "GroupedMxfp4Weights":
+        if packed.dim() != 3 or packed.shape[1] % 32 != 0 or packed.shape[2] % 16 != 0 or packed.numel() == 0:
+            raise ShapeError(f"expert weights must be [experts, out, in / 2] with out and in in multiples of 32, got {tuple(packed.shape)}")
+        e, n, k = packed.shape[0], packed.shape[1], packed.shape[2] * 2
+        if scales_row_major.shape != (e, n, k // 32):
+            raise ShapeError(f"MXFP4 scales must be [{e}, {n}, {k // 32}], got {tuple(scales_row_major.shape)}")
+        _need(packed, torch.uint8, "weight")
+        _need(scales_row_major, torch.uint8, "weight scales")
+        alpha = torch.ones(e, dtype=torch.float32, device=packed.device) if alpha is None else alpha.to(torch.float32).contiguous()
+        if alpha.shape != (e,):
+            raise ShapeError("alpha must have one value per expert")
+        _need_device(packed.device, scales_row_major, alpha)
+        return GroupedMxfp4Weights(_aligned16(packed), scales_row_major, _mxfp4_tiled(scales_row_major, e, n, k), alpha, e, n, k)
+
+    def interleave_gate_up(self) -> "GroupedMxfp4Weights":
+        """The same gate/up weights with the rows of every expert reordered as [32 gate rows, 32 up rows] per 32 features: 64
+        consecutive output columns are one MXFP4 block of both halves, which the GEMM's epilogue turns into SiLU * up.  Done
+        once at load."""
+        n = self.out_features
+        if n % 64 != 0:
+            raise ShapeError("gate/up rows must come in multiples of 64")
+        order = torch.arange(n, device=self.packed.device).reshape(2, -1, 32).transpose(0, 1).reshape(-1)
+        return GroupedMxfp4Weights.from_checkpoint(self.packed.index_select(1, order).contiguous(),
+                                                   self.scales_row_major.index_select(1, order).contiguous(), self.alpha)
+
+    @staticmethod
+    def quantize(weights: torch.Tensor) -> "GroupedMxfp4Weights":
+        """[E, N, K] f32/bf16, block by block."""
+        e, n, k = weights.shape
+        flat = Mxfp4Weight.quantize(weights.reshape(e * n, k).contiguous())
+        return GroupedMxfp4Weights.from_checkpoint(flat.packed.reshape(e, n, -1), flat.scales_row_major.reshape(e, n, -1))
+
+
+class MoeSortedMxfp4Rows:
+    """Expert-major MXFP4 rows with per-expert 128-row scale tiles: MoeSortedNvfp4Rows with blocks of 32."""
+
+    def __init__(self, routes: int, experts: int, k: int, device="cuda"):
+        if k % 32 != 0 or k == 0:
+            raise ShapeError(f"MXFP4 needs K % 32 == 0, got {k}")
+        self.routes, self.experts, self.k = routes, experts, k
+        self.tile_bytes = 128 * ((k // 32 + 3) // 4 * 4)
+        self.packed = torch.zeros(routes, k // 2, dtype=torch.uint8, device=device)
+        # (zeroed: the GEMM's epilogue leaves the padding blocks of a row alone)
+        self.scales = torch.zeros(((routes + 127) // 128 + experts) * self.tile_bytes, dtype=torch.uint8, device=device)
+
+    def quantize_routes(self, x: torch.Tensor, routes: MoeSortedRoutes, routes_per_row: int) -> "MoeSortedMxfp4Rows":
+        """Every token's row, quantized once, at the place of each of its routes."""
+        if x.dim() != 2 or x.shape[1] != self.k or x.shape[0] * routes_per_row != self.routes or routes.routes != self.routes or routes_per_row > 64:
+            raise ShapeError("input does not match the buffer (at most 64 routes a row)")
+        _need_floats(x, "input")
+        x = _aligned16(x)
+        _need_device(self.packed.device, x, routes.sorted_routes)
+        _call(x.device, "eider_b200_moe_quantize_routes_mxfp4_on_stream", x.data_ptr(), int(x.dtype == torch.bfloat16),
+              routes.route_to_sorted.data_ptr(), routes.sorted_routes.data_ptr(), routes.sorted_experts.data_ptr(), routes.expert_offsets.data_ptr(),
+              self.packed.data_ptr(), self.scales.data_ptr(), x.shape[0], routes_per_row, self.k, self.tile_bytes)
+        return self
+
+
+class Mxfp4GroupedGemmPlan(_DevicePlan):
+    """Experts' products in MXFP4: per expert D_e = alpha_e * X_e . W_e^T, bf16 [route, m], token counts stay on the device."""
+    _destroy = "eider_b200_mxfp4_grouped_gemm_destroy"
+
+    def __init__(self, m: int, max_n: int, k: int, groups: int):
+        self.m, self.max_n, self.k, self.groups = m, max_n, k, groups
+        self._make("eider_b200_mxfp4_grouped_gemm_create", f"grouped MXFP4 GEMM m={m} k={k} groups={groups}", m, max_n, k, groups)
+
+    def _operands(self, rows: MoeSortedMxfp4Rows, w: GroupedMxfp4Weights, routes: MoeSortedRoutes) -> None:
+        if (rows.k != self.k or w.in_features != self.k or w.out_features != self.m or w.experts != self.groups or rows.experts != self.groups or
+                routes.experts != self.groups or routes.routes != rows.routes):
+            raise ShapeError("operand shapes do not match the plan")
+        _need_device(self.device, rows.packed, w.packed, routes.expert_offsets)
+
+    def run(self, rows: MoeSortedMxfp4Rows, w: GroupedMxfp4Weights, routes: MoeSortedRoutes, out: torch.Tensor | None = None) -> torch.Tensor:
+        self._operands(rows, w, routes)
+        out, _ = self._output(out, (rows.routes, self.m), torch.bfloat16, 0.0, None)
+        _need(out, torch.bfloat16, "output")
+        _call(self.device, "eider_b200_mxfp4_grouped_gemm_on_stream", self._plan, rows.packed.data_ptr(), rows.scales.data_ptr(), w.packed.data_ptr(),
+              w.scales_tiled.data_ptr(), out.data_ptr(), w.alpha.data_ptr(), routes.expert_offsets.data_ptr(), rows.routes)
+        return out
+
+    def run_silu_quantize(self, rows: MoeSortedMxfp4Rows, w_interleaved: GroupedMxfp4Weights, routes: MoeSortedRoutes,
+                          out: MoeSortedMxfp4Rows) -> MoeSortedMxfp4Rows:
+        """Gate/up GEMM with SiLU(gate) * up -> MXFP4 in the epilogue: fills `out`, the down projection's input.  `w_interleaved` =
+        GroupedMxfp4Weights.interleave_gate_up()."""
+        self._operands(rows, w_interleaved, routes)
+        if out.k * 2 != self.m or out.routes != rows.routes or out.experts != rows.experts:
+            raise ShapeError("operand shapes do not match the plan")
+        _need_device(self.device, out.packed)
+        _call(self.device, "eider_b200_mxfp4_grouped_gemm_silu_quantize_on_stream", self._plan, rows.packed.data_ptr(), rows.scales.data_ptr(),
+              w_interleaved.packed.data_ptr(), w_interleaved.scales_tiled.data_ptr(), w_interleaved.alpha.data_ptr(),
+              routes.expert_offsets.data_ptr(), rows.routes, out.packed.data_ptr(), out.scales.data_ptr(), out.tile_bytes)
+        return out
+
+    def status(self) -> int:
+        v = C.c_uint32(0)
+        check("eider_b200_grouped_plan_status", self._lib.eider_b200_grouped_plan_status(self._plan, C.byref(v)))
+        return v.value
+
+
 def moe_weighted_accumulate(routes: MoeSortedRoutes, route_weights: torch.Tensor, sorted_rows: torch.Tensor,
                             tokens: int, routes_per_row: int, out: torch.Tensor | None = None) -> torch.Tensor:
-    """moe_weighted_accumulate_sorted_bf16_batch (crates/eider-cuda/src/kernels/non_gemm.rs:3336+): f32 [tokens, len]."""
+    """moe_weighted_accumulate_sorted_bf16_batch (crates/eider-cuda/src/kernels/non_gemm.rs:3336+): f32 [tokens, len]; a bf16 `out`
+    takes the f32 sums rounded once."""
     lib = _lib.load()
     _need(sorted_rows, torch.bfloat16, "sorted rows")
     _need(route_weights, torch.float32, "route weights")
     ln = sorted_rows.shape[1]
     if out is None:
         out = torch.empty(tokens, ln, dtype=torch.float32, device=sorted_rows.device)
+    if out.dtype == torch.bfloat16:
+        _need(out, torch.bfloat16, "output")
+        check("eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream",
+              lib.eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream(routes.route_to_sorted.data_ptr(), route_weights.data_ptr(),
+                                                                              sorted_rows.data_ptr(), out.data_ptr(), tokens, ln, routes_per_row,
+                                                                              _stream()))
+        return out
     check("infer_moe_weighted_accumulate_sorted_bf16_batch_on_stream",
           lib.infer_moe_weighted_accumulate_sorted_bf16_batch_on_stream(routes.route_to_sorted.data_ptr(),
                                                                         route_weights.data_ptr(), sorted_rows.data_ptr(),
@@ -900,12 +1274,25 @@ def moe_weighted_accumulate(routes: MoeSortedRoutes, route_weights: torch.Tensor
 
 class GroupedMoe:
     """The routed-MoE prefill pipeline of Qwen36MoeWeights::run_batch (crates/infer/src/qwen3/qwen36/batch.rs:6785-6860):
-    top-k -> sort -> gather + quantize -> grouped gate/up GEMM -> SiLU * up + quantize -> grouped down GEMM -> combine."""
+    top-k -> sort -> gather + quantize -> grouped gate/up GEMM -> SiLU * up + quantize -> grouped down GEMM -> combine.
+    `weight_format`: "nvfp4", or "mxfp4" for GroupedMxfp4Weights, whose gate/up rows are always interleaved.  The buffers between the
+    steps and the f32 result belong to the object: one call at a time."""
 
-    def __init__(self, tokens: int, experts: int, top_k: int, hidden: int, intermediate: int, device="cuda"):
+    def __init__(self, tokens: int, experts: int, top_k: int, hidden: int, intermediate: int, device="cuda", weight_format: str = "nvfp4"):
+        if weight_format not in ("nvfp4", "mxfp4"):
+            raise ShapeError(f"weight_format must be nvfp4 or mxfp4, got {weight_format!r}")
         self.tokens, self.experts, self.top_k, self.hidden, self.inter = tokens, experts, top_k, hidden, intermediate
+        self.weight_format = weight_format
         r = tokens * top_k
         self.routes = MoeSortedRoutes(r, experts, device)
+        if weight_format == "mxfp4":
+            self.gate_up_in, self.down_in = MoeSortedMxfp4Rows(r, experts, hidden, device), MoeSortedMxfp4Rows(r, experts, intermediate, device)
+            with torch.cuda.device(self.down_in.packed.device):
+                self.gate_up_plan = Mxfp4GroupedGemmPlan(2 * intermediate, tokens, hidden, experts)
+                self.down_plan = Mxfp4GroupedGemmPlan(hidden, tokens, intermediate, experts)
+            self.down_out = torch.empty(r, hidden, dtype=torch.bfloat16, device=device)
+            self.out = torch.empty(tokens, hidden, dtype=torch.float32, device=device)
+            return
         self.gate_up_in = MoeSortedNvfp4Rows(r, experts, hidden, tokens, device)
         self.down_in = MoeSortedNvfp4Rows(r, experts, intermediate, tokens, device)
         self.gate_up_plan = Fp4GroupedGemmPlan(2 * intermediate, tokens, hidden, experts)
@@ -915,10 +1302,16 @@ class GroupedMoe:
         self.out = torch.empty(tokens, hidden, dtype=torch.float32, device=device)
 
     def run(self, x: torch.Tensor, router_logits: torch.Tensor, w_gate_up: GroupedNvfp4Weights, w_down: GroupedNvfp4Weights,
-            norm_topk_prob: bool = True, w_gate_up_interleaved: GroupedNvfp4Weights | None = None) -> torch.Tensor:
-        """With `w_gate_up_interleaved` (GroupedNvfp4Weights.interleave_gate_up(), made once at load) the SiLU * up
+            norm_topk_prob: bool = True, w_gate_up_interleaved: GroupedNvfp4Weights | None = None,
+            out_dtype=torch.float32) -> torch.Tensor:
+        """f32 [tokens, hidden] in the object's buffer, or with out_dtype = torch.bfloat16 a new bf16 tensor.  With `w_gate_up_interleaved` (GroupedNvfp4Weights.interleave_gate_up(), made once at load) the SiLU * up
         quantizer runs in the gate/up GEMM's epilogue and the bf16 gate/up rows never reach HBM; the bytes of the down
         projection's input are the same either way."""
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise ShapeError(f"output must be f32 or bf16, got {out_dtype}")
+        out = self.out if out_dtype == torch.float32 else torch.empty(self.tokens, self.hidden, dtype=torch.bfloat16, device=self.out.device)
+        if self.weight_format == "mxfp4":
+            return self._run_mxfp4(x, router_logits, w_down, norm_topk_prob, w_gate_up_interleaved, out)
         idx, weights = moe_topk(router_logits, self.top_k, norm_topk_prob)
         self.routes.sort(idx.reshape(-1))
         self.gate_up_in.gather_quantize(x, self.routes, self.top_k)
@@ -930,7 +1323,23 @@ class GroupedMoe:
         self.down_plan.run(self.down_in, w_down, self.routes, out=self.down_out)
         self.route_weights = weights
         self.route_indices = idx
-        return moe_weighted_accumulate(self.routes, weights.reshape(-1), self.down_out, self.tokens, self.top_k, out=self.out)
+        return moe_weighted_accumulate(self.routes, weights.reshape(-1), self.down_out, self.tokens, self.top_k, out=out)
+
+    def _run_mxfp4(self, x, router_logits, w_down, norm_topk_prob, w_gate_up_interleaved, out):
+        """The same steps over MXFP4 rows; SiLU * up takes the f32 accumulators of the gate/up GEMM."""
+        if not isinstance(w_gate_up_interleaved, GroupedMxfp4Weights) or not isinstance(w_down, GroupedMxfp4Weights):
+            raise ShapeError("an MXFP4 layer takes GroupedMxfp4Weights, the gate/up weights through interleave_gate_up()")
+        if router_logits.shape != (self.tokens, self.experts) or x.shape != (self.tokens, self.hidden):
+            raise ShapeError("x must be [tokens, hidden] and router_logits [tokens, experts]")
+        _need_device(self.out.device, x, router_logits)
+        with torch.cuda.device(self.out.device):
+            idx, weights = moe_topk(router_logits, self.top_k, norm_topk_prob)
+            self.routes.sort(idx.reshape(-1))
+            self.gate_up_in.quantize_routes(x, self.routes, self.top_k)
+            self.gate_up_plan.run_silu_quantize(self.gate_up_in, w_gate_up_interleaved, self.routes, self.down_in)
+            self.down_plan.run(self.down_in, w_down, self.routes, out=self.down_out)
+            self.route_weights, self.route_indices = weights, idx
+            return moe_weighted_accumulate(self.routes, weights.reshape(-1), self.down_out, self.tokens, self.top_k, out=out)
 
 
 # ---- operator composition ---------------------------------------------------------------------------------
@@ -939,9 +1348,12 @@ class DenseFfn:
     gate_up = X . W_gu^T (W4A4, f32 out) -> SiLU(gate) * up -> NVFP4 with the down projection's static input scale (one
     fused producer) -> down = A . W_d^T with beta = 1 on the residual -> bf16.  GEMM plans are cached by row count, as
     run_nvfp4_batch does (crates/infer/src/qwen3/qwen36/batch.rs:1008-1058), so a new chunk length costs one plan creation
-    and a repeated one costs none."""
+    and a repeated one costs none.  Weights in NVFP4 or, both, in MXFP4 (whose blocks need no input scale)."""
 
-    def __init__(self, w_gate_up: ModelOptWeight, w_down: ModelOptWeight):
+    def __init__(self, w_gate_up: ModelOptWeight | Mxfp4Weight, w_down: ModelOptWeight | Mxfp4Weight):
+        self.mxfp4 = isinstance(w_gate_up, Mxfp4Weight)
+        if self.mxfp4 != isinstance(w_down, Mxfp4Weight):
+            raise ShapeError("gate/up and down must be of one format")
         if w_gate_up.out_features % 2 != 0 or w_down.in_features * 2 != w_gate_up.out_features or w_down.out_features != w_gate_up.in_features:
             raise ShapeError("gate/up must be [2 * intermediate, hidden] and down [hidden, intermediate]")
         self.w_gate_up, self.w_down = w_gate_up, w_down
@@ -950,7 +1362,9 @@ class DenseFfn:
 
     def plans(self, rows: int):
         if rows not in self._plans:
-            self._plans[rows] = (Fp4TnMatmulPlan(rows, 2 * self.inter, self.hidden), Fp4TnMatmulPlan(rows, self.hidden, self.inter))
+            plan = Mxfp4MatmulPlan if self.mxfp4 else Fp4TnMatmulPlan
+            with torch.cuda.device(self.w_down.packed.device):
+                self._plans[rows] = (plan(rows, 2 * self.inter, self.hidden), plan(rows, self.hidden, self.inter))
         return self._plans[rows]
 
     def run(self, x: torch.Tensor, residual: torch.Tensor) -> torch.Tensor:
@@ -963,6 +1377,13 @@ class DenseFfn:
         if residual.device != x.device or not residual.is_contiguous():
             raise ShapeError("residual must be row-major and on the device of x")
         gate_up_plan, down_plan = self.plans(rows)
+        if self.mxfp4:
+            xq = quantize_mxfp4(x)
+            if self.inter % 128 == 0 and rows > 128:
+                act = gate_up_plan.run_silu_quantize(xq, self.w_gate_up)
+            else:
+                act = silu_mul_halves_quantize_mxfp4(gate_up_plan.run(xq, self.w_gate_up, out_dtype=torch.float32))
+            return down_plan.run(act, self.w_down, beta=1.0, c=residual)
         xq = quantize_nvfp4_rowscale(x)
         # One row tile leaves the odd CTA of every pair without rows: hidden 5120 / intermediate 13824, 64 rows 23.0 us fused against
         # 18.9 in two launches, 129 rows 23.4 against 25.6, 333 rows 31.3 against 41.9, 2048 rows 116 against 174.  (FFNs that

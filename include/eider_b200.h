@@ -810,6 +810,90 @@ EIDER_B200_API cudaError_t eider_b200_ep_return_rows_on_stream(const uint16_t* r
                                                                uint32_t capacity, uint32_t out_features, uint32_t world,
                                                                cudaStream_t stream);
 
+/* ---- MXFP4 -------------------------------------------------------------------------------------
+ * 32 consecutive elements of a row are a block: E2M1 codes packed two per byte (even element in the low nibble) and one E8M0
+ * scale byte c that stands for 2^(c - 127), 255 for NaN (crates/eider-cuda/src/format.rs:112-119 decodes it).  No tensor-wide scale.
+ * K is a multiple of 32 everywhere.  Scales are row-major [rows][K / 32] (checkpoint layout) or tiled: the 128-row x 4-block tiles of
+ * the NVFP4 layout with blocks of 32, eider_b200_mxfp4_scale_layout_len(rows, K) bytes, 16-byte aligned.  Rows and blocks of the
+ * tiles behind the matrix are padding, and a padding BLOCK must not be 255: the quantizers below write zeros there.
+ * The reference widens MXFP4 checkpoints to NVFP4 (crates/eider-format/src/modelopt.rs:173-248), which refuses scales that E4M3
+ * cannot hold; these entry points run them as they are.  The rule on weights and programmatic launches above holds here too. */
+EIDER_B200_API size_t eider_b200_mxfp4_scale_layout_len(size_t outer, size_t inner);
+/* c = clamp(floor(log2(amax)) - 2 + 127, 0, ..), codes of x * 2^(127 - c) to nearest even, saturating at 6 (the OCP microscaling
+ * conversion); a block with a NaN or an infinity gets c = 255.  input: f32 or bf16 rows `row_stride` elements apart; packed
+ * [tokens][in_features / 2]; scales tiled, written with their padding. */
+EIDER_B200_API cudaError_t eider_b200_quantize_mxfp4_on_stream(const void* input, int input_is_bf16, size_t row_stride, uint8_t* packed,
+                                                               uint8_t* scales, uint32_t tokens, uint32_t in_features, cudaStream_t stream);
+/* The same conversion for weights, with row-major scales [out_features][in_features / 32]; releases no dependent launch early. */
+EIDER_B200_API cudaError_t eider_b200_quantize_mxfp4_weight_on_stream(const void* weight, int input_is_bf16, uint8_t* packed,
+                                                                      uint8_t* scales_row_major, uint32_t out_features,
+                                                                      uint32_t in_features, cudaStream_t stream);
+/* ... of SiLU(gate) * up: f32 rows of gate_up [tokens][2 * inner], the gate half first. */
+EIDER_B200_API cudaError_t eider_b200_silu_mul_halves_quantize_mxfp4_on_stream(const float* gate_up, uint8_t* packed, uint8_t* scales,
+                                                                               uint32_t tokens, uint32_t inner, cudaStream_t stream);
+/* The values that codes and tiled scales stand for, f32 or bf16 [rows][in_features] (16-byte aligned). */
+EIDER_B200_API cudaError_t eider_b200_dequantize_mxfp4_on_stream(const uint8_t* packed, const uint8_t* scales, void* output, int output_is_bf16,
+                                                                 uint32_t rows, uint32_t in_features, cudaStream_t stream);
+/* Row-major scales of `groups` stacked matrices [out_features][in_features / 32] -> tiled, every matrix on 128-row tiles of its own. */
+EIDER_B200_API cudaError_t eider_b200_mxfp4_scales_to_tiled_on_stream(const uint8_t* scales_row_major, uint8_t* scales_tiled, uint32_t groups,
+                                                                      uint32_t out_features, uint32_t in_features, cudaStream_t stream);
+
+/* Dense W4A4 GEMM, D[m][n] = alpha * X . W^T + beta * C, f32 accumulation, bf16 or f32 D and C; shapes, tiles and plan calls
+ * (eider_b200_gemm_plan_*) as for NVFP4, without split K. */
+EIDER_B200_API int eider_b200_mxfp4_gemm_tn_supported(uint32_t m, uint32_t n, uint32_t k);
+EIDER_B200_API void* eider_b200_mxfp4_gemm_tn_create(uint32_t m, uint32_t n, uint32_t k);
+EIDER_B200_API void eider_b200_mxfp4_gemm_tn_destroy(void* plan);
+EIDER_B200_API cudaError_t eider_b200_mxfp4_gemm_tn_on_stream(void* plan, const uint8_t* x_values, const uint8_t* x_scales,
+                                                              const uint8_t* w_values, const uint8_t* w_scales, const void* c, void* d,
+                                                              float alpha, float beta, int out_is_bf16, cudaStream_t stream);
+/* Gate/up GEMM with SiLU(gate) * up -> MXFP4 in its epilogue: n = 2 * intermediate, intermediate % 128 == 0 (else
+ * cudaErrorNotSupported), gate rows first; the bytes of the f32 GEMM followed by the stand-alone quantizer. */
+EIDER_B200_API cudaError_t eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream(void* plan, const uint8_t* x_values, const uint8_t* x_scales,
+                                                                            const uint8_t* w_values, const uint8_t* w_scales, float alpha,
+                                                                            uint8_t* packed, uint8_t* scales, cudaStream_t stream);
+
+/* W4A16 product for 1 to 64 tokens, D[t][n] = X . W^T + beta * C, X f32 or bf16 [tokens][in_features], D and C f32 or bf16.  The
+ * scales are rows of `scale_pitch` bytes (a multiple of 16, at least in_features / 32 rounded up to 8) with zeros behind the
+ * blocks.  X, weights and scales 16-byte aligned.  A plan keeps nothing between calls but the status word: calls on several
+ * streams may overlap. */
+EIDER_B200_API void* eider_b200_mxfp4_decode_create(uint32_t max_tokens, uint32_t out_features, uint32_t in_features);
+EIDER_B200_API void eider_b200_mxfp4_decode_destroy(void* plan);
+EIDER_B200_API cudaError_t eider_b200_mxfp4_decode_status(void* plan, uint32_t* host_status);
+EIDER_B200_API cudaError_t eider_b200_mxfp4_w4a16_gemv_on_stream(void* plan, const void* input, int input_is_bf16, uint32_t tokens,
+                                                                 const uint8_t* w_values, const uint8_t* w_scales_rows, uint32_t scale_pitch,
+                                                                 const void* c, void* d, float beta, int out_is_bf16, cudaStream_t stream);
+
+/* Routed experts.  Rows are expert-major as for NVFP4: the scales of expert e start at ((offset[e] + 127) / 128 + e) tiles of
+ * scale_tile_bytes = 128 * (in_features / 32 rounded up to 4).  The route quantizer writes every route's row and scales; the padding
+ * blocks of `scales` written by the GEMM's epilogue are the caller's to zero once. */
+EIDER_B200_API cudaError_t eider_b200_moe_quantize_routes_mxfp4_on_stream(const void* input, int input_is_bf16, const uint32_t* route_to_sorted,
+                                                                          const uint32_t* sorted_routes, const uint32_t* sorted_experts,
+                                                                          const uint32_t* expert_offsets, uint8_t* packed, uint8_t* scales,
+                                                                          uint32_t rows, uint32_t routes_per_row, uint32_t in_features,
+                                                                          uint32_t scale_tile_bytes, cudaStream_t stream);
+/* m = out features per expert, a multiple of 32; the weights' scales tiled per expert (eider_b200_mxfp4_scales_to_tiled_on_stream
+ * with groups = experts).  Output bf16 [route][m] times alpha[expert]. */
+EIDER_B200_API int eider_b200_mxfp4_grouped_gemm_supported(uint32_t m, uint32_t max_n, uint32_t k, uint32_t groups);
+EIDER_B200_API void* eider_b200_mxfp4_grouped_gemm_create(uint32_t m, uint32_t max_n, uint32_t k, uint32_t groups);
+EIDER_B200_API void eider_b200_mxfp4_grouped_gemm_destroy(void* plan);
+EIDER_B200_API cudaError_t eider_b200_mxfp4_grouped_gemm_on_stream(void* plan, const uint8_t* a_values, const uint8_t* a_scales,
+                                                                   const uint8_t* w_values, const uint8_t* w_scales_tiled, uint16_t* output,
+                                                                   const float* alpha, const uint32_t* expert_offsets, uint32_t total_routes,
+                                                                   cudaStream_t stream);
+/* ... with SiLU(gate) * up -> MXFP4 of the f32 accumulators in the epilogue: m = 2 * intermediate, the weight rows of every expert
+ * interleaved [32 gate, 32 up]. */
+EIDER_B200_API cudaError_t eider_b200_mxfp4_grouped_gemm_silu_quantize_on_stream(void* plan, const uint8_t* a_values, const uint8_t* a_scales,
+                                                                                 const uint8_t* w_values_interleaved,
+                                                                                 const uint8_t* w_scales_tiled_interleaved, const float* alpha,
+                                                                                 const uint32_t* expert_offsets, uint32_t total_routes,
+                                                                                 uint8_t* packed, uint8_t* scales, uint32_t scale_tile_bytes,
+                                                                                 cudaStream_t stream);
+/* infer_moe_weighted_accumulate_sorted_bf16_batch_on_stream with the f32 sums rounded once to bf16. */
+EIDER_B200_API cudaError_t eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream(const uint32_t* route_to_sorted, const float* route_weights,
+                                                                                       const uint16_t* sorted_inputs, uint16_t* output,
+                                                                                       uint32_t rows, uint32_t len, uint32_t routes_per_row,
+                                                                                       cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

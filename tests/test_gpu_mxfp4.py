@@ -1,0 +1,390 @@
+"""MXFP4 kernels against the format's definition in 64 bits: quantizers bit for bit, products within the roundings they make."""
+import pytest
+import torch
+
+from eider_b200 import ops
+from tests import mxfp4_reference as ref
+from tests.util import require_cuda
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _cuda():
+    require_cuda()
+
+
+def gen(seed=0):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.float32, std=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+def check_matrix(m, x):
+    """Codes and scales of a quantized matrix against the definition, padding included."""
+    codes, scales = ref.quantize(x)
+    got, clean = ref.untile(m.scales, m.rows, m.k)
+    assert torch.equal(got, scales)
+    assert clean, "padding scales are not zero"
+    finite = (scales != 255).repeat_interleave(32, 1)  # (the codes of a NaN block mean nothing)
+    assert torch.equal(ref.unpack(m.packed)[finite], codes[finite])
+
+
+# ---- quantisation -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,k", [(1, 32), (1, 5120), (3, 96), (31, 128), (130, 160), (257, 2880), (512, 64), (1029, 416)])
+def test_quantize_is_exact(rows, k, dtype):
+    x = randn(gen(rows + k), rows, k, dtype=dtype, std=3.0)
+    m = ops.quantize_mxfp4(x)
+    check_matrix(m, x)
+    codes, scales = ref.quantize(x)
+    for out in (torch.float32, torch.bfloat16):
+        assert torch.equal(m.dequantize(out).double(), ref.values(codes, scales))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_boundaries(dtype):
+    """Ties between codes, saturation between 6 and 8, zeros of both signs, magnitudes from subnormal to the largest."""
+    steps = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 6.5, 7.0, 7.75, 0.0, -0.0, 0.125, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0, -7.5,
+                          0.2490234375, 0.251953125, 4.96875, 5.03125, 1.0, 2.0, 3.0, 4.0, 0.5, -6.0], device="cuda")
+    exponents = [-148, -140, -133, -130, -128, -127, -126, -125, -120, -60, -2, 0, 1, 60, 120, 124, 125]
+    x = torch.stack([(steps.double() * 2.0 ** e).to(dtype) for e in exponents])
+    x = torch.cat([x, torch.zeros_like(x[:1]), -torch.zeros_like(x[:1])])
+    x = x[torch.isfinite(x).all(1)]
+    check_matrix(ops.quantize_mxfp4(x.contiguous()), x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_poisoned_blocks(dtype):
+    x = randn(gen(3), 70, 160, dtype=dtype)
+    x[1, 33] = float("nan")
+    x[2, 0] = float("inf")
+    x[69, 159] = -float("inf")
+    m = ops.quantize_mxfp4(x)
+    check_matrix(m, x)
+    bad = torch.isnan(m.dequantize())
+    assert bad[1, 32:64].all() and bad[2, :32].all() and bad[69, 128:].all() and int(bad.sum()) == 96
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_strides_and_alignment(dtype):
+    wide = randn(gen(4), 40, 500, dtype=dtype)
+    for x in (wide[:, :96], wide[:, 3:131], wide[::2, 8:40], wide.flatten()[1:1 + 3 * 64].reshape(3, 64)):
+        check_matrix(ops.quantize_mxfp4(x), x)
+    one = wide[5:6, 7:39]  # one row: its stride does not matter
+    check_matrix(ops.quantize_mxfp4(one), one)
+
+
+def test_weight_quantizer_and_layouts():
+    g = gen(5)
+    for n, k in ((1, 32), (130, 96), (200, 2912)):
+        w = randn(g, n, k, std=0.02)
+        m = ops.Mxfp4Weight.quantize(w)
+        codes, scales = ref.quantize(w)
+        assert torch.equal(ref.unpack(m.packed), codes) and torch.equal(m.scales_row_major, scales)
+        tiled, clean = ref.untile(m.scales_tiled, n, k)
+        assert torch.equal(tiled, scales) and clean
+        assert torch.equal(m.scales_rows[:, : k // 32], scales) and not m.scales_rows[:, k // 32:].any() and m.scales_rows.shape[1] % 16 == 0
+        assert torch.equal(m.dequantize().double(), ref.values(codes, scales))
+
+
+def test_silu_quantizer():
+    """The fused producer's values are those of SiLU * up but for codes next to a boundary (f32 exponential and reciprocal)."""
+    for rows, k in ((1, 32), (5, 96), (130, 2784)):
+        x = randn(gen(k), rows, 2 * k, std=2.0)
+        m = ops.silu_mul_halves_quantize_mxfp4(x)
+        act = ref.silu_mul(x.double())
+        codes, scales = ref.quantize(act)
+        got, clean = ref.untile(m.scales, rows, k)
+        assert clean
+        # a boundary is met by about 1e-5 of the values at a relative error of 1e-6; none may be off by more than a step
+        assert (got != scales).float().mean() <= 1e-3 and (ref.unpack(m.packed) != codes).float().mean() <= 1e-3
+        step = torch.exp2(scales.double() - 127).repeat_interleave(32, 1) * 2
+        assert ((m.dequantize().double() - act).abs() <= step * 1.01).all()
+
+
+# ---- dense product ------------------------------------------------------------------------------------------------
+def product_bound(x, w, extra=0):
+    """f32 sums of exact products: the tensor core adds 64 products at a time to what it has, each addition off by at most a step of
+    the sum (2^-23 of the largest partial sum, which sum |x w| bounds)."""
+    return (x.shape[1] // 64 + 4 + extra) * 2.0 ** -23 * (x.abs() @ w.abs().t())
+
+
+def rounded(bound, y, dtype):
+    """... and the result rounded to its type."""
+    return bound + torch.finfo(dtype).eps / 2 * y.abs()
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k,n", [(1, 32, 1), (1, 5120, 320), (5, 96, 40), (64, 160, 136), (129, 224, 264), (300, 2912, 1000), (520, 512, 1296)])
+def test_gemm(m, k, n, out):
+    g = gen(m + k + n)
+    x = randn(g, m, k)
+    xq, w = ops.quantize_mxfp4(x), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k))
+    xv, wv = ref.values(*ref.quantize(x)), w.dequantize().double()
+    plan = ops.Mxfp4MatmulPlan(m, n, k)
+    y = plan.run(xq, w, alpha=0.75, out_dtype=out)
+    want = 0.75 * (xv @ wv.t())
+    assert ((y.double() - want).abs() <= rounded(product_bound(xv, wv), want, out)).all()
+    c = randn(g, m, n, dtype=out)
+    y = plan.run(xq, w, beta=-0.5, c=c, out_dtype=out)
+    want = xv @ wv.t() - 0.5 * c.double()
+    assert ((y.double() - want).abs() <= rounded(product_bound(xv, wv, 2) + 2.0 ** -23 * c.double().abs(), want, out)).all()
+    assert plan.status() == 0
+
+
+@pytest.mark.parametrize("block_n", [64, 128, 192, 256, 384, 512])
+def test_gemm_tiles_agree(block_n):
+    """Every tile shape adds the same products in the same order."""
+    g = gen(7)
+    for m, k, n in ((300, 1184, 840), (128, 256, 512)):
+        xq, w = ops.quantize_mxfp4(randn(g, m, k)), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k))
+        plan = ops.Mxfp4MatmulPlan(m, n, k)
+        plan.set_block_n(64)
+        want = plan.run(xq, w, out_dtype=torch.float32)
+        plan.set_block_n(block_n)
+        assert torch.equal(plan.run(xq, w, out_dtype=torch.float32), want)
+        assert torch.equal(plan.run(xq, w), want.to(torch.bfloat16))
+        assert plan.status() == 0
+
+
+def test_gemm_scale_range():
+    """Every scale from 2^-126 to 2^126 that a product can hold, and NaN scales in one row of each operand."""
+    g = gen(8)
+    m, k, n = 40, 128, 72
+    codes = torch.randint(0, 16, (m, k), generator=g, device="cuda", dtype=torch.uint8)
+    sx = torch.randint(1, 254, (m, 1), generator=g, device="cuda").expand(m, k // 32).contiguous().to(torch.uint8)
+    wp, _ = ref.weight(g, n, k)
+    sw = torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda")
+    sw[1] = 255
+    sx[2, 3] = 255
+    x = ops.Mxfp4Matrix(ref.pack(codes).contiguous(), ops._mxfp4_tiled(sx, 1, m, k), m, k)
+    w = ops.Mxfp4Weight.from_checkpoint(wp, sw)
+    y = ops.Mxfp4MatmulPlan(m, n, k).run(x, w, out_dtype=torch.float32)
+    xv, wv = ref.values(codes, sx), ref.values(ref.unpack(wp), sw)
+    want = xv @ wv.t()
+    assert torch.isnan(y[2]).all() and torch.isnan(y[:, 1]).all()
+    fine = ~torch.isnan(want) & (want.abs() < 3e38)
+    assert ((y.double() - want).abs()[fine] <= (product_bound(xv, wv) + 2.0 ** -126)[fine]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 127, 130, 513])
+def test_gated_gemm_equals_two_launches(rows):
+    g = gen(rows)
+    for inter, k in ((128, 96), (384, 2048)):
+        xq, w = ops.quantize_mxfp4(randn(g, rows, k)), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, 2 * inter, k, std=0.1))
+        plan = ops.Mxfp4MatmulPlan(rows, 2 * inter, k)
+        fused = plan.run_silu_quantize(xq, w)
+        staged = ops.silu_mul_halves_quantize_mxfp4(plan.run(xq, w, out_dtype=torch.float32))
+        assert torch.equal(fused.packed, staged.packed) and torch.equal(fused.scales, staged.scales)
+        assert plan.status() == 0
+
+
+@pytest.mark.parametrize("rows,hidden,inter", [(1, 96, 160), (77, 512, 288), (300, 512, 384)])
+def test_ffn(rows, hidden, inter):
+    """DenseFfn over MXFP4 weights: the activation's codes against 64 bits but for boundaries, then its product exactly."""
+    g = gen(rows)
+    gate_up, down = (ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k, std=0.1)) for n, k in ((2 * inter, hidden), (hidden, inter)))
+    x, residual = randn(g, rows, hidden, dtype=torch.bfloat16), randn(g, rows, hidden, dtype=torch.bfloat16)
+    y = ops.DenseFfn(gate_up, down).run(x, residual)
+    act = ref.silu_mul(ref.values(*ref.quantize(x)) @ gate_up.dequantize().double().t())
+    act = ref.values(*ref.quantize(act))
+    wv = down.dequantize().double()
+    want = act @ wv.t() + residual.double()
+    # one code in a thousand may be a step (a third of its value) off: sqrt(1e-3) / 3 of the product's size, and the rounding
+    off = (y.double() - want).abs()
+    assert (off <= 0.05 * (act.abs() @ wv.abs().t()) + 2.0 ** -8 * want.abs()).all()
+    assert off.norm() <= (0.011 + 2.0 ** -8) * want.norm()
+
+
+# ---- few tokens -----------------------------------------------------------------------------------------------
+def decode_bound(x, w, dtype):
+    """Block sums of two (f32: four) MMAs, K / 32 of them added up in f32 and eleven warps' sums after them; f32 activations go in as
+    two f16 terms that leave 2^-23 of an element; elements far below their token's largest leave 2^-32 of that."""
+    total = x.abs() @ w.abs().t()
+    steps = x.shape[1] // 32 + 16 + (1 if dtype == torch.float32 else 0)
+    return steps * 2.0 ** -23 * total + 2.0 ** -32 * x.abs().amax(1, keepdim=True) * w.abs().sum(1)
+
+
+SHAPES = [(1, 32), (40, 96), (256, 512), (1000, 2912), (6150, 1056), (3001, 8192), (15000, 288)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [1, 2, 7, 8, 9, 16, 17, 31, 33, 64])
+def test_decode(tokens, dtype):
+    g = gen(tokens)
+    for n, k in SHAPES:
+        x, w = randn(g, tokens, k, dtype=dtype), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k))
+        wv, xv = w.dequantize().double(), x.double()
+        want, bound = xv @ wv.t(), decode_bound(xv, wv, dtype)
+        plan = ops.Mxfp4DecodePlan(64, n, k)
+        for out in (torch.float32, torch.bfloat16):
+            y = plan.run(x, w, out_dtype=out)
+            assert y.shape == (tokens, n)
+            assert ((y.double() - want).abs() <= rounded(bound, want, out)).all(), (n, k, out)
+        c = randn(g, tokens, n)
+        y = plan.run(x, w, beta=0.25, c=c, out_dtype=torch.float32)
+        assert ((y.double() - want - 0.25 * c.double()).abs() <= bound + 2.0 ** -22 * (want.abs() + c.double().abs())).all()
+        assert plan.status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_activation_ranges(dtype):
+    """Tokens whose elements start at zero, grow or shrink by many powers of two along K, or are tiny or huge throughout."""
+    g = gen(11)
+    n, k = 200, 5120
+    x = torch.randn(14, k, generator=g, device="cuda")
+    ramp = torch.linspace(0, 1, k, device="cuda")
+    x[0, :3000] = 0
+    x[1, 300:] = 0
+    x[2] = 0
+    x[3] *= torch.exp2(60 * ramp)
+    x[4] *= torch.exp2(-60 * ramp)
+    x[5] *= 2.0 ** -120
+    x[6] *= 2.0 ** 100
+    x[7, ::2] = 0
+    x[8, :5000] *= 2.0 ** -100
+    x[9, 40] = 2.0 ** 90
+    x[10] *= torch.exp2(torch.randint(-40, 40, (k,), generator=g, device="cuda").float())
+    x[11, :] = 0
+    x[11, -1] = 1.0
+    x[12] = 2.0 ** -126
+    x = x.to(dtype)
+    w = ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k))
+    wv, xv = w.dequantize().double(), x.double()
+    y = ops.Mxfp4DecodePlan(16, n, k).run(x, w, out_dtype=torch.float32).double()
+    assert ((y - xv @ wv.t()).abs() <= decode_bound(xv, wv, dtype) + 2.0 ** -140).all()
+    assert not y[2].any()
+
+
+def test_decode_poison_stays_with_its_token_and_row():
+    g = gen(12)
+    n, k = 100, 1024
+    wp, ws = ref.weight(g, n, k)
+    ws[7, 3] = 255
+    ws[9] = 0
+    ws[11, 5] = 254
+    w = ops.Mxfp4Weight.from_checkpoint(wp, ws)
+    x = randn(g, 5, k, dtype=torch.bfloat16)
+    x[1, 100] = float("nan")
+    x[3, 700] = float("inf")
+    y = ops.Mxfp4DecodePlan(8, n, k).run(x, w, out_dtype=torch.float32)
+    wv = ref.values(ref.unpack(wp), ws)
+    want = x.double() @ wv.t()
+    assert torch.isnan(y[1]).all() and not torch.isfinite(y[3]).any() and torch.isnan(y[:, 7]).all()
+    fine = torch.isfinite(want) & (want.abs() < 3e38)
+    fine[:, 7] = False
+    assert fine[0].sum() >= 98 and ((y.double() - want).abs()[fine] <= (decode_bound(x.double().nan_to_num(0, 0, 0), wv.nan_to_num(0), torch.bfloat16) + 1e-38)[fine]).all()
+
+
+def test_decode_is_the_same_in_every_run_and_grouping():
+    """A token's result does not depend on the tokens beside it (within one group width), and two runs agree bit for bit."""
+    g = gen(13)
+    n, k = 6150, 4064
+    x, w = randn(g, 8, k), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k))
+    plan = ops.Mxfp4DecodePlan(8, n, k)
+    y = plan.run(x, w, out_dtype=torch.float32)
+    assert torch.equal(plan.run(x, w, out_dtype=torch.float32), y)
+    for t in (0, 3, 7):
+        assert torch.equal(plan.run(x[t], w, out_dtype=torch.float32)[0], y[t])
+
+
+# ---- routed experts -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,experts,top_k,hidden,inter", [(1, 4, 2, 64, 32), (5, 8, 3, 160, 96), (77, 16, 4, 512, 288), (300, 6, 6, 288, 320), (1000, 32, 2, 256, 128)])
+def test_experts(tokens, experts, top_k, hidden, inter, dtype):
+    g = gen(tokens)
+    gate_up, down = ([t.reshape(experts, -1, t.shape[1]) for t in ref.weight(g, experts * n, k, std=0.1)] for n, k in ((2 * inter, hidden), (hidden, inter)))
+    gu, dn = ops.GroupedMxfp4Weights.from_checkpoint(*gate_up), ops.GroupedMxfp4Weights.from_checkpoint(*down)
+    x, logits = randn(g, tokens, hidden, dtype=dtype), randn(g, tokens, experts)
+    logits[:, 1] -= 20  # an expert that (almost) nobody picks
+    moe = ops.GroupedMoe(tokens, experts, top_k, hidden, inter, weight_format="mxfp4")
+    y = moe.run(x, logits, gu, dn, w_gate_up_interleaved=gu.interleave_gate_up())
+    y16 = moe.run(x, logits, gu, dn, w_gate_up_interleaved=gu.interleave_gate_up(), out_dtype=torch.bfloat16)
+    assert torch.equal(y16, y.to(torch.bfloat16))
+    xv = ref.values(*ref.quantize(x))
+    gv, dv = ref.values(ref.unpack(gate_up[0]), gate_up[1]), ref.values(ref.unpack(down[0]), down[1])
+    # the routes' rows as the layer left them: quantized inputs exactly, activations but for boundaries
+    order, expert = moe.routes.sorted_routes.long(), moe.routes.sorted_experts.long()
+    first = moe.routes.expert_offsets.long()
+    for name, rows_of in (("gate_up_in", hidden), ("down_in", inter)):
+        buffer = getattr(moe, name)
+        blocks, group = rows_of // 32, (rows_of // 32 + 3) // 4
+        tiles = buffer.scales.reshape(-1, group, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-1, group * 4)  # [tile * 128 + row][block]
+        at = ((first[expert] + 127) // 128 + expert) * 128 + torch.arange(len(order), device="cuda") - first[expert]
+        got = ref.values(ref.unpack(buffer.packed), tiles[at][:, :blocks])
+        if name == "gate_up_in":
+            assert torch.equal(got, xv[order // top_k])
+        else:
+            act = ref.silu_mul(torch.stack([xv[r // top_k] @ gv[e].t() for r, e in zip(order.tolist(), expert.tolist())]))
+            codes, scales = ref.quantize(act)
+            assert (got != ref.values(codes, scales)).double().mean() <= 2e-3
+            step = torch.exp2(scales.double() - 127).repeat_interleave(32, 1) * 2
+            assert ((got - act).abs() <= step * 1.01).all()
+            act = got
+    rows = torch.stack([act[i] @ dv[e].t() for i, e in enumerate(expert.tolist())])
+    bound = torch.stack([act[i].abs() @ dv[e].abs().t() for i, e in enumerate(expert.tolist())]) * (inter // 64 + 4) * 2.0 ** -23 + 2.0 ** -8 * rows.abs()
+    assert ((moe.down_out.double() - rows).abs() <= bound).all()
+    weights = torch.softmax(logits.double().topk(top_k, 1)[0], 1).reshape(-1, 1)
+    back, slack = torch.empty_like(rows), torch.empty_like(rows)
+    back[order], slack[order] = rows, bound
+    want = (back * weights).reshape(tokens, top_k, -1).sum(1)
+    limit = ((slack + 2.0 ** -20 * back.abs()) * weights).reshape(tokens, top_k, -1).sum(1)
+    assert ((y.double() - want).abs() <= limit + 1e-30).all()
+    assert moe.gate_up_plan.status() == 0 and moe.down_plan.status() == 0
+
+
+# ---- as they are used ---------------------------------------------------------------------------------------------
+def test_streams_and_graphs():
+    """Calls on a stream of their own, captured and replayed on new inputs; two graphs of one decode plan in flight together."""
+    g = gen(21)
+    n, k = 1000, 2048
+    w = [ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k)) for _ in range(2)]
+    plan, gemm = ops.Mxfp4DecodePlan(8, n, k), ops.Mxfp4MatmulPlan(8, n, k)
+    x = [randn(g, 8, k, dtype=torch.bfloat16) for _ in range(2)]
+    want = [(plan.run(x[i], w[i]), gemm.run(ops.quantize_mxfp4(x[i]), w[i])) for i in range(2)]
+    torch.cuda.synchronize()
+    streams, graphs, held, outs = [torch.cuda.Stream() for _ in range(2)], [], [torch.zeros_like(x[0]) for _ in range(2)], []
+    for i, s in enumerate(streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            outs.append((plan.run(held[i], w[i]), gemm.run(ops.quantize_mxfp4(held[i]), w[i])))
+        graphs.append(graph)
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                held[i].copy_(x[i])
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1])
+
+
+def test_refusals():
+    g = gen(22)
+    w = ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, 64, 96))
+    x = randn(g, 4, 96)
+    for bad in (x.half(), x.t(), x[:, :80], x[:0], x[0]):
+        with pytest.raises(ops.ShapeError):
+            ops.quantize_mxfp4(bad)
+    with pytest.raises(ops.ShapeError):
+        ops.quantize_mxfp4(x[:1].expand(4, 96))
+    plan, gemm = ops.Mxfp4DecodePlan(4, 64, 96), ops.Mxfp4MatmulPlan(4, 64, 96)
+    for args in ({"x": x[:, :64]}, {"x": randn(g, 5, 96)}, {"x": x.half()}, {"x": x.cpu()}, {"x": x, "out": torch.empty(4, 63, device="cuda")},
+                 {"x": x, "beta": 1.0, "c": torch.empty(4, 64, device="cuda").half()}, {"x": x, "out_dtype": torch.float16}, {"x": x[:0]}):
+        with pytest.raises(ops.ShapeError):
+            plan.run(w=w, **args)
+    xq = ops.quantize_mxfp4(x)
+    with pytest.raises(ops.ShapeError):
+        gemm.run(ops.quantize_mxfp4(x[:2]), w)
+    with pytest.raises(ops.ShapeError):
+        gemm.run(xq, w, out=torch.empty(4, 64, device="cuda", dtype=torch.float16))
+    with pytest.raises(ops.ShapeError):
+        gemm.run_silu_quantize(xq, w)
+    with pytest.raises(ops.ShapeError):
+        ops.Mxfp4DecodePlan(65, 64, 96)
+    moe = ops.GroupedMoe(4, 2, 1, 64, 32, weight_format="mxfp4")
+    with pytest.raises(ops.ShapeError):
+        moe.run(randn(g, 4, 64), randn(g, 4, 2), None, None)
