@@ -195,6 +195,9 @@ SIGNATURES = {
     "eider_b200_mxfp4_grouped_gemm_on_stream": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _U32, _P]),
     "eider_b200_mxfp4_grouped_gemm_silu_quantize_on_stream": (_I, [_P, _P, _P, _P, _P, _P, _P, _U32, _P, _P, _U32, _P]),
     "eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _P]),
+    "eider_b200_beam_select_workspace_bytes": (_SZ, [_U32, _U32, _U32, _I]),
+    "eider_b200_beam_select_on_stream": (_I, [_P, _I, _SZ, _P, _P, _U32, _P, _P, _P, _U32, _U32, _U32, _U32, _P, _SZ, _P]),
+    "eider_b200_beam_reorder_on_stream": (_I, [_P, _P, _P, _U32, _P, _SZ, _U32, _U32, _P]),
     "eider_b200_peer_barrier_on_stream": (_I, [_P, _U32, _U32, _U32, _P, C.c_uint64, _P]),
 }
 

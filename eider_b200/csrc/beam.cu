@@ -1,0 +1,461 @@
+// The step behind the lm-head when several hypotheses of a sequence are kept: the k best continuations over beams and vocabulary, and
+// the states of the beams they come from.
+//
+//   score(r, v) = beam_score[r] + logits[r][v] - log sum_u exp(logits[r][u]),   the k largest of a sequence's beams x vocab scores,
+//   equal scores in the order of beam * vocab + v.
+//
+// The scores are compared in 64 bits: log-sum-exps differ from row to row, and f32 would tie what is not equal.
+//
+// Two launches.  beam_scan_kernel reads the logits once (bound: HBM): running maximum and sum of exponentials per thread, and the
+// maximum of every 64 consecutive logits (a segment).  beam_merge_kernel, one CTA per sequence, finds the k best segments by their
+// maxima (the k best elements cannot lie in any others: each of k better segments holds a better element) and then the k best of
+// their elements.  Nothing of the order of vocab is written or sorted; no atomics decide an order.
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "quant_block.cuh"
+#include "eider_b200.h"
+
+namespace eider {
+namespace {
+
+constexpr uint32_t kFullMask = 0xffffffffu;
+constexpr uint32_t kSegment = 64;       // logits that share a maximum
+constexpr uint32_t kScanThreads = 256;
+constexpr uint32_t kAhead = 4;          // 16-byte vectors a thread has on their way
+constexpr uint32_t kMergeThreads = 512;
+constexpr uint32_t kCandidates = 2048;  // of a selection; more are taken one by one
+constexpr uint32_t kMaxBeams = 64, kMaxK = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct BeamArgs {
+    const void* logits;
+    size_t stride;              // elements from row to row
+    const float* beam_scores;   // [batch * beams]
+    const uint8_t* finished;    // [batch * beams] or null
+    float* segment_max;         // [batch * beams][segments]
+    float2* partial;            // [batch * beams][splits]: maximum and sum of exponentials below it
+    float* out_scores;          // [batch][k]
+    int32_t* out_parents;
+    int32_t* out_tokens;
+    uint32_t beams, vocab, k, pad_token, segments, splits, vectors_per_split;
+};
+
+__device__ __forceinline__ bool row_counts(const BeamArgs& a, uint32_t row) {
+    return isfinite(__ldg(a.beam_scores + row)) && !(a.finished && __ldg(a.finished + row));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T> struct Vec {
+    static constexpr uint32_t kElems = 16 / sizeof(T);
+};
+__device__ __forceinline__ float logit_value(float v) { return v; }
+__device__ __forceinline__ float logit_value(uint16_t v) { return bf16_bits_to_float(v); }
+__device__ __forceinline__ void vector_values(const uint4& q, float (&v)[4]) {
+    v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
+}
+__device__ __forceinline__ void vector_values(const uint4& q, float (&v)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+// Rows need not start on 16 bytes: positions count from the 16-byte boundary at or below the row, `lead` elements before it.
+template <typename T> __device__ __forceinline__ uint32_t row_lead(const T* row) {
+    return static_cast<uint32_t>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const BeamArgs a) {
+    constexpr uint32_t E = Vec<T>::kElems, kSegLanes = kSegment / E;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t row = blockIdx.y;
+    if (!row_counts(a, row)) return;
+    const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
+    const uint32_t lead = row_lead(logits), end = lead + a.vocab;
+    const uint32_t v1 = min((blockIdx.x + 1) * a.vectors_per_split, (end + E - 1) / E);
+    float* segment_max = a.segment_max + static_cast<size_t>(row) * a.segments;
+    float top = -INFINITY, sum = 0.0f;
+    // (whole warps run the same number of turns: the split is a multiple of the block)
+    for (uint32_t base = blockIdx.x * a.vectors_per_split; base < v1; base += kScanThreads * kAhead) {
+        float x[kAhead][E];
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            const uint32_t vec = base + j * kScanThreads + threadIdx.x, at = vec * E;
+            if (vec < v1 && at >= lead && at + E <= end) {
+                vector_values(__ldg(reinterpret_cast<const uint4*>(logits - lead) + vec), x[j]);
+            } else {  // the row's first and last vectors
+#pragma unroll
+                for (uint32_t e = 0; e < E; ++e) x[j][e] = vec < v1 && at + e >= lead && at + e < end ? logit_value(__ldg(logits + (at + e - lead))) : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            float m = x[j][0];
+#pragma unroll
+            for (uint32_t e = 1; e < E; ++e) m = fmaxf(m, x[j][e]);
+            const float new_top = fmaxf(top, m);
+            if (new_top > -INFINITY) {
+                sum *= exp2_fast((top - new_top) * kLog2e);
+#pragma unroll
+                for (uint32_t e = 0; e < E; ++e) sum += exp2_fast((x[j][e] - new_top) * kLog2e);
+                top = new_top;
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < E; ++e) sum += x[j][e] != x[j][e] ? x[j][e] : 0.0f;  // (NaNs pass the maximum by)
+            }
+#pragma unroll
+            for (uint32_t o = 1; o < kSegLanes; o *= 2) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
+            const uint32_t vec = base + j * kScanThreads + threadIdx.x;
+            if (threadIdx.x % kSegLanes == 0 && vec < v1) segment_max[vec / kSegLanes] = m;
+        }
+    }
+    __shared__ float tops[kScanThreads / 32], sums[kScanThreads / 32];
+    auto join = [](float& t, float& s, float t2, float s2) {
+        const float n = fmaxf(t, t2);
+        if (n > -INFINITY) {
+            s = s * exp2_fast((t - n) * kLog2e) + s2 * exp2_fast((t2 - n) * kLog2e);
+        } else {
+            s += s2;
+        }
+        t = n;
+    };
+#pragma unroll
+    for (uint32_t o = 16; o > 0; o /= 2) {
+        const float t2 = __shfl_down_sync(kFullMask, top, o), s2 = __shfl_down_sync(kFullMask, sum, o);
+        join(top, sum, t2, s2);
+    }
+    if (threadIdx.x % 32 == 0) {
+        tops[threadIdx.x / 32] = top;
+        sums[threadIdx.x / 32] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (uint32_t w = 1; w < kScanThreads / 32; ++w) join(top, sum, tops[w], sums[w]);
+        a.partial[static_cast<size_t>(row) * a.splits + blockIdx.x] = make_float2(top, sum);
+    }
+}
+
+struct Candidate {
+    double score;
+    uint32_t index;
+};
+__device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) { return a.score > b.score || (a.score == b.score && a.index < b.index); }
+
+struct MergeShared {
+    Candidate best[kMergeThreads];       // a thread's best
+    Candidate candidates[kCandidates];
+    Candidate segments[kMaxK], elements[kMaxK];
+    double base[kMaxBeams], top[kMaxBeams];  // a row's scores are (logit - top) + base: base = beam score - log of the sum below top
+    uint8_t counts[kMaxBeams], ended[kMaxBeams];
+    Candidate threshold;
+    uint32_t found;
+};
+
+// The best `k` (fewer, if fewer have a finite score) of value(0 .. n - 1), in order, into `out`; returns how many.  A thread's best
+// values rank the threads; what is not behind the k-th best thread's best is a candidate, and candidates are ranked by counting.
+template <typename Value>
+__device__ __forceinline__ uint32_t select(MergeShared& sh, uint32_t n, uint32_t k, Candidate* out, Value value) {
+    const Candidate none{-INFINITY, 0xffffffffu};
+    Candidate mine = none;
+    for (uint32_t j = threadIdx.x; j < n; j += kMergeThreads) {
+        const Candidate c = value(j);
+        if (c.score > -INFINITY && before(c, mine)) mine = c;
+    }
+    sh.best[threadIdx.x] = mine;
+    if (threadIdx.x == 0) {
+        sh.threshold = none;
+        sh.found = 0;
+    }
+    const bool any = mine.score > -INFINITY;
+    const uint32_t threads = __syncthreads_count(any);
+    if (any && threads >= k) {
+        uint32_t rank = 0;
+        for (uint32_t t = 0; t < kMergeThreads; ++t) rank += before(sh.best[t], mine);
+        if (rank == k - 1) sh.threshold = mine;
+    }
+    __syncthreads();
+    const Candidate threshold = sh.threshold;
+    for (uint32_t j = threadIdx.x; j < n; j += kMergeThreads) {
+        const Candidate c = value(j);
+        if (c.score > -INFINITY && !before(threshold, c)) {
+            const uint32_t at = atomicAdd(&sh.found, 1u);
+            if (at < kCandidates) sh.candidates[at] = c;
+        }
+    }
+    __syncthreads();
+    const uint32_t found = sh.found;
+    if (found <= kCandidates) {
+        for (uint32_t c = threadIdx.x; c < found; c += kMergeThreads) {
+            const Candidate x = sh.candidates[c];
+            uint32_t rank = 0;
+            for (uint32_t t = 0; t < found; ++t) rank += before(sh.candidates[t], x);
+            if (rank < k) out[rank] = x;
+        }
+        __syncthreads();
+        return min(found, k);
+    }
+    // Too many to rank (long runs of equal scores among few threads): the next one in order, k times.
+    Candidate last{INFINITY, 0};
+    for (uint32_t r = 0; r < k; ++r) {
+        Candidate next = none;
+        for (uint32_t j = threadIdx.x; j < n; j += kMergeThreads) {
+            const Candidate c = value(j);
+            if (c.score > -INFINITY && before(last, c) && before(c, next)) next = c;
+        }
+        sh.best[threadIdx.x] = next;
+        __syncthreads();
+        for (uint32_t half = kMergeThreads / 2; half > 0; half /= 2) {
+            if (threadIdx.x < half && before(sh.best[threadIdx.x + half], sh.best[threadIdx.x])) sh.best[threadIdx.x] = sh.best[threadIdx.x + half];
+            __syncthreads();
+        }
+        last = sh.best[0];
+        if (threadIdx.x == 0) out[r] = last;
+        __syncthreads();
+    }
+    return k;  // (more than kCandidates >= k were found)
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArgs a) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    MergeShared& sh = *reinterpret_cast<MergeShared*>(raw);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t batch = blockIdx.x, row0 = batch * a.beams;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // log-sum-exp of every row from its splits, in 64 bits
+    for (uint32_t w = warp; w < a.beams; w += kMergeThreads / 32) {
+        const uint32_t row = row0 + w;
+        const bool ended = a.finished && __ldg(a.finished + row) && isfinite(__ldg(a.beam_scores + row));
+        bool counts = row_counts(a, row);
+        double base = 0.0;
+        float top = -INFINITY;
+        if (counts) {
+            for (uint32_t s = lane; s < a.splits; s += 32) top = fmaxf(top, a.partial[static_cast<size_t>(row) * a.splits + s].x);
+#pragma unroll
+            for (uint32_t o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+            double sum = 0.0;
+            for (uint32_t s = lane; s < a.splits; s += 32) {
+                const float2 p = a.partial[static_cast<size_t>(row) * a.splits + s];
+                if (p.y != 0.0f) sum += p.y * exp(static_cast<double>(p.x) - top);
+            }
+#pragma unroll
+            for (uint32_t o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(kFullMask, sum, o);
+            // (the top stays apart: among logits of 3e38 a sum with it would lose the rest)
+            const double below = log(sum);
+            counts = isfinite(below) && isfinite(top);
+            base = static_cast<double>(__ldg(a.beam_scores + row)) - below;
+        }
+        if (lane == 0) {
+            sh.base[w] = ended ? static_cast<double>(__ldg(a.beam_scores + row)) : base;
+            sh.top[w] = top;
+            sh.counts[w] = counts;
+            sh.ended[w] = ended;
+        }
+    }
+    __syncthreads();
+    // the best segments; a finished beam is one entry, in the place of its first segment
+    const uint32_t listed = a.beams * a.segments;
+    const uint32_t segments = select(sh, listed, a.k, sh.segments, [&](uint32_t j) {
+        const uint32_t w = j / a.segments, s = j - w * a.segments;
+        Candidate c{-INFINITY, j};
+        if (sh.counts[w]) {
+            const uint32_t lead = row_lead(static_cast<const T*>(a.logits) + (row0 + w) * a.stride);
+            if (s * kSegment < lead + a.vocab) c.score = (a.segment_max[static_cast<size_t>(row0) * a.segments + j] - sh.top[w]) + sh.base[w];
+        } else if (sh.ended[w] && s == 0) {
+            c.score = sh.base[w];
+        }
+        return c;
+    });
+    // the best of their elements
+    const uint32_t elements = select(sh, segments * kSegment, a.k, sh.elements, [&](uint32_t j) {
+        const uint32_t at = sh.segments[j / kSegment].index, w = at / a.segments, s = at - w * a.segments;
+        Candidate c{-INFINITY, 0};
+        if (sh.ended[w]) {
+            if (j % kSegment == 0) c = Candidate{sh.base[w], w * a.vocab + a.pad_token};
+            return c;
+        }
+        const T* logits = static_cast<const T*>(a.logits) + (row0 + w) * a.stride;
+        const uint32_t position = s * kSegment + j % kSegment, lead = row_lead(logits);
+        if (position >= lead && position - lead < a.vocab) {
+            c.score = (logit_value(__ldg(logits + (position - lead))) - sh.top[w]) + sh.base[w];
+            c.index = w * a.vocab + (position - lead);
+        }
+        return c;
+    });
+    for (uint32_t r = threadIdx.x; r < a.k; r += kMergeThreads) {
+        uint32_t index = 0;
+        float score = -INFINITY;
+        if (r < elements) {
+            index = sh.elements[r].index;
+            score = static_cast<float>(sh.elements[r].score);
+        } else {
+            // candidates without a finite score, in order: the (r - elements)-th index that is not among the ones above
+            index = r - elements;
+            bool moved = true;
+            while (moved) {  // (every taken index at or below it moves it on by one; it settles after `elements` steps at most)
+                uint32_t taken = 0;
+                for (uint32_t e = 0; e < elements; ++e) taken += sh.elements[e].index <= index;
+                const uint32_t next = r - elements + taken;
+                moved = next != index;
+                index = next;
+            }
+        }
+        const size_t at = static_cast<size_t>(batch) * a.k + r;
+        a.out_scores[at] = score;
+        a.out_parents[at] = static_cast<int32_t>(index / a.vocab);
+        a.out_tokens[at] = static_cast<int32_t>(index % a.vocab);
+    }
+}
+
+// ---- states ------------------------------------------------------------------------------------------------
+// dst[batch][beam] = src[batch][parents[batch][beam]], several states in one launch.  Bound: HBM, every row read and written once (a
+// row with several children comes out of L2 again).  A CTA copies a stretch of one row, four 16-byte pieces a thread on their way.
+constexpr uint32_t kStates = 24;  // of a launch
+constexpr uint32_t kCopyThreads = 256;
+constexpr uint32_t kStretch = kCopyThreads * 4 * 16;
+struct ReorderArgs {
+    const uint8_t* src[kStates];
+    uint8_t* dst[kStates];
+    size_t row_bytes[kStates];
+    const int32_t* parents;
+    size_t parent_stride;
+    uint32_t beams;
+};
+__global__ void __launch_bounds__(kCopyThreads) beam_reorder_kernel(const ReorderArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t row = blockIdx.x, batch = row / a.beams, beam = row - batch * a.beams;
+    const size_t bytes = a.row_bytes[blockIdx.z];
+    const int32_t parent = __ldg(a.parents + batch * a.parent_stride + beam);
+    if (parent < 0 || static_cast<uint32_t>(parent) >= a.beams) return;  // (no such beam: the row stays as it is)
+    const uint8_t* src = a.src[blockIdx.z] + (static_cast<size_t>(batch) * a.beams + parent) * bytes;
+    uint8_t* dst = a.dst[blockIdx.z] + static_cast<size_t>(row) * bytes;
+    const bool wide = ((reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst)) & 15) == 0;
+    for (size_t at = static_cast<size_t>(blockIdx.y) * kStretch; at < bytes; at += static_cast<size_t>(gridDim.y) * kStretch) {
+        const size_t left = bytes - at;
+        size_t done = 0;
+        if (wide) {
+            uint4 q[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const size_t o = (j * kCopyThreads + threadIdx.x) * 16;
+                if (o + 16 <= left) q[j] = __ldg(reinterpret_cast<const uint4*>(src + at + o));
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const size_t o = (j * kCopyThreads + threadIdx.x) * 16;
+                if (o + 16 <= left) *reinterpret_cast<uint4*>(dst + at + o) = q[j];
+            }
+            done = left / 16 * 16;
+        }
+        for (size_t o = done + threadIdx.x; o < left && o < kStretch; o += kCopyThreads) dst[at + o] = __ldg(src + at + o);
+    }
+}
+
+uint32_t segments_of(uint32_t vocab, bool bf16) { return (vocab + (bf16 ? 7 : 3) + kSegment - 1) / kSegment; }
+// Splits of a row: four CTAs an SM at least while a split keeps a few thousand logits.
+uint32_t vectors_per_split(uint32_t rows, uint32_t vocab, bool bf16) {
+    const uint32_t elems = bf16 ? 8 : 4, vectors = (vocab + elems - 1) / elems + 1;
+    const uint32_t wanted = std::max(1u, (148u * 4u + rows - 1) / rows);
+    const uint32_t per = (vectors + wanted - 1) / wanted;
+    return (std::max(per, 1u) + kScanThreads - 1) / kScanThreads * kScanThreads;
+}
+uint32_t splits_of(uint32_t rows, uint32_t vocab, bool bf16) {
+    const uint32_t elems = bf16 ? 8 : 4, vectors = (vocab + elems - 1) / elems + 1, per = vectors_per_split(rows, vocab, bf16);
+    return (vectors + per - 1) / per;
+}
+bool beam_shape_ok(uint32_t batch, uint32_t beams, uint32_t vocab) {
+    return batch != 0 && beams != 0 && beams <= kMaxBeams && vocab != 0 && batch <= 0xffffu / beams && vocab <= 0x7fffffffu / beams - 64;
+}
+
+}  // namespace
+}  // namespace eider
+
+using namespace eider;
+
+extern "C" {
+
+size_t eider_b200_beam_select_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, int logits_are_bf16) {
+    if (!beam_shape_ok(batch, beams, vocab)) return 0;
+    const size_t rows = static_cast<size_t>(batch) * beams;
+    return rows * (splits_of(batch * beams, vocab, logits_are_bf16) * sizeof(float2) + segments_of(vocab, logits_are_bf16) * sizeof(float));
+}
+
+cudaError_t eider_b200_beam_select_on_stream(const void* logits, int logits_are_bf16, size_t row_stride, const float* beam_scores,
+                                             const uint8_t* finished, uint32_t pad_token, float* out_scores, int32_t* out_parents,
+                                             int32_t* out_tokens, uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t k, void* workspace,
+                                             size_t workspace_bytes, cudaStream_t stream) {
+    if (!logits || !beam_scores || !out_scores || !out_parents || !out_tokens || !workspace || !beam_shape_ok(batch, beams, vocab) ||
+        row_stride < vocab || k == 0 || k > kMaxK || k > static_cast<uint64_t>(beams) * vocab || (finished && pad_token >= vocab) ||
+        (reinterpret_cast<uintptr_t>(logits) & (logits_are_bf16 ? 1 : 3)) != 0 || (reinterpret_cast<uintptr_t>(workspace) & 7) != 0 ||
+        workspace_bytes < eider_b200_beam_select_workspace_bytes(batch, beams, vocab, logits_are_bf16))
+        return cudaErrorInvalidValue;
+    BeamArgs a{};
+    const uint32_t rows = batch * beams;
+    a.logits = logits;
+    a.stride = row_stride;
+    a.beam_scores = beam_scores;
+    a.finished = finished;
+    a.out_scores = out_scores;
+    a.out_parents = out_parents;
+    a.out_tokens = out_tokens;
+    a.beams = beams;
+    a.vocab = vocab;
+    a.k = k;
+    a.pad_token = pad_token;
+    a.segments = segments_of(vocab, logits_are_bf16);
+    a.vectors_per_split = vectors_per_split(rows, vocab, logits_are_bf16);
+    a.splits = splits_of(rows, vocab, logits_are_bf16);
+    a.partial = static_cast<float2*>(workspace);
+    a.segment_max = reinterpret_cast<float*>(a.partial + static_cast<size_t>(rows) * a.splits);
+    const dim3 scan(a.splits, rows);
+    cudaError_t st = logits_are_bf16 ? launch_dependent(beam_scan_kernel<uint16_t>, scan, kScanThreads, 0, stream, a)
+                                     : launch_dependent(beam_scan_kernel<float>, scan, kScanThreads, 0, stream, a);
+    if (st != cudaSuccess) return st;
+    return logits_are_bf16 ? launch_dependent(beam_merge_kernel<uint16_t>, dim3(batch), kMergeThreads, sizeof(MergeShared), stream, a)
+                           : launch_dependent(beam_merge_kernel<float>, dim3(batch), kMergeThreads, sizeof(MergeShared), stream, a);
+}
+
+cudaError_t eider_b200_beam_reorder_on_stream(const void* const* src, void* const* dst, const size_t* row_bytes, uint32_t count,
+                                              const int32_t* parents, size_t parent_stride, uint32_t batch, uint32_t beams, cudaStream_t stream) {
+    if (!src || !dst || !row_bytes || count == 0 || !parents || batch == 0 || beams == 0 || parent_stride < beams ||
+        static_cast<uint64_t>(batch) * beams > 0x7fffffffu)
+        return cudaErrorInvalidValue;
+    for (uint32_t i = 0; i < count; ++i) {
+        if (!src[i] || !dst[i] || row_bytes[i] == 0) return cudaErrorInvalidValue;
+        // (rows are read after others have been written: a state cannot be reordered in place)
+        const auto s = reinterpret_cast<uintptr_t>(src[i]), d = reinterpret_cast<uintptr_t>(dst[i]);
+        const uintptr_t bytes = row_bytes[i] * batch * beams;
+        if (s < d + bytes && d < s + bytes) return cudaErrorInvalidValue;
+    }
+    for (uint32_t first = 0; first < count; first += kStates) {
+        ReorderArgs a{};
+        const uint32_t states = std::min(kStates, count - first);
+        size_t longest = 0;
+        for (uint32_t i = 0; i < states; ++i) {
+            a.src[i] = static_cast<const uint8_t*>(src[first + i]);
+            a.dst[i] = static_cast<uint8_t*>(dst[first + i]);
+            a.row_bytes[i] = row_bytes[first + i];
+            longest = std::max(longest, a.row_bytes[i]);
+        }
+        a.parents = parents;
+        a.parent_stride = parent_stride;
+        a.beams = beams;
+        const uint32_t stretches = static_cast<uint32_t>(std::min<size_t>((longest + kStretch - 1) / kStretch, 1024));
+        const cudaError_t st = launch_dependent(beam_reorder_kernel, dim3(batch * beams, stretches, states), kCopyThreads, 0, stream, a);
+        if (st != cudaSuccess) return st;
+    }
+    return cudaSuccess;
+}
+
+}  // extern "C"

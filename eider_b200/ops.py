@@ -1342,6 +1342,69 @@ class GroupedMoe:
             return moe_weighted_accumulate(self.routes, weights.reshape(-1), self.down_out, self.tokens, self.top_k, out=out)
 
 
+# ---- beam search --------------------------------------------------------------------------------------------
+def beam_search_select(logits: torch.Tensor, beam_scores: torch.Tensor, k: int, finished: torch.Tensor | None = None, pad_token: int = 0):
+    """The k best continuations of every sequence over its beams and the vocabulary: logits [batch, beams, vocab] (f32 or bf16, e.g.
+    an lm-head's over batch * beams tokens), beam_scores [batch, beams] f32.  Returns (scores [batch, k] f32, parents [batch, k] int32,
+    tokens [batch, k] int32), best first, equal scores by the lower beam * vocab + token.  A beam marked in `finished` (bool or u8
+    [batch, beams]) goes on only as (pad_token, its score)."""
+    if logits.dim() != 3 or not logits.is_cuda or logits.dtype not in (torch.float32, torch.bfloat16) or logits.numel() == 0:
+        raise ShapeError("logits must be a CUDA tensor [batch, beams, vocab] of f32 or bf16")
+    batch, beams, vocab = logits.shape
+    row = logits.stride(1) if beams > 1 else logits.stride(0) if batch > 1 else vocab
+    if logits.stride(2) != 1 or row < vocab or (batch > 1 and logits.stride(0) != beams * row):
+        raise ShapeError("logits must have contiguous rows at one distance")
+    if beam_scores.shape != (batch, beams):
+        raise ShapeError(f"beam_scores must be [{batch}, {beams}], got {tuple(beam_scores.shape)}")
+    _need(beam_scores, torch.float32, "beam_scores")
+    if finished is not None:
+        if finished.shape != (batch, beams) or finished.dtype not in (torch.bool, torch.uint8):
+            raise ShapeError(f"finished must be bool or u8 [{batch}, {beams}]")
+        _need(finished, finished.dtype, "finished")
+        if not 0 <= pad_token < vocab:
+            raise ShapeError(f"pad_token must be a token, got {pad_token}")
+    device, bf16 = logits.device, int(logits.dtype == torch.bfloat16)
+    _need_device(device, beam_scores, finished)
+    size = _lib.load().eider_b200_beam_select_workspace_bytes(batch, beams, vocab, bf16)
+    if size == 0 or not 0 < k <= min(128, beams * vocab):
+        raise ShapeError(f"unsupported beam search batch={batch} beams={beams} vocab={vocab} k={k}")
+    out = torch.empty(3, batch, k, dtype=torch.int32, device=device)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    scores, parents, tokens = out.unbind(0)
+    _call(device, "eider_b200_beam_select_on_stream", logits.data_ptr(), bf16, row, beam_scores.data_ptr(), _ptr(finished), pad_token if finished is not None else 0,
+          scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), batch, beams, vocab, k, workspace.data_ptr(), size)
+    return scores.view(torch.float32), parents, tokens
+
+
+def beam_search_reorder(states: list, parents: torch.Tensor, out: list | None = None) -> list:
+    """The beams' states behind a selection: out[i][b, j] = states[i][b, parents[b, j]] for tensors [batch, beams, ...] of any type.
+    `parents` [batch, beams] int32 (rows may be apart, as in the first `beams` columns of a selection).  Never in place: `out`
+    takes other tensors of the same shapes, e.g. the second of two sets that a decode loop swaps.  A parent that is no beam leaves its
+    row of `out` as it is."""
+    if parents.dim() != 2 or not parents.is_cuda or parents.dtype != torch.int32 or parents.numel() == 0 or parents.stride(1) != 1:
+        raise ShapeError("parents must be a CUDA tensor [batch, beams] of int32")
+    batch, beams = parents.shape
+    stride = parents.stride(0) if batch > 1 else beams
+    if stride < beams:
+        raise ShapeError("rows of parents overlap")
+    if out is None:
+        out = [torch.empty_like(t) for t in states]
+    if not states or len(out) != len(states):
+        raise ShapeError("as many outputs as states are wanted, and one at least")
+    for s, o in zip(states, out):
+        if s.shape[:2] != (batch, beams) or s.numel() == 0 or o.shape != s.shape or o.dtype != s.dtype or not s.is_contiguous() or not o.is_contiguous():
+            raise ShapeError(f"states must be contiguous [{batch}, {beams}, ...], and outputs like them")
+        first, other, size = s.data_ptr(), o.data_ptr(), s.numel() * s.element_size()
+        if first < other + size and other < first + size:
+            raise ShapeError("a state cannot be reordered in place")
+    _need_device(parents.device, *states, *out)
+    n = len(states)
+    rows = (C.c_size_t * n)(*[s.numel() // (batch * beams) * s.element_size() for s in states])
+    _call(parents.device, "eider_b200_beam_reorder_on_stream", (C.c_void_p * n)(*[s.data_ptr() for s in states]),
+          (C.c_void_p * n)(*[o.data_ptr() for o in out]), rows, n, parents.data_ptr(), stride, batch, beams)
+    return out
+
+
 # ---- operator composition ---------------------------------------------------------------------------------
 class DenseFfn:
     """The dense gated FFN as the reference composes it for a batch of rows (crates/infer/src/qwen3/qwen36.rs:7175-7280):

@@ -894,6 +894,24 @@ EIDER_B200_API cudaError_t eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_
                                                                                        uint32_t rows, uint32_t len, uint32_t routes_per_row,
                                                                                        cudaStream_t stream);
 
+/* ---- beam search (beside the lm-head arg-max above; the reference decodes one hypothesis) -------------------
+ * score[r][v] = beam_scores[r] + log_softmax(logits[r])[v] for the batch x beams rows of logits (f32 or bf16, `row_stride` elements
+ * apart); per sequence the k largest over its beams x vocab scores in descending order, compared in 64 bits, equal ones in the order
+ * of beam * vocab + v.  A finished beam (finished may be NULL) has one candidate, pad_token, with its score unchanged.  A row
+ * whose beam score or log-sum-exp is not finite (a NaN or +infinity among its logits, or nothing above -infinity) has candidates of
+ * score -infinity only; where fewer than k scores are finite, candidates of score -infinity follow in the order of their index.
+ * beams <= 64, k <= 128 and <= beams * vocab, batch * beams <= 65535.  The workspace (8-byte aligned) is one call's. */
+EIDER_B200_API size_t eider_b200_beam_select_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, int logits_are_bf16);
+EIDER_B200_API cudaError_t eider_b200_beam_select_on_stream(const void* logits, int logits_are_bf16, size_t row_stride, const float* beam_scores,
+                                                            const uint8_t* finished, uint32_t pad_token, float* out_scores, int32_t* out_parents,
+                                                            int32_t* out_tokens, uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t k,
+                                                            void* workspace, size_t workspace_bytes, cudaStream_t stream);
+/* dst[i][b][j] = src[i][b][parents[b][j]] for `count` states of rows of row_bytes[i] bytes (host arrays of device pointers; read before
+ * the call returns).  No state may overlap its destination.  A parent outside 0 .. beams - 1 leaves its row as it is. */
+EIDER_B200_API cudaError_t eider_b200_beam_reorder_on_stream(const void* const* src, void* const* dst, const size_t* row_bytes, uint32_t count,
+                                                             const int32_t* parents, size_t parent_stride, uint32_t batch, uint32_t beams,
+                                                             cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
