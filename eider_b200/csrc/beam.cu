@@ -12,6 +12,7 @@
 // their elements.  Nothing of the order of vocab is written or sorted; no atomics decide an order.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "common.cuh"
 #include "quant_block.cuh"
@@ -24,7 +25,7 @@ constexpr uint32_t kFullMask = 0xffffffffu;
 constexpr uint32_t kSegment = 64;       // logits that share a maximum
 constexpr uint32_t kScanThreads = 256;
 constexpr uint32_t kAhead = 4;          // 16-byte vectors a thread has on their way
-constexpr uint32_t kMergeThreads = 512;
+constexpr uint32_t kMergeThreads = 1024;
 constexpr uint32_t kCandidates = 2048;  // of a selection; more are taken one by one
 constexpr uint32_t kMaxBeams = 64, kMaxK = 128;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -54,6 +55,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 template <typename T> struct Vec {
     static constexpr uint32_t kElems = 16 / sizeof(T);
 };
+template <typename T> __device__ __forceinline__ T minus_infinity();
+template <> __device__ __forceinline__ float minus_infinity<float>() { return -INFINITY; }
+template <> __device__ __forceinline__ uint16_t minus_infinity<uint16_t>() { return 0xff80; }
 __device__ __forceinline__ float logit_value(float v) { return v; }
 __device__ __forceinline__ float logit_value(uint16_t v) { return bf16_bits_to_float(v); }
 __device__ __forceinline__ void vector_values(const uint4& q, float (&v)[4]) {
@@ -84,38 +88,67 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const BeamArgs 
     const uint32_t v1 = min((blockIdx.x + 1) * a.vectors_per_split, (end + E - 1) / E);
     float* segment_max = a.segment_max + static_cast<size_t>(row) * a.segments;
     float top = -INFINITY, sum = 0.0f;
-    // (whole warps run the same number of turns: the split is a multiple of the block)
-    for (uint32_t base = blockIdx.x * a.vectors_per_split; base < v1; base += kScanThreads * kAhead) {
-        float x[kAhead][E];
+    // A turn's vectors, requested while the turn before is worked on.  (Whole warps run the same number of turns: a split is a
+    // multiple of the block.)
+    uint4 next[kAhead];
+    auto fetch = [&](uint32_t base) {
+        const bool inside = base + kScanThreads * kAhead <= v1 && base * E >= lead && (base + kScanThreads * kAhead) * E <= end;
+        const uint4* vectors = reinterpret_cast<const uint4*>(logits - lead) + base + threadIdx.x;
+        if (inside) {
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead; ++j) next[j] = __ldg(vectors + j * kScanThreads);
+            return;
+        }
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
             const uint32_t vec = base + j * kScanThreads + threadIdx.x, at = vec * E;
             if (vec < v1 && at >= lead && at + E <= end) {
-                vector_values(__ldg(reinterpret_cast<const uint4*>(logits - lead) + vec), x[j]);
-            } else {  // the row's first and last vectors
+                next[j] = __ldg(vectors + j * kScanThreads);
+            } else {  // the row's first and last vectors, and none
+                T v[E];
 #pragma unroll
-                for (uint32_t e = 0; e < E; ++e) x[j][e] = vec < v1 && at + e >= lead && at + e < end ? logit_value(__ldg(logits + (at + e - lead))) : -INFINITY;
+                for (uint32_t e = 0; e < E; ++e) v[e] = vec < v1 && at + e >= lead && at + e < end ? __ldg(logits + (at + e - lead)) : minus_infinity<T>();
+                memcpy(&next[j], v, 16);
             }
+        }
+    };
+    uint32_t base = blockIdx.x * a.vectors_per_split;
+    if (base < v1) fetch(base);
+    for (; base < v1; base += kScanThreads * kAhead) {
+        uint4 now[kAhead];
+        float m[kAhead];
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) now[j] = next[j];
+        if (base + kScanThreads * kAhead < v1) fetch(base + kScanThreads * kAhead);
+        float new_top = top;
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            float x[E];
+            vector_values(now[j], x);
+            m[j] = x[0];
+#pragma unroll
+            for (uint32_t e = 1; e < E; ++e) m[j] = fmaxf(m[j], x[e]);
+            new_top = fmaxf(new_top, m[j]);
+        }
+        // (with nothing but -infinity so far, differences to 0 keep the sum 0, or NaN for a NaN, which passes the maximum by)
+        const float to = new_top > -INFINITY ? new_top : 0.0f;
+        sum *= exp2_fast((top - to) * kLog2e);
+        top = new_top;
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            float x[E];
+            vector_values(now[j], x);
+            float part = 0.0f;
+#pragma unroll
+            for (uint32_t e = 0; e < E; ++e) part += exp2_fast((x[e] - to) * kLog2e);
+            sum += part;
         }
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
-            float m = x[j][0];
 #pragma unroll
-            for (uint32_t e = 1; e < E; ++e) m = fmaxf(m, x[j][e]);
-            const float new_top = fmaxf(top, m);
-            if (new_top > -INFINITY) {
-                sum *= exp2_fast((top - new_top) * kLog2e);
-#pragma unroll
-                for (uint32_t e = 0; e < E; ++e) sum += exp2_fast((x[j][e] - new_top) * kLog2e);
-                top = new_top;
-            } else {
-#pragma unroll
-                for (uint32_t e = 0; e < E; ++e) sum += x[j][e] != x[j][e] ? x[j][e] : 0.0f;  // (NaNs pass the maximum by)
-            }
-#pragma unroll
-            for (uint32_t o = 1; o < kSegLanes; o *= 2) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
+            for (uint32_t o = 1; o < kSegLanes; o *= 2) m[j] = fmaxf(m[j], __shfl_xor_sync(kFullMask, m[j], o));
             const uint32_t vec = base + j * kScanThreads + threadIdx.x;
-            if (threadIdx.x % kSegLanes == 0 && vec < v1) segment_max[vec / kSegLanes] = m;
+            if (threadIdx.x % kSegLanes == 0 && vec < v1) segment_max[vec / kSegLanes] = m[j];
         }
     }
     __shared__ float tops[kScanThreads / 32], sums[kScanThreads / 32];
@@ -149,48 +182,62 @@ struct Candidate {
     uint32_t index;
 };
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) { return a.score > b.score || (a.score == b.score && a.index < b.index); }
+// The upper half of a score as an integer of the same order (20 bits of mantissa; -0 below 0 only splits what is then compared whole).
+__device__ __forceinline__ int score_key(double score) {
+    const int h = __double2hiint(score + 0.0);
+    return h ^ ((h >> 31) & 0x7fffffff);
+}
+constexpr int kNoKey = static_cast<int>(0x80000000);
 
 struct MergeShared {
-    Candidate best[kMergeThreads];       // a thread's best
     Candidate candidates[kCandidates];
     Candidate segments[kMaxK], elements[kMaxK];
+    Candidate best[kMergeThreads / 32];
     double base[kMaxBeams], top[kMaxBeams];  // a row's scores are (logit - top) + base: base = beam score - log of the sum below top
     uint8_t counts[kMaxBeams], ended[kMaxBeams];
-    Candidate threshold;
+    int low, high;
     uint32_t found;
 };
 
-// The best `k` (fewer, if fewer have a finite score) of value(0 .. n - 1), in order, into `out`; returns how many.  A thread's best
-// values rank the threads; what is not behind the k-th best thread's best is a candidate, and candidates are ranked by counting.
-template <typename Value>
-__device__ __forceinline__ uint32_t select(MergeShared& sh, uint32_t n, uint32_t k, Candidate* out, Value value) {
-    const Candidate none{-INFINITY, 0xffffffffu};
-    Candidate mine = none;
-    for (uint32_t j = threadIdx.x; j < n; j += kMergeThreads) {
-        const Candidate c = value(j);
-        if (c.score > -INFINITY && before(c, mine)) mine = c;
-    }
-    sh.best[threadIdx.x] = mine;
+// The best `k` (fewer, if fewer have a finite score) of the entries that each(use) hands to use(candidate), spread over the threads and
+// the same ones in every pass, in order, into `out`; returns how many.  The k-th largest of the threads' best keys, found by
+// bisection with one counting barrier a step, bounds the k-th best entry from below; what is not under it (a few more than k
+// entries) is ranked by counting, in 64 bits.
+template <typename Each>
+__device__ __forceinline__ uint32_t select(MergeShared& sh, uint32_t k, Candidate* out, Each each) {
+    int key = kNoKey;
+    each([&](const Candidate& c) {
+        if (c.score > -INFINITY) key = max(key, score_key(c.score));
+    });
     if (threadIdx.x == 0) {
-        sh.threshold = none;
+        sh.low = 0x7fffffff;
+        sh.high = kNoKey;
         sh.found = 0;
     }
-    const bool any = mine.score > -INFINITY;
-    const uint32_t threads = __syncthreads_count(any);
-    if (any && threads >= k) {
-        uint32_t rank = 0;
-        for (uint32_t t = 0; t < kMergeThreads; ++t) rank += before(sh.best[t], mine);
-        if (rank == k - 1) sh.threshold = mine;
+    const uint32_t threads = __syncthreads_count(key != kNoKey);
+    int threshold = kNoKey + 1;  // every finite score
+    if (threads >= k) {
+        const int highest = __reduce_max_sync(kFullMask, key), lowest = __reduce_min_sync(kFullMask, key == kNoKey ? 0x7fffffff : key);
+        if (threadIdx.x % 32 == 0) {
+            atomicMax(&sh.high, highest);
+            atomicMin(&sh.low, lowest);
+        }
+        __syncthreads();
+        // at least k threads have `low` or more, fewer than k have more than `high`; a few steps short of the end it is near enough
+        int low = sh.low, high = sh.high;
+        for (int step = 0; step < 20 && low < high; ++step) {
+            const int mid = static_cast<int>((static_cast<long long>(low) + high + 1) >> 1);
+            if (static_cast<uint32_t>(__syncthreads_count(key >= mid)) >= k) low = mid;
+            else high = mid - 1;
+        }
+        threshold = low;
     }
-    __syncthreads();
-    const Candidate threshold = sh.threshold;
-    for (uint32_t j = threadIdx.x; j < n; j += kMergeThreads) {
-        const Candidate c = value(j);
-        if (c.score > -INFINITY && !before(threshold, c)) {
+    each([&](const Candidate& c) {
+        if (c.score > -INFINITY && score_key(c.score) >= threshold) {
             const uint32_t at = atomicAdd(&sh.found, 1u);
             if (at < kCandidates) sh.candidates[at] = c;
         }
-    }
+    });
     __syncthreads();
     const uint32_t found = sh.found;
     if (found <= kCandidates) {
@@ -203,21 +250,25 @@ __device__ __forceinline__ uint32_t select(MergeShared& sh, uint32_t n, uint32_t
         __syncthreads();
         return min(found, k);
     }
-    // Too many to rank (long runs of equal scores among few threads): the next one in order, k times.
+    // Too many to rank (long runs of equal scores): the next one in order, k times.
     Candidate last{INFINITY, 0};
     for (uint32_t r = 0; r < k; ++r) {
-        Candidate next = none;
-        for (uint32_t j = threadIdx.x; j < n; j += kMergeThreads) {
-            const Candidate c = value(j);
+        Candidate next{-INFINITY, 0xffffffffu};
+        each([&](const Candidate& c) {
             if (c.score > -INFINITY && before(last, c) && before(c, next)) next = c;
-        }
-        sh.best[threadIdx.x] = next;
+        });
+        auto join = [&](uint32_t o) {
+            const Candidate other{__shfl_xor_sync(kFullMask, next.score, o), __shfl_xor_sync(kFullMask, next.index, o)};
+            if (before(other, next)) next = other;
+        };
+#pragma unroll
+        for (uint32_t o = 16; o > 0; o /= 2) join(o);
+        if (threadIdx.x % 32 == 0) sh.best[threadIdx.x / 32] = next;
         __syncthreads();
-        for (uint32_t half = kMergeThreads / 2; half > 0; half /= 2) {
-            if (threadIdx.x < half && before(sh.best[threadIdx.x + half], sh.best[threadIdx.x])) sh.best[threadIdx.x] = sh.best[threadIdx.x + half];
-            __syncthreads();
-        }
-        last = sh.best[0];
+        next = sh.best[threadIdx.x % (kMergeThreads / 32)];
+#pragma unroll
+        for (uint32_t o = 16; o > 0; o /= 2) join(o);
+        last = next;
         if (threadIdx.x == 0) out[r] = last;
         __syncthreads();
     }
@@ -232,20 +283,22 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t batch = blockIdx.x, row0 = batch * a.beams;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    // log-sum-exp of every row from its splits, in 64 bits
+    // the sum of exponentials of every row from its splits, in 64 bits
     for (uint32_t w = warp; w < a.beams; w += kMergeThreads / 32) {
         const uint32_t row = row0 + w;
         const bool ended = a.finished && __ldg(a.finished + row) && isfinite(__ldg(a.beam_scores + row));
         bool counts = row_counts(a, row);
-        double base = 0.0;
-        float top = -INFINITY;
+        double base = __ldg(a.beam_scores + row);
+        float top = 0.0f;
         if (counts) {
-            for (uint32_t s = lane; s < a.splits; s += 32) top = fmaxf(top, a.partial[static_cast<size_t>(row) * a.splits + s].x);
+            const float2* partial = a.partial + static_cast<size_t>(row) * a.splits;
+            top = -INFINITY;
+            for (uint32_t s = lane; s < a.splits; s += 32) top = fmaxf(top, partial[s].x);
 #pragma unroll
             for (uint32_t o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
             double sum = 0.0;
             for (uint32_t s = lane; s < a.splits; s += 32) {
-                const float2 p = a.partial[static_cast<size_t>(row) * a.splits + s];
+                const float2 p = partial[s];
                 if (p.y != 0.0f) sum += p.y * exp(static_cast<double>(p.x) - top);
             }
 #pragma unroll
@@ -253,44 +306,53 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             // (the top stays apart: among logits of 3e38 a sum with it would lose the rest)
             const double below = log(sum);
             counts = isfinite(below) && isfinite(top);
-            base = static_cast<double>(__ldg(a.beam_scores + row)) - below;
+            base -= below;
         }
         if (lane == 0) {
-            sh.base[w] = ended ? static_cast<double>(__ldg(a.beam_scores + row)) : base;
+            sh.base[w] = base;
             sh.top[w] = top;
             sh.counts[w] = counts;
             sh.ended[w] = ended;
         }
     }
     __syncthreads();
-    // the best segments; a finished beam is one entry, in the place of its first segment
-    const uint32_t listed = a.beams * a.segments;
-    const uint32_t segments = select(sh, listed, a.k, sh.segments, [&](uint32_t j) {
-        const uint32_t w = j / a.segments, s = j - w * a.segments;
-        Candidate c{-INFINITY, j};
-        if (sh.counts[w]) {
-            const uint32_t lead = row_lead(static_cast<const T*>(a.logits) + (row0 + w) * a.stride);
-            if (s * kSegment < lead + a.vocab) c.score = (a.segment_max[static_cast<size_t>(row0) * a.segments + j] - sh.top[w]) + sh.base[w];
-        } else if (sh.ended[w] && s == 0) {
-            c.score = sh.base[w];
+    // The best segments: a row's maxima are read by a warp or several, eight a lane on their way; a finished beam is one entry, in the
+    // place of its first segment.
+    const float* maxima = a.segment_max + static_cast<size_t>(row0) * a.segments;
+    constexpr uint32_t kWarps = kMergeThreads / 32, kFetch = 8;
+    const uint32_t parts = (kWarps + a.beams - 1) / a.beams, per_part = (a.segments + parts - 1) / parts;
+    const uint32_t segments = select(sh, a.k, sh.segments, [&](auto use) {
+        for (uint32_t item = warp; item < a.beams * parts; item += kWarps) {
+            const uint32_t w = item / parts, part = item - w * parts;
+            if (!sh.counts[w]) {
+                if (sh.ended[w] && part == 0 && lane == 0) use(Candidate{sh.base[w], w * a.segments});
+                continue;
+            }
+            const double top = sh.top[w], base = sh.base[w];
+            const uint32_t used = (row_lead(static_cast<const T*>(a.logits) + (row0 + w) * a.stride) + a.vocab + kSegment - 1) / kSegment;
+            const uint32_t last = min((part + 1) * per_part, used);
+            for (uint32_t s = part * per_part + lane; s < last; s += 32 * kFetch) {
+                float x[kFetch];
+#pragma unroll
+                for (uint32_t i = 0; i < kFetch; ++i) x[i] = s + 32 * i < last ? maxima[static_cast<size_t>(w) * a.segments + s + 32 * i] : -INFINITY;
+#pragma unroll
+                for (uint32_t i = 0; i < kFetch; ++i) use(Candidate{(x[i] - top) + base, w * a.segments + s + 32 * i});
+            }
         }
-        return c;
     });
     // the best of their elements
-    const uint32_t elements = select(sh, segments * kSegment, a.k, sh.elements, [&](uint32_t j) {
-        const uint32_t at = sh.segments[j / kSegment].index, w = at / a.segments, s = at - w * a.segments;
-        Candidate c{-INFINITY, 0};
-        if (sh.ended[w]) {
-            if (j % kSegment == 0) c = Candidate{sh.base[w], w * a.vocab + a.pad_token};
-            return c;
+    const uint32_t elements = select(sh, a.k, sh.elements, [&](auto use) {
+        for (uint32_t j = threadIdx.x; j < segments * kSegment; j += kMergeThreads) {
+            const uint32_t at = sh.segments[j / kSegment].index, w = at / a.segments, s = at - w * a.segments;
+            if (sh.ended[w]) {
+                if (j % kSegment == 0) use(Candidate{sh.base[w], w * a.vocab + a.pad_token});
+                continue;
+            }
+            const T* logits = static_cast<const T*>(a.logits) + (row0 + w) * a.stride;
+            const uint32_t position = s * kSegment + j % kSegment, lead = row_lead(logits);
+            if (position >= lead && position - lead < a.vocab)
+                use(Candidate{(logit_value(__ldg(logits + (position - lead))) - sh.top[w]) + sh.base[w], w * a.vocab + (position - lead)});
         }
-        const T* logits = static_cast<const T*>(a.logits) + (row0 + w) * a.stride;
-        const uint32_t position = s * kSegment + j % kSegment, lead = row_lead(logits);
-        if (position >= lead && position - lead < a.vocab) {
-            c.score = (logit_value(__ldg(logits + (position - lead))) - sh.top[w]) + sh.base[w];
-            c.index = w * a.vocab + (position - lead);
-        }
-        return c;
     });
     for (uint32_t r = threadIdx.x; r < a.k; r += kMergeThreads) {
         uint32_t index = 0;
@@ -363,10 +425,10 @@ __global__ void __launch_bounds__(kCopyThreads) beam_reorder_kernel(const Reorde
 }
 
 uint32_t segments_of(uint32_t vocab, bool bf16) { return (vocab + (bf16 ? 7 : 3) + kSegment - 1) / kSegment; }
-// Splits of a row: four CTAs an SM at least while a split keeps a few thousand logits.
+// Splits of a row: a dozen CTAs an SM, so that the last ones do not leave most SMs idle, while a split keeps a few thousand logits.
 uint32_t vectors_per_split(uint32_t rows, uint32_t vocab, bool bf16) {
     const uint32_t elems = bf16 ? 8 : 4, vectors = (vocab + elems - 1) / elems + 1;
-    const uint32_t wanted = std::max(1u, (148u * 4u + rows - 1) / rows);
+    const uint32_t wanted = std::max(1u, (148u * 12u + rows - 1) / rows);
     const uint32_t per = (vectors + wanted - 1) / wanted;
     return (std::max(per, 1u) + kScanThreads - 1) / kScanThreads * kScanThreads;
 }

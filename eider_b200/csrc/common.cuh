@@ -37,6 +37,19 @@ __host__ __device__ inline size_t tiled_scale_offset(uint32_t outer, uint32_t kb
     return base + (in_tile % 32) * 16 + (in_tile / 32) * 4 + (kb % 4);
 }
 
+// n / d for n < 2^31 by multiplication (d > 0).
+struct FastDiv {
+    uint32_t d, magic, shift;
+    FastDiv() : d(1), magic(1), shift(0) {}
+    explicit FastDiv(uint32_t divisor) : d(divisor), shift(0) {
+        while ((1ull << shift) < d) ++shift;
+        magic = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
+#endif
+};
+
 // E4M3 byte -> f32 (crates/eider-cuda/src/format.rs:121-133).
 __host__ __device__ inline float e4m3_value(uint8_t code) {
     uint32_t sign = static_cast<uint32_t>(code & 0x80) << 24;

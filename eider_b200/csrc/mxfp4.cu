@@ -17,16 +17,6 @@ namespace {
 constexpr uint32_t kFullMask = 0xffffffffu;
 constexpr uint32_t kUnit = 128;
 
-// n / d for n < 2^31 by multiplication (d > 0).
-struct FastDiv {
-    uint32_t d, magic, shift;
-    explicit FastDiv(uint32_t divisor) : d(divisor), shift(0) {
-        while ((1ull << shift) < d) ++shift;
-        magic = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-    }
-    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, magic) + n) >> shift; }
-};
-
 // Eight elements at p, from aligned rows in 16-byte loads.
 template <bool VEC> __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
     if (VEC) {
