@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -353,14 +354,21 @@ class Fp8TnMatmulPlan:
 
 
 # ---- MXFP4 ------------------------------------------------------------------------------------------
+# (torch.cuda.current_stream() builds a stream object for every call: 3.2 us of a call's 16, this takes 0.1)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(device: torch.device, name: str, *args) -> None:
     """One entry point on the current stream of `device` (the device of its tensors, whichever is current)."""
     fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == device.index:
-        check(name, fn(*args, _stream()))
+    index = device.index
+    if torch.cuda.current_device() == index:
+        code = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            check(name, fn(*args, _stream()))
+            code = fn(*args, _raw_stream(index))
+    if code != 0:
+        check(name, code)
 
 
 def _need_floats(t: torch.Tensor, label: str) -> None:
@@ -384,28 +392,53 @@ def mxfp4_scale_layout_len(outer: int, inner: int) -> int:
     return (outer + 127) // 128 * 128 * (((inner + 31) // 32 + 3) // 4 * 4)
 
 
-@dataclass
 class Mxfp4Matrix:
-    """Device MXFP4 matrix: packed E2M1 [rows, K/2] + tiled E8M0 scales, one per 32 elements."""
-    packed: torch.Tensor
-    scales: torch.Tensor
-    rows: int
-    k: int
+    """Device MXFP4 matrix: `packed` E2M1 [rows, K/2] + `scales`, tiled E8M0, one per 32 elements."""
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, rows: int, k: int):
+        if rows <= 0 or k <= 0 or k % 32 != 0 or packed.shape != (rows, k // 2) or scales.numel() < mxfp4_scale_layout_len(rows, k):
+            raise ShapeError(f"codes [{rows}, {k // 2}] with {mxfp4_scale_layout_len(rows, k)} tiled scale bytes are wanted")
+        _need(packed, torch.uint8, "codes")
+        _need(scales, torch.uint8, "scales")
+        _need_device(packed.device, scales)
+        self.rows, self.k, self.device = rows, k, packed.device
+        self._parts = packed, scales
+        self.packed_ptr, self.scales_ptr = packed.data_ptr(), scales.data_ptr()
 
     @staticmethod
     def _unwritten(rows: int, k: int, device) -> "Mxfp4Matrix":
-        """Storage for a quantizer, which writes all of it (zero scales for padding rows and blocks included)."""
+        """Storage for a quantizer, which writes all of it (zero scales for padding rows and blocks included): one allocation, the
+        scales (whole 512-byte tiles) in front of the codes.  The two tensors are made when somebody asks for them."""
         if k % 32 != 0 or k == 0 or rows == 0:
             raise ShapeError(f"MXFP4 needs rows of whole 32-element blocks, got [{rows}, {k}]")
-        return Mxfp4Matrix(torch.empty(rows, k // 2, dtype=torch.uint8, device=device),
-                           torch.empty(mxfp4_scale_layout_len(rows, k), dtype=torch.uint8, device=device), rows, k)
+        m = object.__new__(Mxfp4Matrix)
+        size = mxfp4_scale_layout_len(rows, k)
+        m._storage = torch.empty(size + rows * (k // 2), dtype=torch.uint8, device=device)
+        m.rows, m.k, m.device, m._parts = rows, k, m._storage.device, None
+        m.scales_ptr = m._storage.data_ptr()
+        m.packed_ptr = m.scales_ptr + size
+        return m
+
+    def _split(self):
+        if self._parts is None:
+            size = mxfp4_scale_layout_len(self.rows, self.k)
+            self._parts = self._storage[size:].view(self.rows, self.k // 2), self._storage[:size]
+        return self._parts
+
+    @property
+    def packed(self) -> torch.Tensor:
+        return self._split()[0]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._split()[1]
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         """The values the codes stand for, [rows, K] f32 or bf16 (both hold every E2M1 multiple of a block scale exactly)."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ShapeError(f"values are f32 or bf16, got {dtype}")
-        out = torch.empty(self.rows, self.k, dtype=dtype, device=self.packed.device)
-        _call(out.device, "eider_b200_dequantize_mxfp4_on_stream", self.packed.data_ptr(), self.scales.data_ptr(), out.data_ptr(),
+        out = torch.empty(self.rows, self.k, dtype=dtype, device=self.device)
+        _call(self.device, "eider_b200_dequantize_mxfp4_on_stream", self.packed_ptr, self.scales_ptr, out.data_ptr(),
               int(dtype == torch.bfloat16), self.rows, self.k)
         return out
 
@@ -420,8 +453,8 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Matrix:
     if stride < k:
         raise ShapeError("activation rows overlap")
     out = Mxfp4Matrix._unwritten(tokens, k, x.device)
-    _call(x.device, "eider_b200_quantize_mxfp4_on_stream", x.data_ptr(), int(x.dtype == torch.bfloat16), stride, out.packed.data_ptr(),
-          out.scales.data_ptr(), tokens, k)
+    _call(out.device, "eider_b200_quantize_mxfp4_on_stream", x.data_ptr(), int(x.dtype == torch.bfloat16), stride, out.packed_ptr, out.scales_ptr,
+          tokens, k)
     return out
 
 
@@ -432,8 +465,7 @@ def silu_mul_halves_quantize_mxfp4(gate_up: torch.Tensor) -> Mxfp4Matrix:
     _need(gate_up, torch.float32, "gate_up")
     gate_up = _aligned16(gate_up)
     out = Mxfp4Matrix._unwritten(gate_up.shape[0], gate_up.shape[1] // 2, gate_up.device)
-    _call(gate_up.device, "eider_b200_silu_mul_halves_quantize_mxfp4_on_stream", gate_up.data_ptr(), out.packed.data_ptr(), out.scales.data_ptr(),
-          out.rows, out.k)
+    _call(gate_up.device, "eider_b200_silu_mul_halves_quantize_mxfp4_on_stream", gate_up.data_ptr(), out.packed_ptr, out.scales_ptr, out.rows, out.k)
     return out
 
 
@@ -502,18 +534,20 @@ class _DevicePlan:
         if out is None:
             if dtype not in (torch.float32, torch.bfloat16):
                 raise ShapeError(f"output must be f32 or bf16, got {dtype}")
-            out = torch.empty(shape, dtype=dtype, device=self.device)
-        elif tuple(out.shape) != tuple(shape):
-            raise ShapeError(f"output must be {tuple(shape)}, got {tuple(out.shape)}")
-        _need_floats(out, "output")
+            out = torch.empty(*shape, dtype=dtype, device=self.device)
+        else:
+            if out.shape != shape:
+                raise ShapeError(f"output must be {shape}, got {tuple(out.shape)}")
+            _need_floats(out, "output")
+            _need_device(self.device, out)
         if beta != 0.0:
             c = out if c is None else c
             if c.shape != out.shape or c.dtype != out.dtype:
                 raise ShapeError("C must have the output's shape and type")
             _need(c, c.dtype, "C")
+            _need_device(self.device, c)
         else:
             c = None
-        _need_device(self.device, out, c)
         return out, c
 
     def close(self) -> None:
@@ -549,13 +583,14 @@ class Mxfp4MatmulPlan(_DevicePlan):
     def _operands(self, x: Mxfp4Matrix, w: Mxfp4Weight) -> None:
         if x.rows != self.m or x.k != self.k or w.out_features != self.n or w.in_features != self.k:
             raise ShapeError("operand shapes do not match the plan")
-        _need_device(self.device, x.packed, w.packed)
+        if x.device != self.device or w.packed.device != self.device:
+            raise ShapeError(f"operands must be on {self.device}")
 
     def run(self, x: Mxfp4Matrix, w: Mxfp4Weight, out: torch.Tensor | None = None, alpha: float = 1.0, beta: float = 0.0,
             c: torch.Tensor | None = None, out_dtype=torch.bfloat16) -> torch.Tensor:
         self._operands(x, w)
         out, c = self._output(out, (self.m, self.n), out_dtype, beta, c)
-        _call(self.device, "eider_b200_mxfp4_gemm_tn_on_stream", self._plan, x.packed.data_ptr(), x.scales.data_ptr(), w.packed.data_ptr(),
+        _call(self.device, "eider_b200_mxfp4_gemm_tn_on_stream", self._plan, x.packed_ptr, x.scales_ptr, w.packed.data_ptr(),
               w.scales_tiled.data_ptr(), _ptr(c), out.data_ptr(), alpha, beta, int(out.dtype == torch.bfloat16))
         return out
 
@@ -566,8 +601,8 @@ class Mxfp4MatmulPlan(_DevicePlan):
         if self.n % 256 != 0:
             raise ShapeError("the intermediate size must be a multiple of 128")
         out = Mxfp4Matrix._unwritten(self.m, self.n // 2, self.device)
-        _call(self.device, "eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream", self._plan, x.packed.data_ptr(), x.scales.data_ptr(),
-              w.packed.data_ptr(), w.scales_tiled.data_ptr(), alpha, out.packed.data_ptr(), out.scales.data_ptr())
+        _call(self.device, "eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream", self._plan, x.packed_ptr, x.scales_ptr, w.packed.data_ptr(),
+              w.scales_tiled.data_ptr(), alpha, out.packed_ptr, out.scales_ptr)
         return out
 
     def status(self) -> int:
@@ -1343,6 +1378,11 @@ class GroupedMoe:
 
 
 # ---- beam search --------------------------------------------------------------------------------------------
+@lru_cache(maxsize=256)
+def _beam_workspace(batch: int, beams: int, vocab: int, bf16: int) -> int:
+    return int(_lib.load().eider_b200_beam_select_workspace_bytes(batch, beams, vocab, bf16))
+
+
 def beam_search_select(logits: torch.Tensor, beam_scores: torch.Tensor, k: int, finished: torch.Tensor | None = None, pad_token: int = 0):
     """The k best continuations of every sequence over its beams and the vocabulary: logits [batch, beams, vocab] (f32 or bf16, e.g.
     an lm-head's over batch * beams tokens), beam_scores [batch, beams] f32.  Returns (scores [batch, k] f32, parents [batch, k] int32,
@@ -1365,15 +1405,16 @@ def beam_search_select(logits: torch.Tensor, beam_scores: torch.Tensor, k: int, 
             raise ShapeError(f"pad_token must be a token, got {pad_token}")
     device, bf16 = logits.device, int(logits.dtype == torch.bfloat16)
     _need_device(device, beam_scores, finished)
-    size = _lib.load().eider_b200_beam_select_workspace_bytes(batch, beams, vocab, bf16)
+    size = _beam_workspace(batch, beams, vocab, bf16)
     if size == 0 or not 0 < k <= min(128, beams * vocab):
         raise ShapeError(f"unsupported beam search batch={batch} beams={beams} vocab={vocab} k={k}")
-    out = torch.empty(3, batch, k, dtype=torch.int32, device=device)
+    scores = torch.empty(batch, k, dtype=torch.float32, device=device)
+    parents = torch.empty(batch, k, dtype=torch.int32, device=device)
+    tokens = torch.empty(batch, k, dtype=torch.int32, device=device)
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    scores, parents, tokens = out.unbind(0)
     _call(device, "eider_b200_beam_select_on_stream", logits.data_ptr(), bf16, row, beam_scores.data_ptr(), _ptr(finished), pad_token if finished is not None else 0,
           scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), batch, beams, vocab, k, workspace.data_ptr(), size)
-    return scores.view(torch.float32), parents, tokens
+    return scores, parents, tokens
 
 
 def beam_search_reorder(states: list, parents: torch.Tensor, out: list | None = None) -> list:
@@ -1391,17 +1432,19 @@ def beam_search_reorder(states: list, parents: torch.Tensor, out: list | None = 
         out = [torch.empty_like(t) for t in states]
     if not states or len(out) != len(states):
         raise ShapeError("as many outputs as states are wanted, and one at least")
+    sizes = []
     for s, o in zip(states, out):
         if s.shape[:2] != (batch, beams) or s.numel() == 0 or o.shape != s.shape or o.dtype != s.dtype or not s.is_contiguous() or not o.is_contiguous():
             raise ShapeError(f"states must be contiguous [{batch}, {beams}, ...], and outputs like them")
-        first, other, size = s.data_ptr(), o.data_ptr(), s.numel() * s.element_size()
+        first, other, size = s.data_ptr(), o.data_ptr(), s.nbytes
         if first < other + size and other < first + size:
             raise ShapeError("a state cannot be reordered in place")
+        sizes.append(size // (batch * beams))
     _need_device(parents.device, *states, *out)
     n = len(states)
-    rows = (C.c_size_t * n)(*[s.numel() // (batch * beams) * s.element_size() for s in states])
-    _call(parents.device, "eider_b200_beam_reorder_on_stream", (C.c_void_p * n)(*[s.data_ptr() for s in states]),
-          (C.c_void_p * n)(*[o.data_ptr() for o in out]), rows, n, parents.data_ptr(), stride, batch, beams)
+    pointers = C.c_void_p * n
+    _call(parents.device, "eider_b200_beam_reorder_on_stream", pointers(*[s.data_ptr() for s in states]), pointers(*[o.data_ptr() for o in out]),
+          (C.c_size_t * n)(*sizes), n, parents.data_ptr(), stride, batch, beams)
     return out
 
 
