@@ -1,16 +1,17 @@
 // W4A16 product of MXFP4 weights for few tokens: y[t][n] = sum_k x[t][k] * w[n][k] (+ beta * C), the weights streamed once.
 //
-// Bound: HBM, N * K * 17/32 bytes of weights.  Every CTA has N / 148 rows of its own for the whole K (as many passes as rows do not fit), so
-// that all SMs stream the same number of bytes whatever N is and no partial sum leaves a CTA: one launch, no workspace, the same
-// order of additions in every run.
+// Bound: HBM, N * K * 17/32 bytes of weights.  Every CTA, two of them on an SM, has N / 296 rows of its own for the whole K (as many passes
+// as rows do not fit), or a pair of CTAs N / 148 for half of the K each, so that all SMs stream the same number of bytes whatever N is:
+// one launch, no workspace, the same order of additions in every run.
 //  * A producer warp streams the rows in chunks of 256 elements (TMA boxes of 128 bytes x rows, 128-byte swizzle) through a ring of
-//    shared memory; weights and scales are requested before the launch in front is awaited.
-//  * Each chunk is one warp's, for all of the CTA's rows: 16 rows x 32 elements (a block) at a time through mma.m16n8k16 with the tokens
+//    shared memory; weights and scales are requested before the launch in front is awaited, and a CTA of the next launch has room
+//    beside one of this.
+//  * Half a chunk is one warp's, for all of the CTA's rows: 16 rows x 32 elements (a block) at a time through mma.m16n8k16 with the tokens
 //    as the eight columns.  E2M1 codes become f16 by one conversion per pair (exact), the sum of a block (two MMAs) is taken in f32 and
 //    then added times its block scale in f32, so the weights are never multiplied out and no MMA chain is longer than a block.
 //  * x becomes f16 by a power of two per token and warp that brings its largest element so far to 2^8..2^9 (it grows to 2^15 before the
 //    sums are rescaled): bf16's eight bits fit, f32 goes as two f16 terms.  What is lost lies 2^-33 below the largest element.
-//  * The warps' sums over K meet in shared memory, in warp order.
+//  * The warps' sums over K meet in shared memory, in warp order, a pair's in that of the first.
 #include <algorithm>
 #include <atomic>
 #include <new>
@@ -25,10 +26,10 @@ namespace decode_mx {
 
 constexpr uint32_t kChunkBytes = 128;               // 256 elements of a row
 constexpr uint32_t kChunkBlocks = 8;
-constexpr uint32_t kMaxWarps = 11;                  // consumer warps; with the producer three a scheduler, 168 registers each
-constexpr uint32_t kMaxRows = 96;                   // rows of a CTA in a pass: six MMA tiles
-constexpr uint32_t kSmemLimit = 227 * 1024;
-constexpr uint32_t kMaxSlots = 64;
+constexpr uint32_t kMaxWarps = 7;                   // consumer warps; with the producer, and two CTAs an SM, 128 registers each
+constexpr uint32_t kMaxTiles = 3;                   // 16-row MMA tiles of a CTA in a pass
+constexpr uint32_t kSmemLimit = 113 * 1024;         // two CTAs an SM, of this launch or of the next one
+constexpr uint32_t kMaxSlots = 32;
 constexpr uint32_t kFull = 0xffffffffu;
 
 struct Params {
@@ -40,14 +41,15 @@ struct Params {
     float beta;
     int out_is_bf16;
     uint32_t tokens, n, k, pitch;
-    uint32_t rows;    // of a CTA in a pass
+    uint32_t rows;    // of a CTA (pair) in a pass
     uint32_t passes, chunks, slots, warps;
+    uint32_t split;   // CTAs of a cluster that share the chunks of their rows
 };
 
 __host__ __device__ constexpr uint32_t reduce_pitch(uint32_t tiles) { return tiles * 16 + 4; }  // (rows of a token; + 4: the fragments' stores meet no bank twice)
 __host__ __device__ constexpr uint32_t slot_bytes(uint32_t tiles) { return tiles * 16 * kChunkBytes; }
 inline uint32_t fixed_bytes(uint32_t tiles, uint32_t warps, uint32_t pitch, uint32_t passes) {
-    return 1024 /*alignment*/ + (passes > 1 ? 2 : 1) * tiles * 16 * pitch + warps * 8 * reduce_pitch(tiles) * 4 + (2 * kMaxSlots + 4) * 8 + 16;
+    return 1024 /*alignment*/ + (passes > 1 ? 2 : 1) * tiles * 16 * pitch + (warps + 1) * 8 * reduce_pitch(tiles) * 4 + (2 * kMaxSlots + 4) * 8 + 16;
 }
 
 __device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&p)[4]) {
@@ -60,10 +62,16 @@ __device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&p)[4]) {
         : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3])
         : "r"(w));
 }
+template <bool FIRST>
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if (FIRST)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
     uint32_t r;
@@ -81,17 +89,58 @@ __device__ __forceinline__ uint32_t lds32(uint32_t address) {
     return v;
 }
 
-// Eight consecutive elements of a token.
+// 2^(c - 127) of byte `I` of a word.  255 gives an infinity here: a row with such a scale comes out infinite or NaN and is looked at
+// again at the end.
+template <int I> __device__ __forceinline__ float scale_of(uint32_t word) {
+    const uint32_t field = (I < 3 ? word << (23 - 8 * I) : word >> 1) & 0x7f800000u;
+    return __uint_as_float(max(field, 0x00400000u));
+}
+
+__device__ __forceinline__ uint32_t lds16(uint32_t address) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(address));
+    return v;
+}
+template <int N, typename F> __device__ __forceinline__ void static_for(F f) {
+    if constexpr (N > 0) {
+        static_for<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+
+// Eight consecutive elements of a token, and what becomes of them: the largest finite magnitude, and f16 terms of x * factor.
 template <typename T> struct Raw8;
 template <> struct Raw8<uint16_t> {
     uint4 q;
     __device__ __forceinline__ void load(const uint16_t* p, bool live) { q = live ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
+    static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+    __device__ __forceinline__ float amax() const {
+        const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(pair(q.x)), __habs2(pair(q.y))), __hmax2(__habs2(pair(q.z)), __habs2(pair(q.w))));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
     __device__ __forceinline__ void values(float (&v)[8]) const {
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            v[2 * i] = __uint_as_float(word(i) << 16);
+            v[2 * i + 1] = __uint_as_float(word(i) & 0xffff0000u);
+        }
+    }
+    __device__ __forceinline__ float finite() const {
+        float v[8], m = 0.0f;
+        values(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[e]));
+        return m;
+    }
+    // (the factor is a power of two: the product is exact in bf16 but far below anything that counts)
+    __device__ __forceinline__ void terms(float factor, uint32_t (&t)[1][4]) const {
+        const __nv_bfloat162 f = __float2bfloat162_rn(factor);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 p = __hmul2(pair(word(i)), f);
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(&p);
+            t[0][i] = f16x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
         }
     }
 };
@@ -101,33 +150,66 @@ template <> struct Raw8<float> {
         a = live ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
         b = live ? __ldg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
     }
+    __device__ __forceinline__ float amax() const {
+        return fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))), fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
+    }
     __device__ __forceinline__ void values(float (&v)[8]) const {
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     }
+    __device__ __forceinline__ float finite() const {
+        float v[8], m = 0.0f;
+        values(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[e]));
+        return m;
+    }
+    __device__ __forceinline__ void terms(float factor, uint32_t (&t)[2][4]) const {
+        float v[8];
+        values(v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float lo = v[2 * i] * factor, hi = v[2 * i + 1] * factor;
+            t[0][i] = f16x2(lo, hi);
+            const float2 first = f16x2_values(t[0][i]);
+            // (of an infinity or NaN the first term is all there is)
+            t[1][i] = f16x2(fabsf(first.x) < INFINITY ? lo - first.x : 0.0f, fabsf(first.y) < INFINITY ? hi - first.y : 0.0f);
+        }
+    }
 };
 
-// TILES: 16-row MMA tiles of a CTA's rows.  COLS: groups of eight tokens.
-template <int TILES, int COLS, typename XT>
-__global__ void __launch_bounds__(32 * (kMaxWarps + 1), 1) decode_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const Params p) {
-    constexpr bool kF32 = sizeof(XT) == 4;
-    constexpr int kTerms = kF32 ? 2 : 1;
-    constexpr int kStep = COLS * kTerms >= 4 ? 1 : 4 / (COLS * kTerms);  // blocks of x that a warp holds (and has on their way) at a time
+// TILES: 16-row MMA tiles of a CTA's rows.  COLS: groups of eight MMA columns.
+// SPREAD: consecutive blocks that take an MMA column each (with COLS 1).  Few tokens leave most of the eight columns empty, so block j
+// of SPREAD goes through column j of its token alone: the MMAs of SPREAD blocks add up in one accumulator, whose columns then get
+// their block scales in one go, and every lane converts the activations of one block instead of all of them.  About 18
+// instructions for 16 x 32 weights at SPREAD 8 against 34 at 1.  SPLIT_TERMS: the two f16 terms of f32 are columns too (up to four
+// tokens) instead of MMAs of their own.
+template <int TILES, int COLS, int SPREAD, bool SPLIT_TERMS, typename XT>
+__global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const Params p) {
+    constexpr int kTerms = sizeof(XT) == 4 && !SPLIT_TERMS ? 2 : 1;      // MMAs of the same weights
+    constexpr int kSpan = SPREAD * (SPLIT_TERMS ? 2 : 1);                // columns of a token
+    constexpr uint32_t kItemBlocks = SPREAD == 8 ? 8 : 4;                // blocks of a work item: a warp's share at a time
+    constexpr int kStep = COLS * kTerms >= 4 ? 1 : 4 / (COLS * kTerms);  // blocks of x that a warp holds (and has on their way) at a time, COLS > 1
+    constexpr int kGroups = kItemBlocks / SPREAD;                        // the same for COLS 1: a block of each of these groups
+    static_assert(COLS == 1 || (SPREAD == 1 && !SPLIT_TERMS), "columns are spread within one group of eight");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const uint32_t scale_bytes = TILES * 16 * p.pitch;
     uint8_t* scales = ring + p.slots * slot_bytes(TILES);
-    float* sums = reinterpret_cast<float*>(scales + (p.passes > 1 ? 2 : 1) * scale_bytes);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sums + p.warps * 8 * reduce_pitch(TILES));  // [slots]
-    uint64_t* empty = full + kMaxSlots;                                                     // [slots]
-    uint64_t* scales_full = empty + kMaxSlots;                                              // [2]
-    uint64_t* scales_empty = scales_full + 2;                                               // [2]
+    float* sums = reinterpret_cast<float*>(scales + (p.passes > 1 ? 2 : 1) * scale_bytes);  // [warps][8][rows], then the other CTA's [8][rows]
+    uint64_t* full = reinterpret_cast<uint64_t*>(sums + (p.warps + 1) * 8 * reduce_pitch(TILES));  // [slots]
+    uint64_t* empty = full + kMaxSlots;                                                           // [slots]
+    uint64_t* scales_full = empty + kMaxSlots;                                                    // [2]
+    uint64_t* scales_empty = scales_full + 2;                                                     // [2]
     volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(scales_empty + 2);
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = p.split > 1 ? umma::cluster_ctarank() : 0, group = p.split > 1 ? blockIdx.x / p.split : blockIdx.x;
+    const uint32_t groups = p.split > 1 ? gridDim.x / p.split : gridDim.x;
+    const uint32_t chunks = (p.chunks + p.split - 1 - rank) / p.split;  // this CTA's: rank, rank + split, ..
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < p.slots; ++i) {
             umma::mbar_init(&full[i], 1);
-            umma::mbar_init(&empty[i], 1);
+            umma::mbar_init(&empty[i], kChunkBlocks / kItemBlocks);  // (the warps whose items the chunk is)
         }
         for (uint32_t i = 0; i < 2; ++i) {
             umma::mbar_init(&scales_full[i], 1);
@@ -146,18 +228,19 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 1) decode_mxfp4_kernel(c
             uint32_t i = 0, pass = 0;
             bool ok = true;
             for (; ok && pass < p.passes; ++pass) {
-                const uint32_t row0 = (pass * gridDim.x + blockIdx.x) * p.rows;
+                const uint32_t row0 = (pass * groups + group) * p.rows;
                 if (row0 >= p.n) break;
                 const uint32_t buffer = pass & 1;
                 if (!umma::mbar_wait(&scales_empty[buffer], ((pass >> 1) & 1) ^ 1, abort_flag, p.status, umma::kTimeoutEmpty)) break;  // (pass: those begun)
                 const uint32_t bytes = min(p.rows, p.n - row0) * p.pitch;
                 umma::mbar_arrive_expect_tx(&scales_full[buffer], bytes);
                 umma::bulk_load_1d(scales + buffer * scale_bytes, p.scales + static_cast<size_t>(row0) * p.pitch, bytes, &scales_full[buffer]);
-                for (uint32_t c = 0; c < p.chunks; ++c, ++i) {
+                for (uint32_t c = 0; c < chunks; ++c, ++i) {
                     const uint32_t slot = i % p.slots, phase = (i / p.slots) & 1;
                     if (!umma::mbar_wait(&empty[slot], phase ^ 1, abort_flag, p.status, umma::kTimeoutEmpty)) { ok = false; break; }
                     umma::mbar_arrive_expect_tx(&full[slot], p.rows * kChunkBytes);
-                    umma::tma_load_2d(ring + slot * slot_bytes(TILES), &map_w, &full[slot], static_cast<int32_t>(c * kChunkBytes), static_cast<int32_t>(row0));
+                    umma::tma_load_2d(ring + slot * slot_bytes(TILES), &map_w, &full[slot], static_cast<int32_t>((c * p.split + rank) * kChunkBytes),
+                                      static_cast<int32_t>(row0));
                 }
             }
             // The block does not leave before its copies have landed, not even after a wait ran out: bounded too.
@@ -168,6 +251,14 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 1) decode_mxfp4_kernel(c
             for (uint32_t j = i > p.slots ? i - p.slots : 0; j < i; ++j) landed(&full[j % p.slots], (j / p.slots) & 1);
             for (uint32_t j = pass > 2 ? pass - 2 : 0; j < pass; ++j) landed(&scales_full[j & 1], (j >> 1) & 1);
         }
+        __syncwarp();
+        if (p.split > 1) {  // (the meetings below are the whole cluster's)
+            for (uint32_t pass = 0; pass < p.passes && (pass * groups + group) * p.rows < p.n; ++pass)
+                for (uint32_t n = 0; n < COLS && n * 8 < p.tokens * kSpan; ++n) {
+                    umma::cluster_sync_all();
+                    umma::cluster_sync_all();
+                }
+        }
         return;
     }
 
@@ -175,18 +266,24 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 1) decode_mxfp4_kernel(c
     const uint32_t g = lane >> 2, t = lane & 3;
     const uint32_t blocks = p.k / mx::kBlock;
     const uint32_t ring_addr = umma::smem_u32(ring), scales_addr = umma::smem_u32(scales);
+    constexpr uint32_t kPerChunk = kChunkBlocks / kItemBlocks;
+    const uint32_t items = chunks * kPerChunk;
     umma::griddep_wait();
     const XT* x = static_cast<const XT*>(p.x) + t * 8;
+    const uint32_t sub = g % SPREAD;  // this lane's block of SPREAD
     bool live[COLS];
-    size_t x_at[COLS];
+    const XT* x_of[COLS];
 #pragma unroll
     for (int n = 0; n < COLS; ++n) {
-        live[n] = n * 8 + g < p.tokens;
-        x_at[n] = live[n] ? static_cast<size_t>(n * 8 + g) * p.k : 0;
+        const uint32_t token = (n * 8 + g) / kSpan;
+        live[n] = token < p.tokens;
+        x_of[n] = x + (live[n] ? static_cast<size_t>(token) * p.k : 0) + sub * mx::kBlock;
     }
+    // first block (of K) of this CTA's item
+    auto item_block = [&](uint32_t item) { return (item / kPerChunk * p.split + rank) * kChunkBlocks + item % kPerChunk * kItemBlocks; };
     bool ok = true;
     for (uint32_t pass = 0; pass < p.passes; ++pass) {
-        const uint32_t row0 = (pass * gridDim.x + blockIdx.x) * p.rows;
+        const uint32_t row0 = (pass * groups + group) * p.rows;
         if (row0 >= p.n) break;
         float acc[TILES][COLS][4];
 #pragma unroll
@@ -199,121 +296,202 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 1) decode_mxfp4_kernel(c
 #pragma unroll
         for (int n = 0; n < COLS; ++n) factor[n] = 0.0f;
 
-        Raw8<XT> raw[COLS][kStep];
+        // Largest finite magnitude in hand -> whether the column's factor has to change, and what the sums so far change by.
+        auto rescale = [&](int n, float amax, auto finite_amax) {
+            amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
+            if (__any_sync(kFull, factor[n] == 0.0f ? amax != 0.0f : amax * factor[n] >= 32768.0f)) {
+                if (__any_sync(kFull, amax == INFINITY)) {  // an infinity goes through as it is; the finite ones set the scale
+                    amax = finite_amax();
+                    amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
+                    amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
+                }
+                float change = 1.0f;
+                if (factor[n] == 0.0f ? amax != 0.0f : amax * factor[n] >= 32768.0f) {
+                    const float wanted = __uint_as_float(min(254u, 262u - (__float_as_uint(amax) >> 23)) << 23);  // the largest element to 2^8..2^9
+                    // (the sums so far are zero, or change by a power of two; a change too small for f32 leaves nothing of them either way)
+                    if (factor[n] != 0.0f) change = __fdiv_rn(wanted, factor[n]);
+                    factor[n] = wanted;
+                }
+                const float c0 = __shfl_sync(kFull, change, t * 8), c1 = __shfl_sync(kFull, change, t * 8 + 4);
+#pragma unroll
+                for (int u = 0; u < TILES; ++u) {
+                    acc[u][n][0] *= c0;
+                    acc[u][n][1] *= c1;
+                    acc[u][n][2] *= c0;
+                    acc[u][n][3] *= c1;
+                }
+            }
+            return factor[n] == 0.0f ? 1.0f : factor[n];
+        };
+        constexpr int kHeld = COLS == 1 ? kGroups : kStep;
+        Raw8<XT> raw[COLS][kHeld];
         auto load_x = [&](uint32_t block) {
 #pragma unroll
             for (int n = 0; n < COLS; ++n)
 #pragma unroll
-                for (int s = 0; s < kStep; ++s) raw[n][s].load(x + x_at[n] + static_cast<size_t>(block + s) * mx::kBlock, live[n] && block + s < blocks);
+                for (int s = 0; s < kHeld; ++s) raw[n][s].load(x_of[n] + (block + s * SPREAD) * mx::kBlock, live[n] && block + s * SPREAD + sub < blocks);
         };
-        if (warp < p.chunks) load_x(warp * kChunkBlocks);
+        if (warp < items) load_x(item_block(warp));
         if (ok && !umma::mbar_wait(&scales_full[pass & 1], (pass >> 1) & 1, abort_flag, p.status, umma::kTimeoutFull)) ok = false;
-        const uint32_t pass_scales = scales_addr + (pass & 1) * scale_bytes;
-        for (uint32_t c = warp; ok && c < p.chunks; c += p.warps) {
-            const uint32_t i = pass * p.chunks + c, slot = i % p.slots, phase = (i / p.slots) & 1;
-            const uint32_t tile = ring_addr + slot * slot_bytes(TILES) + g * kChunkBytes + t * 4;
-            bool arrived = false;
-#pragma unroll 1
-            for (uint32_t step = 0; step < kChunkBlocks; step += kStep) {
-                // this step's x as f16, then the next step's is requested
-                uint32_t b[kStep][COLS][kTerms][4];
+        const uint32_t pass_scales = scales_addr + (pass & 1) * scale_bytes + g * p.pitch;
+        for (uint32_t item = warp; ok && item < items; item += p.warps) {
+            const uint32_t i = pass * chunks + item / kPerChunk, slot = i % p.slots, phase = (i / p.slots) & 1;
+            const uint32_t block0 = item_block(item);
+            const uint32_t tile = ring_addr + slot * slot_bytes(TILES) + g * kChunkBytes + t * 4, half = item % kPerChunk * kItemBlocks;
+            auto arrive = [&] {
+                ok = __all_sync(kFull, umma::mbar_wait(&full[slot], phase, abort_flag, p.status, umma::kTimeoutFull));
+                return ok;
+            };
+            // block `in` of the item: rows of tile u as f16
+            auto weights = [&](uint32_t in, int u, uint32_t (&lo)[4], uint32_t (&hi)[4]) {
+                const uint32_t at = tile + (((half + in) ^ g) << 4);
+                e2m1_f16(lds32(at + u * 16 * kChunkBytes), lo);
+                e2m1_f16(lds32(at + (u * 16 + 8) * kChunkBytes), hi);
+            };
+            if constexpr (COLS == 1) {
+                float amax = 0.0f;
 #pragma unroll
-                for (int n = 0; n < COLS; ++n) {
-                    float v[kStep][8];
-                    uint32_t amax = 0;
+                for (int s = 0; s < kHeld; ++s) amax = fmaxf(amax, raw[0][s].amax());
+                const float f = rescale(0, amax, [&] {
+                    float m = 0.0f;
 #pragma unroll
-                    for (int s = 0; s < kStep; ++s) {
-                        raw[n][s].values(v[s]);
+                    for (int s = 0; s < kHeld; ++s) m = fmaxf(m, raw[0][s].finite());
+                    return m;
+                });
+                uint32_t b[kHeld][kTerms][4];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) amax = max(amax, mx::abs_bits(v[s][e]));
+                for (int s = 0; s < kHeld; ++s) {
+                    if constexpr (SPLIT_TERMS) {
+                        uint32_t both[2][4];
+                        raw[0][s].terms(f, both);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) b[s][0][e] = (g / SPREAD) & 1 ? both[1][e] : both[0][e];
+                    } else {
+                        raw[0][s].terms(f, b[s]);
                     }
-                    if (amax >= 0x7f800000u) {  // an infinity or NaN goes through as it is; the finite ones set the scale
-                        amax = 0;
+                }
+                if (item + p.warps < items) load_x(item_block(item + p.warps));
+                if (!arrive()) break;
+                [[maybe_unused]] uint32_t lo4[TILES], hi4[TILES];
+                if constexpr (SPREAD == 1) {
 #pragma unroll
-                        for (int s = 0; s < kStep; ++s)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) amax = max(amax, mx::abs_bits(v[s][e]) < 0x7f800000u ? mx::abs_bits(v[s][e]) : 0u);
+                    for (int u = 0; u < TILES; ++u) {
+                        lo4[u] = lds32(pass_scales + block0 + u * 16 * p.pitch);
+                        hi4[u] = lds32(pass_scales + block0 + (u * 16 + 8) * p.pitch);
                     }
-                    amax = max(amax, __shfl_xor_sync(kFull, amax, 1));
-                    amax = max(amax, __shfl_xor_sync(kFull, amax, 2));
-                    const bool rescale = factor[n] == 0.0f ? amax != 0 : __uint_as_float(amax) * factor[n] >= 32768.0f;
-                    if (__any_sync(kFull, rescale)) {
-                        float change = 1.0f;
-                        if (rescale) {
-                            const uint32_t e = amax >> 23;
-                            const float wanted = __uint_as_float(min(254u, 262u - e) << 23);  // the largest element to 2^8..2^9
-                            // (the sums so far are zero, or change by a power of two; a change too small for f32 leaves nothing of them either way)
-                            if (factor[n] != 0.0f) change = __fdiv_rn(wanted, factor[n]);
-                            factor[n] = wanted;
-                        }
-                        const float c0 = __shfl_sync(kFull, change, t * 8), c1 = __shfl_sync(kFull, change, t * 8 + 4);
+                }
+                static_for<kGroups>([&](auto which) {
+                    constexpr int s = decltype(which)::value;
+                    float d[TILES][4];
+#pragma unroll
+                    for (int in = 0; in < SPREAD; ++in) {
+                        uint32_t m[kTerms][4];
+#pragma unroll
+                        for (int q = 0; q < kTerms; ++q)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) m[q][e] = SPREAD == 1 || sub == static_cast<uint32_t>(in) ? b[s][q][e] : 0u;
 #pragma unroll
                         for (int u = 0; u < TILES; ++u) {
-                            acc[u][n][0] *= c0;
-                            acc[u][n][1] *= c1;
-                            acc[u][n][2] *= c0;
-                            acc[u][n][3] *= c1;
-                        }
-                    }
-                    const float f = factor[n] == 0.0f ? 1.0f : factor[n];
-#pragma unroll
-                    for (int s = 0; s < kStep; ++s)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float lo = v[s][2 * e] * f, hi = v[s][2 * e + 1] * f;
-                            b[s][n][0][e] = f16x2(lo, hi);
-                            if constexpr (kF32) {
-                                const float2 first = f16x2_values(b[s][n][0][e]);
-                                // (of an infinity or NaN the first term is all there is)
-                                b[s][n][kTerms - 1][e] = f16x2(fabsf(first.x) < INFINITY ? lo - first.x : 0.0f, fabsf(first.y) < INFINITY ? hi - first.y : 0.0f);
+                            uint32_t lo[4], hi[4];
+                            weights(s * SPREAD + in, u, lo, hi);
+                            if (in == 0) mma_f16<true>(d[u], lo[0], hi[0], lo[1], hi[1], m[0][0], m[0][1]);
+                            else mma_f16<false>(d[u], lo[0], hi[0], lo[1], hi[1], m[0][0], m[0][1]);
+                            mma_f16<false>(d[u], lo[2], hi[2], lo[3], hi[3], m[0][2], m[0][3]);
+                            if constexpr (kTerms == 2) {
+                                mma_f16<false>(d[u], lo[0], hi[0], lo[1], hi[1], m[kTerms - 1][0], m[kTerms - 1][1]);
+                                mma_f16<false>(d[u], lo[2], hi[2], lo[3], hi[3], m[kTerms - 1][2], m[kTerms - 1][3]);
                             }
                         }
-                }
-                const uint32_t next = step + kStep;
-                if (next < kChunkBlocks) load_x(c * kChunkBlocks + next);
-                else if (c + p.warps < p.chunks) load_x((c + p.warps) * kChunkBlocks);
-                if (!arrived) {
-                    if (!__all_sync(kFull, umma::mbar_wait(&full[slot], phase, abort_flag, p.status, umma::kTimeoutFull))) { ok = false; break; }
-                    arrived = true;
-                }
-                // scale bytes of these blocks
-                const uint32_t scale_at = pass_scales + g * p.pitch + c * kChunkBlocks + (step & ~3u);
+                    }
+                    // this thread's columns 2t and 2t + 1 are neighbouring blocks of a token (or the same block of two)
 #pragma unroll
-                for (int u = 0; u < TILES; ++u) {
-                    const uint32_t lo4 = lds32(scale_at + u * 16 * p.pitch), hi4 = lds32(scale_at + (u * 16 + 8) * p.pitch);
+                    for (int u = 0; u < TILES; ++u) {
+                        float lo0, lo1, hi0, hi1;
+                        if constexpr (SPREAD == 1) {
+                            lo0 = lo1 = scale_of<s>(lo4[u]);
+                            hi0 = hi1 = scale_of<s>(hi4[u]);
+                        } else {
+                            const uint32_t at = pass_scales + block0 + s * SPREAD + (2 * t) % SPREAD;
+                            const uint32_t lo2 = lds16(at + u * 16 * p.pitch), hi2 = lds16(at + (u * 16 + 8) * p.pitch);
+                            lo0 = scale_of<0>(lo2);
+                            lo1 = scale_of<1>(lo2);
+                            hi0 = scale_of<0>(hi2);
+                            hi1 = scale_of<1>(hi2);
+                        }
+                        acc[u][0][0] = fmaf(d[u][0], lo0, acc[u][0][0]);
+                        acc[u][0][1] = fmaf(d[u][1], lo1, acc[u][0][1]);
+                        acc[u][0][2] = fmaf(d[u][2], hi0, acc[u][0][2]);
+                        acc[u][0][3] = fmaf(d[u][3], hi1, acc[u][0][3]);
+                    }
+                });
+            } else {
+                uint32_t lo4[TILES], hi4[TILES];
+                static_for<kItemBlocks / kStep>([&](auto which) {
+                    constexpr int step = decltype(which)::value * kStep;
+                    if (!ok) return;
+                    // this step's x as f16, then the next step's is requested
+                    uint32_t b[kStep][COLS][kTerms][4];
 #pragma unroll
-                    for (int s = 0; s < kStep; ++s) {
-                        const uint32_t block = step + s, shift = 8 * (block & 3);
-                        const uint32_t at = tile + u * 16 * kChunkBytes + ((block ^ g) << 4);
-                        uint32_t lo[4], hi[4];
-                        e2m1_f16(lds32(at), lo);
-                        e2m1_f16(lds32(at + 8 * kChunkBytes), hi);
-                        const float s_lo = mx::scale_value(lo4 >> shift & 255u), s_hi = mx::scale_value(hi4 >> shift & 255u);
+                    for (int n = 0; n < COLS; ++n) {
+                        float amax = 0.0f;
 #pragma unroll
-                        for (int n = 0; n < COLS; ++n) {
-                            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int s = 0; s < kStep; ++s) amax = fmaxf(amax, raw[n][s].amax());
+                        const float f = rescale(n, amax, [&] {
+                            float m = 0.0f;
 #pragma unroll
-                            for (int term = 0; term < kTerms; ++term) {
-                                mma_f16(d, lo[0], hi[0], lo[1], hi[1], b[s][n][term][0], b[s][n][term][1]);
-                                mma_f16(d, lo[2], hi[2], lo[3], hi[3], b[s][n][term][2], b[s][n][term][3]);
-                            }
-                            acc[u][n][0] = fmaf(d[0], s_lo, acc[u][n][0]);
-                            acc[u][n][1] = fmaf(d[1], s_lo, acc[u][n][1]);
-                            acc[u][n][2] = fmaf(d[2], s_hi, acc[u][n][2]);
-                            acc[u][n][3] = fmaf(d[3], s_hi, acc[u][n][3]);
+                            for (int s = 0; s < kStep; ++s) m = fmaxf(m, raw[n][s].finite());
+                            return m;
+                        });
+#pragma unroll
+                        for (int s = 0; s < kStep; ++s) raw[n][s].terms(f, b[s][n]);
+                    }
+                    if (step + kStep < static_cast<int>(kItemBlocks)) load_x(block0 + step + kStep);
+                    else if (item + p.warps < items) load_x(item_block(item + p.warps));
+                    if (step == 0) {
+                        if (!arrive()) return;
+#pragma unroll
+                        for (int u = 0; u < TILES; ++u) {
+                            lo4[u] = lds32(pass_scales + block0 + u * 16 * p.pitch);
+                            hi4[u] = lds32(pass_scales + block0 + (u * 16 + 8) * p.pitch);
                         }
                     }
-                }
+                    static_for<kStep>([&](auto in_step) {
+                        constexpr int s = decltype(in_step)::value;
+#pragma unroll
+                        for (int u = 0; u < TILES; ++u) {
+                            uint32_t lo[4], hi[4];
+                            weights(step + s, u, lo, hi);
+                            const float s_lo = scale_of<step + s>(lo4[u]), s_hi = scale_of<step + s>(hi4[u]);
+#pragma unroll
+                            for (int n = 0; n < COLS; ++n) {
+                                float d[4];
+                                mma_f16<true>(d, lo[0], hi[0], lo[1], hi[1], b[s][n][0][0], b[s][n][0][1]);
+                                mma_f16<false>(d, lo[2], hi[2], lo[3], hi[3], b[s][n][0][2], b[s][n][0][3]);
+                                if constexpr (kTerms == 2) {
+                                    mma_f16<false>(d, lo[0], hi[0], lo[1], hi[1], b[s][n][kTerms - 1][0], b[s][n][kTerms - 1][1]);
+                                    mma_f16<false>(d, lo[2], hi[2], lo[3], hi[3], b[s][n][kTerms - 1][2], b[s][n][kTerms - 1][3]);
+                                }
+                                acc[u][n][0] = fmaf(d[0], s_lo, acc[u][n][0]);
+                                acc[u][n][1] = fmaf(d[1], s_lo, acc[u][n][1]);
+                                acc[u][n][2] = fmaf(d[2], s_hi, acc[u][n][2]);
+                                acc[u][n][3] = fmaf(d[3], s_hi, acc[u][n][3]);
+                            }
+                        }
+                    });
+                });
+                if (!ok) break;
             }
             __syncwarp();
             if (ok && lane == 0) umma::mbar_arrive(&empty[slot]);
         }
         if (lane == 0) umma::mbar_arrive(&scales_empty[pass & 1]);
 
-        // ------------------------------------------------------------------ the warps' sums meet, eight tokens at a time
+        // ------------------------------------------------------------------ the warps' (and CTAs') sums meet, eight tokens at a time
+        float* others = sums + p.warps * 8 * reduce_pitch(TILES);
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
-            if (n * 8 >= p.tokens) break;
+            if (n * 8 >= p.tokens * kSpan) break;
             // (1 / factor, exact: 2^-127 is subnormal)
             const uint32_t field = __float_as_uint(factor[n]) >> 23;
             const float back = factor[n] == 0.0f ? 1.0f : __uint_as_float(field == 254 ? 0x00400000u : (254u - field) << 23);
@@ -327,18 +505,42 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 1) decode_mxfp4_kernel(c
                 mine[(2 * t + 1) * reduce_pitch(TILES) + u * 16 + g + 8] = acc[u][n][3] * b1;
             }
             asm volatile("bar.sync 1, %0;" ::"r"(p.warps * 32) : "memory");
-            const uint32_t tokens = min(8u, p.tokens - n * 8), rows = min(p.rows, p.n - row0);
-            for (uint32_t i = threadIdx.x; i < tokens * rows; i += p.warps * 32) {
-                const uint32_t token = i / rows, row = i - token * rows;
+            const uint32_t tokens = min(8u / kSpan, p.tokens - n * 8), rows = min(p.rows, p.n - row0);
+            auto warps_sum = [&](uint32_t token, uint32_t row) {
                 float sum = 0.0f;
-                for (uint32_t w = 0; w < p.warps; ++w) sum += sums[(w * 8 + token) * reduce_pitch(TILES) + row];
-                const size_t index = static_cast<size_t>(n * 8 + token) * p.n + row0 + row;
-                if (p.beta != 0.0f)
-                    sum = fmaf(p.beta, p.out_is_bf16 ? bf16_bits_to_float(static_cast<const uint16_t*>(p.c)[index]) : static_cast<const float*>(p.c)[index], sum);
-                if (p.out_is_bf16) static_cast<uint16_t*>(p.out)[index] = float_to_bf16_bits(sum);
-                else static_cast<float*>(p.out)[index] = sum;
+                for (uint32_t w = 0; w < p.warps; ++w)
+#pragma unroll
+                    for (uint32_t c = 0; c < kSpan; ++c) sum += sums[(w * 8 + token * kSpan + c) * reduce_pitch(TILES) + row];
+                return sum;
+            };
+            if (p.split > 1) {
+                if (rank != 0) {
+                    const uint32_t there = umma::map_to_cta(umma::smem_u32(others), 0);
+                    for (uint32_t i = threadIdx.x; i < tokens * rows; i += p.warps * 32) {
+                        const uint32_t token = i / rows, row = i - token * rows;
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there + (token * reduce_pitch(TILES) + row) * 4), "f"(warps_sum(token, row)) : "memory");
+                    }
+                }
+                umma::cluster_sync_all();
             }
-            asm volatile("bar.sync 1, %0;" ::"r"(p.warps * 32) : "memory");
+            if (rank == 0)
+                for (uint32_t i = threadIdx.x; i < tokens * rows; i += p.warps * 32) {
+                    const uint32_t token = i / rows, row = i - token * rows;
+                    float sum = warps_sum(token, row);
+                    if (p.split > 1) sum += others[token * reduce_pitch(TILES) + row];
+                    if (!(fabsf(sum) < INFINITY)) {  // a NaN scale among the row's?
+                        const uint8_t* s = p.scales + static_cast<size_t>(row0 + row) * p.pitch;
+                        for (uint32_t q = 0; q < blocks; ++q)
+                            if (s[q] == mx::kNanCode) sum = NAN;
+                    }
+                    const size_t index = static_cast<size_t>(n * 8 + token) * p.n + row0 + row;
+                    if (p.beta != 0.0f)
+                        sum = fmaf(p.beta, p.out_is_bf16 ? bf16_bits_to_float(static_cast<const uint16_t*>(p.c)[index]) : static_cast<const float*>(p.c)[index], sum);
+                    if (p.out_is_bf16) static_cast<uint16_t*>(p.out)[index] = float_to_bf16_bits(sum);
+                    else static_cast<float*>(p.out)[index] = sum;
+                }
+            if (p.split > 1) umma::cluster_sync_all();
+            else asm volatile("bar.sync 1, %0;" ::"r"(p.warps * 32) : "memory");
         }
     }
 }
@@ -349,35 +551,38 @@ struct Plan {
     gemm::MapCache maps_w;
 };
 
-// How a call is cut: rows of a CTA and pass, MMA tiles they take, consumer warps, ring slots.
+// How a call is cut: rows of a CTA (pair) and pass, MMA tiles they take, consumer warps, ring slots.
 struct Cut {
-    uint32_t rows, passes, tiles, warps, slots, smem;
+    uint32_t rows, passes, tiles, warps, slots, split, smem;
 };
-inline Cut cut(uint32_t n, uint32_t k, uint32_t pitch, uint32_t sms) {
-    Cut r{};
+inline Cut cut(uint32_t n, uint32_t k, uint32_t pitch, uint32_t item_blocks, uint32_t sms) {
     const uint32_t chunks = (k + 2 * kChunkBytes - 1) / (2 * kChunkBytes);
-    const uint32_t rounds = (chunks + kMaxWarps - 1) / kMaxWarps;  // chunks of the warp that has most
-    r.warps = (chunks + rounds - 1) / rounds;
-    for (uint32_t most = kMaxRows; most >= 16; most -= 16) {
-        r.passes = (n + sms * most - 1) / (sms * most);
-        r.rows = (n + sms * r.passes - 1) / (sms * r.passes);
-        r.tiles = (r.rows + 15) / 16;
-        if (r.tiles == 5) r.tiles = 6;
-        const uint32_t fixed = fixed_bytes(r.tiles, r.warps, pitch, r.passes);
-        if (fixed + 2 * slot_bytes(r.tiles) > kSmemLimit) continue;
-        r.slots = std::min(std::min(kMaxSlots, chunks * r.passes), (kSmemLimit - fixed) / slot_bytes(r.tiles));
-        // (half of the shared memory in flight at least, while fewer rows would allow it)
-        if (r.slots < std::min(4u, chunks) && most > 16) continue;
-        r.smem = fixed + r.slots * slot_bytes(r.tiles);
-        return r;
+    Cut best{};
+    float best_cost = 1e30f;
+    for (uint32_t split = 1; split <= 2 && split <= chunks; ++split) {
+        const uint32_t mine = (chunks + split - 1) / split, items = mine * (kChunkBlocks / item_blocks);
+        const uint32_t rounds = (items + kMaxWarps - 1) / kMaxWarps;  // items of the warp that has most
+        const uint32_t warps = (items + rounds - 1) / rounds, groups = 2 * sms / split;
+        for (uint32_t tiles = 1; tiles <= kMaxTiles; ++tiles) {
+            const uint32_t passes = (n + groups * tiles * 16 - 1) / (groups * tiles * 16), rows = (n + groups * passes - 1) / (groups * passes);
+            if ((rows + 15) / 16 != tiles) continue;
+            if (split > 1 && passes > 1) continue;  // (the producer joins the pair's meetings only once all of its loads are out)
+            const uint32_t fixed = fixed_bytes(tiles, warps, pitch, passes);
+            if (fixed + 2 * slot_bytes(tiles) > kSmemLimit) continue;
+            // a warp's time: its items of every pass, a tile's share of each and the activation's, and the meeting at a pass's end
+            const float cost = passes * (rounds * (tiles + 0.8f) * (item_blocks / 4) + 3.0f + (split > 1 ? 2.0f : 0.0f));
+            if (cost >= best_cost) continue;
+            best_cost = cost;
+            best = Cut{rows, passes, tiles, warps, std::min(std::min(kMaxSlots, mine * passes), (kSmemLimit - fixed) / slot_bytes(tiles)), split, 0};
+            best.smem = fixed + best.slots * slot_bytes(tiles);
+        }
     }
-    r.slots = 0;
-    return r;
+    return best;
 }
 
-template <int TILES, int COLS, typename XT>
+template <int TILES, int COLS, int SPREAD, bool SPLIT_TERMS, typename XT>
 cudaError_t launch(const CUtensorMap& map, const Params& p, uint32_t ctas, uint32_t smem, cudaStream_t stream) {
-    auto kernel = decode_mxfp4_kernel<TILES, COLS, XT>;
+    auto kernel = decode_mxfp4_kernel<TILES, COLS, SPREAD, SPLIT_TERMS, XT>;
     static std::atomic<uint8_t> configured[gemm::kMaxDevices];
     if (cudaError_t st = gemm::opt_in_smem(configured, kernel, kSmemLimit); st != cudaSuccess) return st;
     cudaLaunchConfig_t cfg = {};
@@ -385,28 +590,57 @@ cudaError_t launch(const CUtensorMap& map, const Params& p, uint32_t ctas, uint3
     cfg.blockDim = dim3(32 * (p.warps + 1));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = p.split > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, map, p);
 }
-template <int COLS, typename XT>
-cudaError_t launch_tiles(uint32_t tiles, const CUtensorMap& map, const Params& p, uint32_t ctas, uint32_t smem, cudaStream_t stream) {
-    switch (tiles) {
-        case 1: return launch<1, COLS, XT>(map, p, ctas, smem, stream);
-        case 2: return launch<2, COLS, XT>(map, p, ctas, smem, stream);
-        case 3: return launch<3, COLS, XT>(map, p, ctas, smem, stream);
-        case 4: return launch<4, COLS, XT>(map, p, ctas, smem, stream);
-        default: return launch<6, COLS, XT>(map, p, ctas, smem, stream);
+struct Call {
+    Plan& plan;
+    Params p;
+    const uint8_t* w_values;
+    cudaStream_t stream;
+};
+template <int COLS, int SPREAD, bool SPLIT_TERMS, typename XT> cudaError_t run(Call& call) {
+    Params& p = call.p;
+    const Cut how = cut(p.n, p.k, p.pitch, SPREAD == 8 ? 8 : 4, static_cast<uint32_t>(gemm::sm_count()));
+    if (how.slots == 0) return cudaErrorInvalidValue;
+    const CUtensorMap* map;
+    cudaError_t st = call.plan.maps_w.get(&map, call.w_values, p.n, p.k / 2, p.k / 2, how.rows);
+    if (st != cudaSuccess) return st;
+    p.rows = how.rows;
+    p.passes = how.passes;
+    p.chunks = (p.k + 2 * kChunkBytes - 1) / (2 * kChunkBytes);
+    p.slots = how.slots;
+    p.warps = how.warps;
+    p.split = how.split;
+    const uint32_t ctas = (p.n + how.rows * how.passes - 1) / (how.rows * how.passes) * how.split;
+    switch (how.tiles) {
+        case 1: return launch<1, COLS, SPREAD, SPLIT_TERMS, XT>(*map, p, ctas, how.smem, call.stream);
+        case 2: return launch<2, COLS, SPREAD, SPLIT_TERMS, XT>(*map, p, ctas, how.smem, call.stream);
+        default: return launch<3, COLS, SPREAD, SPLIT_TERMS, XT>(*map, p, ctas, how.smem, call.stream);
     }
 }
-template <typename XT>
-cudaError_t launch_cols(uint32_t cols, uint32_t tiles, const CUtensorMap& map, const Params& p, uint32_t ctas, uint32_t smem, cudaStream_t stream) {
-    if (cols == 1) return launch_tiles<1, XT>(tiles, map, p, ctas, smem, stream);
-    if (cols == 2) return launch_tiles<2, XT>(tiles, map, p, ctas, smem, stream);
-    return launch_tiles<4, XT>(tiles, map, p, ctas, smem, stream);
+cudaError_t run_tokens(Call& call, bool bf16) {
+    const uint32_t tokens = call.p.tokens;
+    if (bf16) {
+        if (tokens == 1) return run<1, 8, false, uint16_t>(call);
+        if (tokens == 2) return run<1, 4, false, uint16_t>(call);
+        if (tokens <= 4) return run<1, 2, false, uint16_t>(call);
+        if (tokens <= 8) return run<1, 1, false, uint16_t>(call);
+        return tokens <= 16 ? run<2, 1, false, uint16_t>(call) : run<4, 1, false, uint16_t>(call);
+    }
+    if (tokens == 1) return run<1, 4, true, float>(call);
+    if (tokens == 2) return run<1, 2, true, float>(call);
+    if (tokens <= 4) return run<1, 1, true, float>(call);
+    if (tokens <= 8) return run<1, 1, false, float>(call);
+    return tokens <= 16 ? run<2, 1, false, float>(call) : run<4, 1, false, float>(call);
 }
 
 }  // namespace decode_mx
@@ -452,14 +686,9 @@ cudaError_t eider_b200_mxfp4_w4a16_gemv_on_stream(void* raw, const void* input, 
         return cudaErrorInvalidValue;
     const uint32_t groups = (tokens + 31) / 32, each = (tokens + groups - 1) / groups;
     for (uint32_t first = 0; first < tokens; first += each) {
-        Params p{};
+        Call call{*plan, {}, w_values, stream};
+        Params& p = call.p;
         p.tokens = std::min(each, tokens - first);
-        const uint32_t cols = p.tokens <= 8 ? 1 : p.tokens <= 16 ? 2 : 4;
-        const Cut how = cut(plan->n, plan->k, scale_pitch, static_cast<uint32_t>(gemm::sm_count()));
-        if (how.slots == 0) return cudaErrorInvalidValue;
-        const CUtensorMap* map;
-        cudaError_t st = plan->maps_w.get(&map, w_values, plan->n, plan->k / 2, plan->k / 2, how.rows);
-        if (st != cudaSuccess) return st;
         const size_t x_bytes = input_is_bf16 ? 2 : 4, out_bytes = out_is_bf16 ? 2 : 4;
         p.x = static_cast<const uint8_t*>(input) + first * x_bytes * plan->k;
         p.scales = w_scales_rows;
@@ -471,14 +700,7 @@ cudaError_t eider_b200_mxfp4_w4a16_gemv_on_stream(void* raw, const void* input, 
         p.n = plan->n;
         p.k = plan->k;
         p.pitch = scale_pitch;
-        p.rows = how.rows;
-        p.passes = how.passes;
-        p.chunks = (plan->k + 2 * kChunkBytes - 1) / (2 * kChunkBytes);
-        p.slots = how.slots;
-        p.warps = how.warps;
-        const uint32_t ctas = (plan->n + how.rows * how.passes - 1) / (how.rows * how.passes);
-        st = input_is_bf16 ? launch_cols<uint16_t>(cols, how.tiles, *map, p, ctas, how.smem, stream)
-                           : launch_cols<float>(cols, how.tiles, *map, p, ctas, how.smem, stream);
+        const cudaError_t st = run_tokens(call, input_is_bf16);
         if (st != cudaSuccess) return st;
     }
     return cudaSuccess;

@@ -212,7 +212,7 @@ SHAPES = [(1, 32), (40, 96), (256, 512), (1000, 2912), (6150, 1056), (3001, 8192
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("tokens", [1, 2, 7, 8, 9, 16, 17, 31, 33, 64])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 8, 9, 16, 17, 31, 33, 64])
 def test_decode(tokens, dtype):
     g = gen(tokens)
     for n, k in SHAPES:
@@ -279,16 +279,19 @@ def test_decode_poison_stays_with_its_token_and_row():
     assert fine[0].sum() >= 98 and ((y.double() - want).abs()[fine] <= (decode_bound(x.double().nan_to_num(0, 0, 0), wv.nan_to_num(0), torch.bfloat16) + 1e-38)[fine]).all()
 
 
-def test_decode_is_the_same_in_every_run_and_grouping():
-    """A token's result does not depend on the tokens beside it (within one group width), and two runs agree bit for bit."""
+@pytest.mark.parametrize("tokens,dtype", [(1, torch.bfloat16), (2, torch.float32), (4, torch.bfloat16), (8, torch.float32), (16, torch.bfloat16), (40, torch.bfloat16)])
+def test_decode_is_the_same_in_every_run_and_order(tokens, dtype):
+    """Two runs agree bit for bit, and a token's result depends neither on its place nor on the tokens beside it."""
     g = gen(13)
     n, k = 6150, 4064
-    x, w = randn(g, 8, k), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k))
-    plan = ops.Mxfp4DecodePlan(8, n, k)
+    x, w = randn(g, tokens, k, dtype=dtype), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k))
+    plan = ops.Mxfp4DecodePlan(64, n, k)
     y = plan.run(x, w, out_dtype=torch.float32)
     assert torch.equal(plan.run(x, w, out_dtype=torch.float32), y)
-    for t in (0, 3, 7):
-        assert torch.equal(plan.run(x[t], w, out_dtype=torch.float32)[0], y[t])
+    order = torch.randperm(tokens, generator=g, device="cuda")
+    assert torch.equal(plan.run(x[order], w, out_dtype=torch.float32), y[order])
+    x[1:] *= 2.0 ** 30
+    assert torch.equal(plan.run(x, w, out_dtype=torch.float32)[0], y[0])
 
 
 # ---- routed experts -----------------------------------------------------------------------------------------------
