@@ -1,17 +1,17 @@
 // W4A16 product of MXFP4 weights for few tokens: y[t][n] = sum_k x[t][k] * w[n][k] (+ beta * C), the weights streamed once.
 //
-// Bound: HBM, N * K * 17/32 bytes of weights.  Every CTA, two of them on an SM, has N / 296 rows of its own for the whole K (as many passes
-// as rows do not fit), or a pair of CTAs N / 148 for half of the K each, so that all SMs stream the same number of bytes whatever N is:
-// one launch, no workspace, the same order of additions in every run.
+// Bound: HBM, N * K * 17/32 bytes of weights.  Every SM has one CTA with N / 148 rows of its own for the whole K (as many passes as rows do
+// not fit), so that all of them stream the same number of bytes whatever N is: one launch, no workspace, the same order of
+// additions in every run.  A CTA takes half of an SM, so that the next launch's is resident beside it, with its barriers set up and its
+// first hundred kilobytes of weights on their way, when this one ends.
 //  * A producer warp streams the rows in chunks of 256 elements (TMA boxes of 128 bytes x rows, 128-byte swizzle) through a ring of
-//    shared memory; weights and scales are requested before the launch in front is awaited, and a CTA of the next launch has room
-//    beside one of this.
-//  * Half a chunk is one warp's, for all of the CTA's rows: 16 rows x 32 elements (a block) at a time through mma.m16n8k16 with the tokens
+//    shared memory; weights and scales are requested before the launch in front is awaited.
+//  * A chunk is one warp's, for all of the CTA's rows: 16 rows x 32 elements (a block) at a time through mma.m16n8k16 with the tokens
 //    as the eight columns.  E2M1 codes become f16 by one conversion per pair (exact), the sum of a block (two MMAs) is taken in f32 and
 //    then added times its block scale in f32, so the weights are never multiplied out and no MMA chain is longer than a block.
 //  * x becomes f16 by a power of two per token and warp that brings its largest element so far to 2^8..2^9 (it grows to 2^15 before the
 //    sums are rescaled): bf16's eight bits fit, f32 goes as two f16 terms.  What is lost lies 2^-33 below the largest element.
-//  * The warps' sums over K meet in shared memory, in warp order, a pair's in that of the first.
+//  * The warps' sums over K meet in shared memory, in warp order.
 #include <algorithm>
 #include <atomic>
 #include <new>
@@ -26,9 +26,10 @@ namespace decode_mx {
 
 constexpr uint32_t kChunkBytes = 128;               // 256 elements of a row
 constexpr uint32_t kChunkBlocks = 8;
-constexpr uint32_t kMaxWarps = 7;                   // consumer warps; with the producer, and two CTAs an SM, 128 registers each
+constexpr uint32_t kMaxWarps = 7;                   // consumer warps; the producer is the eighth
 constexpr uint32_t kMaxTiles = 3;                   // 16-row MMA tiles of a CTA in a pass
-constexpr uint32_t kSmemLimit = 113 * 1024;         // two CTAs an SM, of this launch or of the next one
+// Half of an SM: one CTA of this launch and one of the next.
+constexpr uint32_t kSmemLimit = 113 * 1024;
 constexpr uint32_t kMaxSlots = 32;
 constexpr uint32_t kFull = 0xffffffffu;
 
@@ -41,15 +42,15 @@ struct Params {
     float beta;
     int out_is_bf16;
     uint32_t tokens, n, k, pitch;
-    uint32_t rows;    // of a CTA (pair) in a pass
-    uint32_t passes, chunks, slots, warps;
-    uint32_t split;   // CTAs of a cluster that share the chunks of their rows
+    uint32_t rows;    // of a CTA in a pass
+    uint32_t passes, chunks, warps;
+    uint32_t depth;   // ring slots of a warp
 };
 
 __host__ __device__ constexpr uint32_t reduce_pitch(uint32_t tiles) { return tiles * 16 + 4; }  // (rows of a token; + 4: the fragments' stores meet no bank twice)
 __host__ __device__ constexpr uint32_t slot_bytes(uint32_t tiles) { return tiles * 16 * kChunkBytes; }
-inline uint32_t fixed_bytes(uint32_t tiles, uint32_t warps, uint32_t pitch, uint32_t passes) {
-    return 1024 /*alignment*/ + (passes > 1 ? 2 : 1) * tiles * 16 * pitch + (warps + 1) * 8 * reduce_pitch(tiles) * 4 + (2 * kMaxSlots + 4) * 8 + 16;
+inline uint32_t fixed_bytes(uint32_t tiles, uint32_t warps, uint32_t tokens, uint32_t pitch, uint32_t passes) {
+    return 1024 /*alignment*/ + (passes > 1 ? 2 : 1) * tiles * 16 * pitch + warps * tokens * reduce_pitch(tiles) * 4 + (2 * kMaxSlots + 4) * 8 + 16;
 }
 
 __device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&p)[4]) {
@@ -187,29 +188,29 @@ template <int TILES, int COLS, int SPREAD, bool SPLIT_TERMS, typename XT>
 __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const Params p) {
     constexpr int kTerms = sizeof(XT) == 4 && !SPLIT_TERMS ? 2 : 1;      // MMAs of the same weights
     constexpr int kSpan = SPREAD * (SPLIT_TERMS ? 2 : 1);                // columns of a token
-    constexpr uint32_t kItemBlocks = SPREAD == 8 ? 8 : 4;                // blocks of a work item: a warp's share at a time
+    constexpr uint32_t kStepBlocks = SPREAD == 8 ? 8 : 4;                // blocks of a warp's step
+    constexpr uint32_t kSteps = kChunkBlocks / kStepBlocks;              // steps of a chunk
     constexpr int kStep = COLS * kTerms >= 4 ? 1 : 4 / (COLS * kTerms);  // blocks of x that a warp holds (and has on their way) at a time, COLS > 1
-    constexpr int kGroups = kItemBlocks / SPREAD;                        // the same for COLS 1: a block of each of these groups
+    constexpr int kGroups = kStepBlocks / SPREAD;                        // the same for COLS 1: a block of each of these groups
+    constexpr int kAhead = SPREAD == 8 || (SPREAD == 4 && sizeof(XT) == 2) ? 4 : SPREAD > 1 ? 2 : 1;  // steps whose x is on its way, COLS 1
+    constexpr uint32_t kTokens = 8 / kSpan;                              // of a group of eight columns
     static_assert(COLS == 1 || (SPREAD == 1 && !SPLIT_TERMS), "columns are spread within one group of eight");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    const uint32_t scale_bytes = TILES * 16 * p.pitch;
-    uint8_t* scales = ring + p.slots * slot_bytes(TILES);
-    float* sums = reinterpret_cast<float*>(scales + (p.passes > 1 ? 2 : 1) * scale_bytes);  // [warps][8][rows], then the other CTA's [8][rows]
-    uint64_t* full = reinterpret_cast<uint64_t*>(sums + (p.warps + 1) * 8 * reduce_pitch(TILES));  // [slots]
+    const uint32_t scale_bytes = TILES * 16 * p.pitch, slots = p.warps * p.depth;
+    uint8_t* scales = ring + slots * slot_bytes(TILES);
+    float* sums = reinterpret_cast<float*>(scales + (p.passes > 1 ? 2 : 1) * scale_bytes);  // [warps][kTokens][rows]
+    uint64_t* full = reinterpret_cast<uint64_t*>(sums + p.warps * kTokens * reduce_pitch(TILES));  // [slots]
     uint64_t* empty = full + kMaxSlots;                                                           // [slots]
     uint64_t* scales_full = empty + kMaxSlots;                                                    // [2]
     uint64_t* scales_empty = scales_full + 2;                                                     // [2]
     volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(scales_empty + 2);
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = p.split > 1 ? umma::cluster_ctarank() : 0, group = p.split > 1 ? blockIdx.x / p.split : blockIdx.x;
-    const uint32_t groups = p.split > 1 ? gridDim.x / p.split : gridDim.x;
-    const uint32_t chunks = (p.chunks + p.split - 1 - rank) / p.split;  // this CTA's: rank, rank + split, ..
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < p.slots; ++i) {
+        for (uint32_t i = 0; i < slots; ++i) {
             umma::mbar_init(&full[i], 1);
-            umma::mbar_init(&empty[i], kChunkBlocks / kItemBlocks);  // (the warps whose items the chunk is)
+            umma::mbar_init(&empty[i], 1);
         }
         for (uint32_t i = 0; i < 2; ++i) {
             umma::mbar_init(&scales_full[i], 1);
@@ -222,25 +223,30 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
     __syncthreads();
     umma::griddep_launch_dependents();
 
+    // Chunk i (counted through the passes) is warp i % warps' alone, in one of that warp's own slots.  So a warp sees every filling of a
+    // slot that it waits on, and a parity can only mean the filling before or the one it waits for.  (In a ring that all warps share a
+    // warp could come to a slot a lap ahead of a copy that lands late, and take the parity of the lap before for its own.)
+    auto slot_of = [&](uint32_t i) { return i % p.warps * p.depth + i / p.warps % p.depth; };
+    auto phase_of = [&](uint32_t i) { return i / slots & 1; };
+
     if (warp == p.warps) {
         // ------------------------------------------------------------------ producer
         if (lane == 0) {
             uint32_t i = 0, pass = 0;
             bool ok = true;
             for (; ok && pass < p.passes; ++pass) {
-                const uint32_t row0 = (pass * groups + group) * p.rows;
+                const uint32_t row0 = (pass * gridDim.x + blockIdx.x) * p.rows;
                 if (row0 >= p.n) break;
                 const uint32_t buffer = pass & 1;
                 if (!umma::mbar_wait(&scales_empty[buffer], ((pass >> 1) & 1) ^ 1, abort_flag, p.status, umma::kTimeoutEmpty)) break;  // (pass: those begun)
                 const uint32_t bytes = min(p.rows, p.n - row0) * p.pitch;
                 umma::mbar_arrive_expect_tx(&scales_full[buffer], bytes);
                 umma::bulk_load_1d(scales + buffer * scale_bytes, p.scales + static_cast<size_t>(row0) * p.pitch, bytes, &scales_full[buffer]);
-                for (uint32_t c = 0; c < chunks; ++c, ++i) {
-                    const uint32_t slot = i % p.slots, phase = (i / p.slots) & 1;
-                    if (!umma::mbar_wait(&empty[slot], phase ^ 1, abort_flag, p.status, umma::kTimeoutEmpty)) { ok = false; break; }
+                for (uint32_t c = 0; c < p.chunks; ++c, ++i) {
+                    const uint32_t slot = slot_of(i);
+                    if (!umma::mbar_wait(&empty[slot], phase_of(i) ^ 1, abort_flag, p.status, umma::kTimeoutEmpty)) { ok = false; break; }
                     umma::mbar_arrive_expect_tx(&full[slot], p.rows * kChunkBytes);
-                    umma::tma_load_2d(ring + slot * slot_bytes(TILES), &map_w, &full[slot], static_cast<int32_t>((c * p.split + rank) * kChunkBytes),
-                                      static_cast<int32_t>(row0));
+                    umma::tma_load_2d(ring + slot * slot_bytes(TILES), &map_w, &full[slot], static_cast<int32_t>(c * kChunkBytes), static_cast<int32_t>(row0));
                 }
             }
             // The block does not leave before its copies have landed, not even after a wait ran out: bounded too.
@@ -248,16 +254,8 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
             auto landed = [&](uint64_t* bar, uint32_t parity) {
                 while (!umma::mbar_try_wait(bar, parity) && clock64() - start < umma::kWaitLimitCycles) {}
             };
-            for (uint32_t j = i > p.slots ? i - p.slots : 0; j < i; ++j) landed(&full[j % p.slots], (j / p.slots) & 1);
+            for (uint32_t j = i > slots ? i - slots : 0; j < i; ++j) landed(&full[slot_of(j)], phase_of(j));
             for (uint32_t j = pass > 2 ? pass - 2 : 0; j < pass; ++j) landed(&scales_full[j & 1], (j >> 1) & 1);
-        }
-        __syncwarp();
-        if (p.split > 1) {  // (the meetings below are the whole cluster's)
-            for (uint32_t pass = 0; pass < p.passes && (pass * groups + group) * p.rows < p.n; ++pass)
-                for (uint32_t n = 0; n < COLS && n * 8 < p.tokens * kSpan; ++n) {
-                    umma::cluster_sync_all();
-                    umma::cluster_sync_all();
-                }
         }
         return;
     }
@@ -266,8 +264,6 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
     const uint32_t g = lane >> 2, t = lane & 3;
     const uint32_t blocks = p.k / mx::kBlock;
     const uint32_t ring_addr = umma::smem_u32(ring), scales_addr = umma::smem_u32(scales);
-    constexpr uint32_t kPerChunk = kChunkBlocks / kItemBlocks;
-    const uint32_t items = chunks * kPerChunk;
     umma::griddep_wait();
     const XT* x = static_cast<const XT*>(p.x) + t * 8;
     const uint32_t sub = g % SPREAD;  // this lane's block of SPREAD
@@ -279,11 +275,9 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
         live[n] = token < p.tokens;
         x_of[n] = x + (live[n] ? static_cast<size_t>(token) * p.k : 0) + sub * mx::kBlock;
     }
-    // first block (of K) of this CTA's item
-    auto item_block = [&](uint32_t item) { return (item / kPerChunk * p.split + rank) * kChunkBlocks + item % kPerChunk * kItemBlocks; };
     bool ok = true;
     for (uint32_t pass = 0; pass < p.passes; ++pass) {
-        const uint32_t row0 = (pass * groups + group) * p.rows;
+        const uint32_t row0 = (pass * gridDim.x + blockIdx.x) * p.rows;
         if (row0 >= p.n) break;
         float acc[TILES][COLS][4];
 #pragma unroll
@@ -325,25 +319,37 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
             return factor[n] == 0.0f ? 1.0f : factor[n];
         };
         constexpr int kHeld = COLS == 1 ? kGroups : kStep;
-        Raw8<XT> raw[COLS][kHeld];
+        Raw8<XT> raw[COLS][kHeld], later[kAhead - 1 + (kAhead == 1)][kHeld];  // (`later`: of the steps behind the next, COLS 1)
         auto load_x = [&](uint32_t block) {
 #pragma unroll
             for (int n = 0; n < COLS; ++n)
 #pragma unroll
                 for (int s = 0; s < kHeld; ++s) raw[n][s].load(x_of[n] + (block + s * SPREAD) * mx::kBlock, live[n] && block + s * SPREAD + sub < blocks);
         };
-        if (warp < items) load_x(item_block(warp));
+        // this warp's chunks of the pass are first, first + warps, ..; its step q lies at block_at(q) of K (behind the last at or past `blocks`)
+        const uint32_t chunk0 = pass * p.chunks, first = (warp + p.warps - chunk0 % p.warps) % p.warps;
+        auto block_at = [&](uint32_t q) { return (first + q / kSteps * p.warps) * kChunkBlocks + q % kSteps * kStepBlocks; };
+        auto load_later = [&](Raw8<XT>(&to)[kHeld], uint32_t q) {
+            const uint32_t block = block_at(q);
+#pragma unroll
+            for (int s = 0; s < kHeld; ++s) to[s].load(x_of[0] + (block + s * SPREAD) * mx::kBlock, live[0] && block + s * SPREAD + sub < blocks);
+        };
+        load_x(block_at(0));
+        if constexpr (COLS == 1) {
+#pragma unroll
+            for (int a = 0; a + 1 < kAhead; ++a) load_later(later[a], a + 1);
+        }
         if (ok && !umma::mbar_wait(&scales_full[pass & 1], (pass >> 1) & 1, abort_flag, p.status, umma::kTimeoutFull)) ok = false;
         const uint32_t pass_scales = scales_addr + (pass & 1) * scale_bytes + g * p.pitch;
-        for (uint32_t item = warp; ok && item < items; item += p.warps) {
-            const uint32_t i = pass * chunks + item / kPerChunk, slot = i % p.slots, phase = (i / p.slots) & 1;
-            const uint32_t block0 = item_block(item);
-            const uint32_t tile = ring_addr + slot * slot_bytes(TILES) + g * kChunkBytes + t * 4, half = item % kPerChunk * kItemBlocks;
+        for (uint32_t q = 0; ok && first + q / kSteps * p.warps < p.chunks; ++q) {
+            const uint32_t i = chunk0 + first + q / kSteps * p.warps, slot = slot_of(i);
+            const uint32_t block0 = block_at(q);
+            const uint32_t tile = ring_addr + slot * slot_bytes(TILES) + g * kChunkBytes + t * 4, half = q % kSteps * kStepBlocks;
             auto arrive = [&] {
-                ok = __all_sync(kFull, umma::mbar_wait(&full[slot], phase, abort_flag, p.status, umma::kTimeoutFull));
+                ok = __all_sync(kFull, umma::mbar_wait(&full[slot], phase_of(i), abort_flag, p.status, umma::kTimeoutFull));
                 return ok;
             };
-            // block `in` of the item: rows of tile u as f16
+            // block `in` of the step: rows of tile u as f16
             auto weights = [&](uint32_t in, int u, uint32_t (&lo)[4], uint32_t (&hi)[4]) {
                 const uint32_t at = tile + (((half + in) ^ g) << 4);
                 e2m1_f16(lds32(at + u * 16 * kChunkBytes), lo);
@@ -371,7 +377,17 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
                         raw[0][s].terms(f, b[s]);
                     }
                 }
-                if (item + p.warps < items) load_x(item_block(item + p.warps));
+                if constexpr (kAhead == 1) {
+                    load_later(raw[0], q + 1);
+                } else {
+#pragma unroll
+                    for (int s = 0; s < kHeld; ++s) raw[0][s] = later[0][s];
+#pragma unroll
+                    for (int a = 0; a + 2 < kAhead; ++a)
+#pragma unroll
+                        for (int s = 0; s < kHeld; ++s) later[a][s] = later[a + 1][s];
+                    load_later(later[kAhead - 2], q + kAhead);
+                }
                 if (!arrive()) break;
                 [[maybe_unused]] uint32_t lo4[TILES], hi4[TILES];
                 if constexpr (SPREAD == 1) {
@@ -427,7 +443,7 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
                 });
             } else {
                 uint32_t lo4[TILES], hi4[TILES];
-                static_for<kItemBlocks / kStep>([&](auto which) {
+                static_for<kStepBlocks / kStep>([&](auto which) {
                     constexpr int step = decltype(which)::value * kStep;
                     if (!ok) return;
                     // this step's x as f16, then the next step's is requested
@@ -446,8 +462,7 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
 #pragma unroll
                         for (int s = 0; s < kStep; ++s) raw[n][s].terms(f, b[s][n]);
                     }
-                    if (step + kStep < static_cast<int>(kItemBlocks)) load_x(block0 + step + kStep);
-                    else if (item + p.warps < items) load_x(item_block(item + p.warps));
+                    load_x(step + kStep < static_cast<int>(kStepBlocks) ? block0 + step + kStep : block_at(q + 1));
                     if (step == 0) {
                         if (!arrive()) return;
 #pragma unroll
@@ -483,12 +498,11 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
                 if (!ok) break;
             }
             __syncwarp();
-            if (ok && lane == 0) umma::mbar_arrive(&empty[slot]);
+            if (ok && lane == 0 && q % kSteps == kSteps - 1) umma::mbar_arrive(&empty[slot]);
         }
         if (lane == 0) umma::mbar_arrive(&scales_empty[pass & 1]);
 
-        // ------------------------------------------------------------------ the warps' (and CTAs') sums meet, eight tokens at a time
-        float* others = sums + p.warps * 8 * reduce_pitch(TILES);
+        // ------------------------------------------------------------------ the warps' sums meet, eight tokens at a time
 #pragma unroll
         for (int n = 0; n < COLS; ++n) {
             if (n * 8 >= p.tokens * kSpan) break;
@@ -496,51 +510,49 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(c
             const uint32_t field = __float_as_uint(factor[n]) >> 23;
             const float back = factor[n] == 0.0f ? 1.0f : __uint_as_float(field == 254 ? 0x00400000u : (254u - field) << 23);
             const float b0 = __shfl_sync(kFull, back, t * 8), b1 = __shfl_sync(kFull, back, t * 8 + 4);
-            float* mine = sums + warp * 8 * reduce_pitch(TILES);
+            float* mine = sums + warp * kTokens * reduce_pitch(TILES);
 #pragma unroll
             for (int u = 0; u < TILES; ++u) {
-                mine[(2 * t) * reduce_pitch(TILES) + u * 16 + g] = acc[u][n][0] * b0;
-                mine[(2 * t + 1) * reduce_pitch(TILES) + u * 16 + g] = acc[u][n][1] * b1;
-                mine[(2 * t) * reduce_pitch(TILES) + u * 16 + g + 8] = acc[u][n][2] * b0;
-                mine[(2 * t + 1) * reduce_pitch(TILES) + u * 16 + g + 8] = acc[u][n][3] * b1;
+                if constexpr (kSpan == 1) {
+                    mine[(2 * t) * reduce_pitch(TILES) + u * 16 + g] = acc[u][n][0] * b0;
+                    mine[(2 * t + 1) * reduce_pitch(TILES) + u * 16 + g] = acc[u][n][1] * b1;
+                    mine[(2 * t) * reduce_pitch(TILES) + u * 16 + g + 8] = acc[u][n][2] * b0;
+                    mine[(2 * t + 1) * reduce_pitch(TILES) + u * 16 + g + 8] = acc[u][n][3] * b1;
+                } else {  // a token's columns
+                    float lo = acc[u][n][0] * b0 + acc[u][n][1] * b1, hi = acc[u][n][2] * b0 + acc[u][n][3] * b1;
+#pragma unroll
+                    for (int o = 1; o < kSpan / 2; o *= 2) {
+                        lo += __shfl_xor_sync(kFull, lo, o);
+                        hi += __shfl_xor_sync(kFull, hi, o);
+                    }
+                    if ((2 * t) % kSpan == 0) {
+                        mine[2 * t / kSpan * reduce_pitch(TILES) + u * 16 + g] = lo;
+                        mine[2 * t / kSpan * reduce_pitch(TILES) + u * 16 + g + 8] = hi;
+                    }
+                }
             }
             asm volatile("bar.sync 1, %0;" ::"r"(p.warps * 32) : "memory");
-            const uint32_t tokens = min(8u / kSpan, p.tokens - n * 8), rows = min(p.rows, p.n - row0);
+            const uint32_t tokens = min(kTokens, p.tokens - n * 8), rows = min(p.rows, p.n - row0);
             auto warps_sum = [&](uint32_t token, uint32_t row) {
                 float sum = 0.0f;
-                for (uint32_t w = 0; w < p.warps; ++w)
-#pragma unroll
-                    for (uint32_t c = 0; c < kSpan; ++c) sum += sums[(w * 8 + token * kSpan + c) * reduce_pitch(TILES) + row];
+                for (uint32_t w = 0; w < p.warps; ++w) sum += sums[(w * kTokens + token) * reduce_pitch(TILES) + row];
                 return sum;
             };
-            if (p.split > 1) {
-                if (rank != 0) {
-                    const uint32_t there = umma::map_to_cta(umma::smem_u32(others), 0);
-                    for (uint32_t i = threadIdx.x; i < tokens * rows; i += p.warps * 32) {
-                        const uint32_t token = i / rows, row = i - token * rows;
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there + (token * reduce_pitch(TILES) + row) * 4), "f"(warps_sum(token, row)) : "memory");
-                    }
+            for (uint32_t i = threadIdx.x; i < tokens * rows; i += p.warps * 32) {
+                const uint32_t token = i / rows, row = i - token * rows;
+                float sum = warps_sum(token, row);
+                if (!(fabsf(sum) < INFINITY)) {  // a NaN scale among the row's?
+                    const uint8_t* s = p.scales + static_cast<size_t>(row0 + row) * p.pitch;
+                    for (uint32_t q = 0; q < blocks; ++q)
+                        if (s[q] == mx::kNanCode) sum = NAN;
                 }
-                umma::cluster_sync_all();
+                const size_t index = static_cast<size_t>(n * 8 + token) * p.n + row0 + row;
+                if (p.beta != 0.0f)
+                    sum = fmaf(p.beta, p.out_is_bf16 ? bf16_bits_to_float(static_cast<const uint16_t*>(p.c)[index]) : static_cast<const float*>(p.c)[index], sum);
+                if (p.out_is_bf16) static_cast<uint16_t*>(p.out)[index] = float_to_bf16_bits(sum);
+                else static_cast<float*>(p.out)[index] = sum;
             }
-            if (rank == 0)
-                for (uint32_t i = threadIdx.x; i < tokens * rows; i += p.warps * 32) {
-                    const uint32_t token = i / rows, row = i - token * rows;
-                    float sum = warps_sum(token, row);
-                    if (p.split > 1) sum += others[token * reduce_pitch(TILES) + row];
-                    if (!(fabsf(sum) < INFINITY)) {  // a NaN scale among the row's?
-                        const uint8_t* s = p.scales + static_cast<size_t>(row0 + row) * p.pitch;
-                        for (uint32_t q = 0; q < blocks; ++q)
-                            if (s[q] == mx::kNanCode) sum = NAN;
-                    }
-                    const size_t index = static_cast<size_t>(n * 8 + token) * p.n + row0 + row;
-                    if (p.beta != 0.0f)
-                        sum = fmaf(p.beta, p.out_is_bf16 ? bf16_bits_to_float(static_cast<const uint16_t*>(p.c)[index]) : static_cast<const float*>(p.c)[index], sum);
-                    if (p.out_is_bf16) static_cast<uint16_t*>(p.out)[index] = float_to_bf16_bits(sum);
-                    else static_cast<float*>(p.out)[index] = sum;
-                }
-            if (p.split > 1) umma::cluster_sync_all();
-            else asm volatile("bar.sync 1, %0;" ::"r"(p.warps * 32) : "memory");
+            asm volatile("bar.sync 1, %0;" ::"r"(p.warps * 32) : "memory");
         }
     }
 }
@@ -551,33 +563,28 @@ struct Plan {
     gemm::MapCache maps_w;
 };
 
-// How a call is cut: rows of a CTA (pair) and pass, MMA tiles they take, consumer warps, ring slots.
+// How a call is cut: rows of a CTA and pass, MMA tiles they take, consumer warps, ring slots of a warp.
 struct Cut {
-    uint32_t rows, passes, tiles, warps, slots, split, smem;
+    uint32_t rows, passes, tiles, warps, depth, smem;
 };
-inline Cut cut(uint32_t n, uint32_t k, uint32_t pitch, uint32_t item_blocks, uint32_t sms) {
+inline Cut cut(uint32_t n, uint32_t k, uint32_t pitch, uint32_t tokens, uint32_t sms) {
     const uint32_t chunks = (k + 2 * kChunkBytes - 1) / (2 * kChunkBytes);
-    Cut best{};
-    float best_cost = 1e30f;
-    for (uint32_t split = 1; split <= 2 && split <= chunks; ++split) {
-        const uint32_t mine = (chunks + split - 1) / split, items = mine * (kChunkBlocks / item_blocks);
-        const uint32_t rounds = (items + kMaxWarps - 1) / kMaxWarps;  // items of the warp that has most
-        const uint32_t warps = (items + rounds - 1) / rounds, groups = 2 * sms / split;
-        for (uint32_t tiles = 1; tiles <= kMaxTiles; ++tiles) {
-            const uint32_t passes = (n + groups * tiles * 16 - 1) / (groups * tiles * 16), rows = (n + groups * passes - 1) / (groups * passes);
-            if ((rows + 15) / 16 != tiles) continue;
-            if (split > 1 && passes > 1) continue;  // (the producer joins the pair's meetings only once all of its loads are out)
-            const uint32_t fixed = fixed_bytes(tiles, warps, pitch, passes);
-            if (fixed + 2 * slot_bytes(tiles) > kSmemLimit) continue;
-            // a warp's time: its items of every pass, a tile's share of each and the activation's, and the meeting at a pass's end
-            const float cost = passes * (rounds * (tiles + 0.8f) * (item_blocks / 4) + 3.0f + (split > 1 ? 2.0f : 0.0f));
-            if (cost >= best_cost) continue;
-            best_cost = cost;
-            best = Cut{rows, passes, tiles, warps, std::min(std::min(kMaxSlots, mine * passes), (kSmemLimit - fixed) / slot_bytes(tiles)), split, 0};
-            best.smem = fixed + best.slots * slot_bytes(tiles);
-        }
+    Cut r{};
+    for (uint32_t most = kMaxTiles; most > 0; --most) {
+        r.passes = (n + sms * most * 16 - 1) / (sms * most * 16);
+        r.rows = (n + sms * r.passes - 1) / (sms * r.passes);
+        r.tiles = (r.rows + 15) / 16;
+        // as few warps as leave the one with most chunks no more of them
+        const uint32_t all = chunks * r.passes, rounds = (all + kMaxWarps - 1) / kMaxWarps;
+        r.warps = (all + rounds - 1) / rounds;
+        const uint32_t fixed = fixed_bytes(r.tiles, r.warps, tokens, pitch, r.passes), slot = slot_bytes(r.tiles) * r.warps;
+        if (fixed + slot > kSmemLimit) continue;  // (long rows of scales: fewer of them at a time)
+        r.depth = std::min(std::min(kMaxSlots / r.warps, rounds), (kSmemLimit - fixed) / slot);
+        r.smem = fixed + r.depth * slot;
+        return r;
     }
-    return best;
+    r.depth = 0;
+    return r;
 }
 
 template <int TILES, int COLS, int SPREAD, bool SPLIT_TERMS, typename XT>
@@ -590,15 +597,11 @@ cudaError_t launch(const CUtensorMap& map, const Params& p, uint32_t ctas, uint3
     cfg.blockDim = dim3(32 * (p.warps + 1));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
+    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = p.split;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = p.split > 1 ? 2 : 1;
+    cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, map, p);
 }
 struct Call {
@@ -609,18 +612,17 @@ struct Call {
 };
 template <int COLS, int SPREAD, bool SPLIT_TERMS, typename XT> cudaError_t run(Call& call) {
     Params& p = call.p;
-    const Cut how = cut(p.n, p.k, p.pitch, SPREAD == 8 ? 8 : 4, static_cast<uint32_t>(gemm::sm_count()));
-    if (how.slots == 0) return cudaErrorInvalidValue;
+    const Cut how = cut(p.n, p.k, p.pitch, 8 / (SPREAD * (SPLIT_TERMS ? 2 : 1)), static_cast<uint32_t>(gemm::sm_count()));
+    if (how.depth == 0) return cudaErrorInvalidValue;
     const CUtensorMap* map;
     cudaError_t st = call.plan.maps_w.get(&map, call.w_values, p.n, p.k / 2, p.k / 2, how.rows);
     if (st != cudaSuccess) return st;
     p.rows = how.rows;
     p.passes = how.passes;
     p.chunks = (p.k + 2 * kChunkBytes - 1) / (2 * kChunkBytes);
-    p.slots = how.slots;
+    p.depth = how.depth;
     p.warps = how.warps;
-    p.split = how.split;
-    const uint32_t ctas = (p.n + how.rows * how.passes - 1) / (how.rows * how.passes) * how.split;
+    const uint32_t ctas = (p.n + how.rows * how.passes - 1) / (how.rows * how.passes);
     switch (how.tiles) {
         case 1: return launch<1, COLS, SPREAD, SPLIT_TERMS, XT>(*map, p, ctas, how.smem, call.stream);
         case 2: return launch<2, COLS, SPREAD, SPLIT_TERMS, XT>(*map, p, ctas, how.smem, call.stream);
