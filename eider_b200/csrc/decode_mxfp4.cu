@@ -1,57 +1,68 @@
 // W4A16 product of MXFP4 weights for few tokens: y[t][n] = sum_k x[t][k] * w[n][k] (+ beta * C), the weights streamed once.
 //
-// Bound: HBM, N * K * 17/32 bytes of weights.  Every SM has one CTA with N / 148 rows of its own for the whole K (as many passes as rows do
-// not fit), so that all of them stream the same number of bytes whatever N is: one launch, no workspace, the same order of
-// additions in every run.  A CTA takes half of an SM, so that the next launch's is resident beside it, with its barriers set up and its
-// first hundred kilobytes of weights on their way, when this one ends.
-//  * A producer warp streams the rows in chunks of 256 elements (TMA boxes of 128 bytes x rows, 128-byte swizzle) through a ring of
-//    shared memory; weights and scales are requested before the launch in front is awaited.
-//  * A chunk is one warp's, for all of the CTA's rows: 16 rows x 32 elements (a block) at a time through mma.m16n8k16 with the tokens
-//    as the eight columns.  E2M1 codes become f16 by one conversion per pair (exact), the sum of a block (two MMAs) is taken in f32 and
-//    then added times its block scale in f32, so the weights are never multiplied out and no MMA chain is longer than a block.
-//  * x becomes f16 by a power of two per token and warp that brings its largest element so far to 2^8..2^9 (it grows to 2^15 before the
-//    sums are rescaled): bf16's eight bits fit, f32 goes as two f16 terms.  What is lost lies 2^-33 below the largest element.
+// Bound: HBM, N * K * 17/32 bytes of weights.  A CTA of eight warps has 16 or 32 rows and their whole K, so nothing leaves a CTA but its
+// results: no partial sums, the same order of additions in every run.
+//  * A warp has every eighth step of 128 elements of the CTA's rows, which it copies (cp.async) into a ring of its own: warps never
+//    wait for each other.  Scales and the first steps are requested before the launch in front is awaited; three CTAs an SM have
+//    up to 190 KB on their way.
+//  * 16 rows x 32 elements (a block) at a time go through mma.m16n8k16 with the tokens as the eight columns.  E2M1 codes become f16 by
+//    one conversion per pair (exact), the sum of a block (two MMAs) is taken in f32 and then added times its block scale in f32, so
+//    the weights are never multiplied out and no MMA chain is longer than a block.
+//  * x is made f16 by a launch of its own (prepare_mxfp4_kernel), which runs while the weights are on their way.  Made in the loop, with a
+//    maximum, two shuffles and a vote a step in front of the MMAs, the product took 13.2 us for one token and 16.6 for eight
+//    (K 5120 -> N 13824), with eight warps or sixteen.
 //  * The warps' sums over K meet in shared memory, in warp order.
 #include <algorithm>
 #include <atomic>
 #include <new>
 
 #include "gemm_launch.cuh"
-#include "tensor_maps.cuh"
 #include "mx_block.cuh"
 #include "eider_b200.h"
 
 namespace eider {
 namespace decode_mx {
 
-constexpr uint32_t kChunkBytes = 128;               // 256 elements of a row
-constexpr uint32_t kChunkBlocks = 8;
-constexpr uint32_t kMaxWarps = 7;                   // consumer warps; the producer is the eighth
-constexpr uint32_t kMaxTiles = 3;                   // 16-row MMA tiles of a CTA in a pass
-// Half of an SM: one CTA of this launch and one of the next.
-constexpr uint32_t kSmemLimit = 113 * 1024;
-constexpr uint32_t kMaxSlots = 32;
+constexpr uint32_t kWarps = 8;
+constexpr uint32_t kStepBytes = 64, kStepBlocks = 4;  // of a row: 128 elements
+constexpr uint32_t kMaxDepth = 8;                     // steps a warp has on their way
+constexpr uint32_t kSmemThird = 75 * 1024, kSmemMost = 227 * 1024;
 constexpr uint32_t kFull = 0xffffffffu;
 
 struct Params {
-    const void* x;
+    const uint16_t* x;      // prepared: f16 [tokens * terms][k]
+    const float* back;      // [tokens]: what a token's sums are multiplied by
+    const uint8_t* w;       // [n][k / 2]
     const uint8_t* scales;  // [n][pitch]
     void* out;
     const void* c;
-    uint32_t* status;
     float beta;
     int out_is_bf16;
-    uint32_t tokens, n, k, pitch;
-    uint32_t rows;    // of a CTA in a pass
-    uint32_t passes, chunks, warps;
-    uint32_t depth;   // ring slots of a warp
+    uint32_t tokens, n, k, pitch, depth;
 };
 
 __host__ __device__ constexpr uint32_t reduce_pitch(uint32_t tiles) { return tiles * 16 + 4; }  // (rows of a token; + 4: the fragments' stores meet no bank twice)
-__host__ __device__ constexpr uint32_t slot_bytes(uint32_t tiles) { return tiles * 16 * kChunkBytes; }
-inline uint32_t fixed_bytes(uint32_t tiles, uint32_t warps, uint32_t tokens, uint32_t pitch, uint32_t passes) {
-    return 1024 /*alignment*/ + (passes > 1 ? 2 : 1) * tiles * 16 * pitch + warps * tokens * reduce_pitch(tiles) * 4 + (2 * kMaxSlots + 4) * 8 + 16;
+
+// 16 bytes into shared memory, zeros if not `live`.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }
+// All but the newest `pending` groups of copies are there.
+__device__ __forceinline__ void wait_copies(uint32_t pending) {
+    switch (pending) {
+        case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+        case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+        case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+        case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+        case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+        case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+        case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
+        case 7: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
+        default: asm volatile("cp.async.wait_group 8;" ::: "memory"); break;
+    }
+}
+// Rows are 64 bytes: piece c of row r lies at c ^ swizzle(r), so that eight rows' equal pieces fall on different banks.
+__device__ __forceinline__ uint32_t swizzle(uint32_t row) { return row >> 1 & 3; }
 
 __device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&p)[4]) {
     asm("{\n\t.reg .b8 a, b, c, d;\n\t"
@@ -97,29 +108,29 @@ template <int I> __device__ __forceinline__ float scale_of(uint32_t word) {
     return __uint_as_float(max(field, 0x00400000u));
 }
 
-__device__ __forceinline__ uint32_t lds16(uint32_t address) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(address));
-    return v;
-}
 template <int N, typename F> __device__ __forceinline__ void static_for(F f) {
     if constexpr (N > 0) {
         static_for<N - 1>(f);
         f(std::integral_constant<int, N - 1>{});
     }
 }
-
-// Eight consecutive elements of a token, and what becomes of them: the largest finite magnitude, and f16 terms of x * factor.
+__device__ __forceinline__ uint32_t lds8(uint32_t address) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(address));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t address) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(address));
+    return v;
+}
+// Eight consecutive elements of a token, their largest finite magnitude, and f16 terms of x * factor.
 template <typename T> struct Raw8;
 template <> struct Raw8<uint16_t> {
     uint4 q;
     __device__ __forceinline__ void load(const uint16_t* p, bool live) { q = live ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
     static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
-    __device__ __forceinline__ float amax() const {
-        const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(pair(q.x)), __habs2(pair(q.y))), __hmax2(__habs2(pair(q.z)), __habs2(pair(q.w))));
-        return fmaxf(__low2float(m), __high2float(m));
-    }
     __device__ __forceinline__ void values(float (&v)[8]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -151,9 +162,6 @@ template <> struct Raw8<float> {
         a = live ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
         b = live ? __ldg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
     }
-    __device__ __forceinline__ float amax() const {
-        return fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))), fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
-    }
     __device__ __forceinline__ void values(float (&v)[8]) const {
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     }
@@ -178,472 +186,288 @@ template <> struct Raw8<float> {
     }
 };
 
-// TILES: 16-row MMA tiles of a CTA's rows.  COLS: groups of eight MMA columns.
-// SPREAD: consecutive blocks that take an MMA column each (with COLS 1).  Few tokens leave most of the eight columns empty, so block j
-// of SPREAD goes through column j of its token alone: the MMAs of SPREAD blocks add up in one accumulator, whose columns then get
-// their block scales in one go, and every lane converts the activations of one block instead of all of them.  About 18
-// instructions for 16 x 32 weights at SPREAD 8 against 34 at 1.  SPLIT_TERMS: the two f16 terms of f32 are columns too (up to four
-// tokens) instead of MMAs of their own.
-template <int TILES, int COLS, int SPREAD, bool SPLIT_TERMS, typename XT>
-__global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) decode_mxfp4_kernel(const __grid_constant__ CUtensorMap map_w, const Params p) {
-    constexpr int kTerms = sizeof(XT) == 4 && !SPLIT_TERMS ? 2 : 1;      // MMAs of the same weights
-    constexpr int kSpan = SPREAD * (SPLIT_TERMS ? 2 : 1);                // columns of a token
-    constexpr uint32_t kStepBlocks = SPREAD == 8 ? 8 : 4;                // blocks of a warp's step
-    constexpr uint32_t kSteps = kChunkBlocks / kStepBlocks;              // steps of a chunk
-    constexpr int kStep = COLS * kTerms >= 4 ? 1 : 4 / (COLS * kTerms);  // blocks of x that a warp holds (and has on their way) at a time, COLS > 1
-    constexpr int kGroups = kStepBlocks / SPREAD;                        // the same for COLS 1: a block of each of these groups
-    constexpr int kAhead = SPREAD == 8 || (SPREAD == 4 && sizeof(XT) == 2) ? 4 : SPREAD > 1 ? 2 : 1;  // steps whose x is on its way, COLS 1
-    constexpr uint32_t kTokens = 8 / kSpan;                              // of a group of eight columns
-    static_assert(COLS == 1 || (SPREAD == 1 && !SPLIT_TERMS), "columns are spread within one group of eight");
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    const uint32_t scale_bytes = TILES * 16 * p.pitch, slots = p.warps * p.depth;
-    uint8_t* scales = ring + slots * slot_bytes(TILES);
-    float* sums = reinterpret_cast<float*>(scales + (p.passes > 1 ? 2 : 1) * scale_bytes);  // [warps][kTokens][rows]
-    uint64_t* full = reinterpret_cast<uint64_t*>(sums + p.warps * kTokens * reduce_pitch(TILES));  // [slots]
-    uint64_t* empty = full + kMaxSlots;                                                           // [slots]
-    uint64_t* scales_full = empty + kMaxSlots;                                                    // [2]
-    uint64_t* scales_empty = scales_full + 2;                                                     // [2]
-    volatile uint32_t* abort_flag = reinterpret_cast<uint32_t*>(scales_empty + 2);
-
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < slots; ++i) {
-            umma::mbar_init(&full[i], 1);
-            umma::mbar_init(&empty[i], 1);
-        }
-        for (uint32_t i = 0; i < 2; ++i) {
-            umma::mbar_init(&scales_full[i], 1);
-            umma::mbar_init(&scales_empty[i], p.warps);
-        }
-        *abort_flag = 0;
-        umma::fence_barrier_init();
-        umma::prefetch_tensormap(&map_w);
-    }
+// x as f16: every token times the power of two that brings its largest finite element to 2^14..2^15 (bf16's eight bits fit, f32 goes as
+// two terms, row 2 * token and the next), and the inverse.  What is lost lies 2^-38 below the largest element.  One CTA per token.
+constexpr uint32_t kPrepareThreads = 512;
+constexpr uint32_t kHeld = 4;  // groups of eight elements that a thread keeps between the two passes: rows up to 16384
+template <typename XT>
+__global__ void __launch_bounds__(kPrepareThreads) prepare_mxfp4_kernel(const XT* __restrict__ x, uint16_t* __restrict__ prepared, float* __restrict__ back,
+                                                                        uint32_t k) {
+    constexpr uint32_t kTerms = sizeof(XT) == 4 ? 2 : 1;
+    __shared__ uint32_t largest;
+    umma::griddep_launch_dependents();
+    if (threadIdx.x == 0) largest = 0;
     __syncthreads();
+    umma::griddep_wait();
+    const XT* row = x + static_cast<size_t>(blockIdx.x) * k;
+    const uint32_t groups = k / 8;
+    Raw8<XT> held[kHeld];
+    float amax = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld; ++i) held[i].load(row + (threadIdx.x + i * kPrepareThreads) * 8, threadIdx.x + i * kPrepareThreads < groups);
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld; ++i) amax = fmaxf(amax, held[i].finite());
+    for (uint32_t q = threadIdx.x + kHeld * kPrepareThreads; q < groups; q += kPrepareThreads) {
+        Raw8<XT> r;
+        r.load(row + q * 8, true);
+        amax = fmaxf(amax, r.finite());
+    }
+    const uint32_t warp_max = __reduce_max_sync(kFull, __float_as_uint(amax));
+    if (threadIdx.x % 32 == 0) atomicMax(&largest, warp_max);
+    __syncthreads();
+    const uint32_t e = largest >> 23;
+    // 2^(14 - floor(log2 amax)), and its inverse (2^-127 is subnormal); an all-zero row keeps 1
+    const uint32_t field = largest == 0 ? 127u : min(254u, 268u - e);
+    const float factor = __uint_as_float(field << 23);
+    if (threadIdx.x == 0) back[blockIdx.x] = __uint_as_float(field == 254 ? 0x00400000u : (254u - field) << 23);
+    uint16_t* out = prepared + static_cast<size_t>(blockIdx.x) * kTerms * k;
+    auto store = [&](const Raw8<XT>& r, uint32_t q) {
+        uint32_t t[kTerms][4];
+        r.terms(factor, t);
+#pragma unroll
+        for (uint32_t i = 0; i < kTerms; ++i) reinterpret_cast<uint4*>(out + i * k)[q] = make_uint4(t[i][0], t[i][1], t[i][2], t[i][3]);
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld; ++i)
+        if (threadIdx.x + i * kPrepareThreads < groups) store(held[i], threadIdx.x + i * kPrepareThreads);
+    for (uint32_t q = threadIdx.x + kHeld * kPrepareThreads; q < groups; q += kPrepareThreads) {
+        Raw8<XT> r;
+        r.load(row + q * 8, true);
+        store(r, q);
+    }
+}
+
+// TILES: 16-row MMA tiles of a CTA.
+// SPREAD: consecutive blocks that take an MMA column each.  Few tokens leave most of the eight columns empty, so block j of SPREAD goes
+// through column j of its token alone: the MMAs of SPREAD blocks add up in one accumulator, whose columns then get their block
+// scales in one go.  SPLIT_TERMS: the two f16 terms of f32 are columns too (up to four tokens).  Else TERMS 2: MMAs of the same weights.
+// COLS: groups of eight columns.
+template <int TILES, int SPREAD, int TERMS, bool SPLIT_TERMS, int COLS>
+__global__ void __launch_bounds__(32 * kWarps, 3) decode_mxfp4_kernel(const Params p) {
+    constexpr int kSpan = SPREAD * (SPLIT_TERMS ? 2 : 1);  // columns of a token
+    constexpr int kTokens = 8 * COLS / kSpan;
+    constexpr int kGroups = kStepBlocks / SPREAD;
+    constexpr uint32_t kRows = TILES * 16, kStage = kRows * kStepBytes;
+    static_assert(COLS == 1 || kSpan == 1, "columns are spread within one group of eight");
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* scales = smem;                                  // [rows][pitch]
+    uint8_t* ring = smem + kRows * p.pitch;                  // [warps][depth][rows][64 bytes], 16-byte pieces swizzled
+    float* sums = reinterpret_cast<float*>(ring);            // [warps][tokens][rows], once the ring is done with
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t row0 = blockIdx.x * kRows, rows = min(kRows, p.n - row0);
+    const uint32_t blocks = p.k / mx::kBlock, row_bytes = p.k / 2, steps = (p.k + 127) / 128;
     umma::griddep_launch_dependents();
 
-    // Chunk i (counted through the passes) is warp i % warps' alone, in one of that warp's own slots.  So a warp sees every filling of a
-    // slot that it waits on, and a parity can only mean the filling before or the one it waits for.  (In a ring that all warps share a
-    // warp could come to a slot a lap ahead of a copy that lands late, and take the parity of the lap before for its own.)
-    auto slot_of = [&](uint32_t i) { return i % p.warps * p.depth + i / p.warps % p.depth; };
-    auto phase_of = [&](uint32_t i) { return i / slots & 1; };
-
-    if (warp == p.warps) {
-        // ------------------------------------------------------------------ producer
-        if (lane == 0) {
-            uint32_t i = 0, pass = 0;
-            bool ok = true;
-            for (; ok && pass < p.passes; ++pass) {
-                const uint32_t row0 = (pass * gridDim.x + blockIdx.x) * p.rows;
-                if (row0 >= p.n) break;
-                const uint32_t buffer = pass & 1;
-                if (!umma::mbar_wait(&scales_empty[buffer], ((pass >> 1) & 1) ^ 1, abort_flag, p.status, umma::kTimeoutEmpty)) break;  // (pass: those begun)
-                const uint32_t bytes = min(p.rows, p.n - row0) * p.pitch;
-                umma::mbar_arrive_expect_tx(&scales_full[buffer], bytes);
-                umma::bulk_load_1d(scales + buffer * scale_bytes, p.scales + static_cast<size_t>(row0) * p.pitch, bytes, &scales_full[buffer]);
-                for (uint32_t c = 0; c < p.chunks; ++c, ++i) {
-                    const uint32_t slot = slot_of(i);
-                    if (!umma::mbar_wait(&empty[slot], phase_of(i) ^ 1, abort_flag, p.status, umma::kTimeoutEmpty)) { ok = false; break; }
-                    umma::mbar_arrive_expect_tx(&full[slot], p.rows * kChunkBytes);
-                    umma::tma_load_2d(ring + slot * slot_bytes(TILES), &map_w, &full[slot], static_cast<int32_t>(c * kChunkBytes), static_cast<int32_t>(row0));
-                }
-            }
-            // The block does not leave before its copies have landed, not even after a wait ran out: bounded too.
-            const long long start = clock64();
-            auto landed = [&](uint64_t* bar, uint32_t parity) {
-                while (!umma::mbar_try_wait(bar, parity) && clock64() - start < umma::kWaitLimitCycles) {}
-            };
-            for (uint32_t j = i > slots ? i - slots : 0; j < i; ++j) landed(&full[slot_of(j)], phase_of(j));
-            for (uint32_t j = pass > 2 ? pass - 2 : 0; j < pass; ++j) landed(&scales_full[j & 1], (j >> 1) & 1);
-        }
-        return;
+    // Scales of all steps, and the first steps of weights, before the launch in front is awaited.
+    for (uint32_t q = threadIdx.x; q < kRows * p.pitch / 16; q += 32 * kWarps) {
+        const uint32_t row = q / (p.pitch / 16);
+        copy16(umma::smem_u32(scales) + q * 16, p.scales + static_cast<size_t>(row0) * p.pitch + (row < rows ? q * 16 : 0), row < rows);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    // this lane's 16-byte pieces of a step: piece lane % 4 of rows lane / 4, + 8, ..
+    const uint8_t* w = p.w + static_cast<size_t>(row0) * row_bytes + t * 16;
+    const uint32_t mine = umma::smem_u32(ring) + warp * p.depth * kStage;
+    auto fetch = [&](uint32_t step, uint32_t slot) {
+        if (step < steps) {
+            const bool inside = step * kStepBytes + t * 16 < row_bytes;
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; r += 8) {
+                const bool live = inside && g + r < rows;
+                copy16(mine + slot * kStage + (g + r) * kStepBytes + ((t ^ swizzle(g + r)) << 4), live ? w + static_cast<size_t>(g + r) * row_bytes + step * kStepBytes : p.w, live);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");  // (a group for every turn, empty ones too)
+    };
+    for (uint32_t i = 0; i < p.depth; ++i) fetch(warp + i * kWarps, i);
 
-    // ---------------------------------------------------------------------- consumers
-    const uint32_t g = lane >> 2, t = lane & 3;
-    const uint32_t blocks = p.k / mx::kBlock;
-    const uint32_t ring_addr = umma::smem_u32(ring), scales_addr = umma::smem_u32(scales);
     umma::griddep_wait();
-    const XT* x = static_cast<const XT*>(p.x) + t * 8;
     const uint32_t sub = g % SPREAD;  // this lane's block of SPREAD
     bool live[COLS];
-    const XT* x_of[COLS];
+    const uint16_t* x[COLS];
 #pragma unroll
-    for (int n = 0; n < COLS; ++n) {
-        const uint32_t token = (n * 8 + g) / kSpan;
-        live[n] = token < p.tokens;
-        x_of[n] = x + (live[n] ? static_cast<size_t>(token) * p.k : 0) + sub * mx::kBlock;
+    for (int c = 0; c < COLS; ++c) {
+        const uint32_t column = c * 8 + g;
+        live[c] = column / kSpan < p.tokens;
+        x[c] = p.x + (live[c] ? static_cast<size_t>(TERMS == 2 ? 2 * column : column / SPREAD) * p.k : 0) + sub * mx::kBlock + t * 8;
     }
-    bool ok = true;
-    for (uint32_t pass = 0; pass < p.passes; ++pass) {
-        const uint32_t row0 = (pass * gridDim.x + blockIdx.x) * p.rows;
-        if (row0 >= p.n) break;
-        float acc[TILES][COLS][4];
+    float acc[TILES][COLS][4];
 #pragma unroll
-        for (int u = 0; u < TILES; ++u)
+    for (int u = 0; u < TILES; ++u)
 #pragma unroll
-            for (int n = 0; n < COLS; ++n)
+        for (int c = 0; c < COLS; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[u][n][i] = 0.0f;
-        float factor[COLS];  // what token g of each group is multiplied by, a power of two; 0: nothing but zeros yet
-#pragma unroll
-        for (int n = 0; n < COLS; ++n) factor[n] = 0.0f;
+            for (int i = 0; i < 4; ++i) acc[u][c][i] = 0.0f;
+    const uint32_t scale_row = umma::smem_u32(scales) + g * p.pitch;
+    wait_copies(p.depth);
+    __syncthreads();  // the scales are all warps'
 
-        // Largest finite magnitude in hand -> whether the column's factor has to change, and what the sums so far change by.
-        auto rescale = [&](int n, float amax, auto finite_amax) {
-            amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
-            if (__any_sync(kFull, factor[n] == 0.0f ? amax != 0.0f : amax * factor[n] >= 32768.0f)) {
-                if (__any_sync(kFull, amax == INFINITY)) {  // an infinity goes through as it is; the finite ones set the scale
-                    amax = finite_amax();
-                    amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
-                    amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
-                }
-                float change = 1.0f;
-                if (factor[n] == 0.0f ? amax != 0.0f : amax * factor[n] >= 32768.0f) {
-                    const float wanted = __uint_as_float(min(254u, 262u - (__float_as_uint(amax) >> 23)) << 23);  // the largest element to 2^8..2^9
-                    // (the sums so far are zero, or change by a power of two; a change too small for f32 leaves nothing of them either way)
-                    if (factor[n] != 0.0f) change = __fdiv_rn(wanted, factor[n]);
-                    factor[n] = wanted;
-                }
-                const float c0 = __shfl_sync(kFull, change, t * 8), c1 = __shfl_sync(kFull, change, t * 8 + 4);
+    uint32_t slot = 0;
+    for (uint32_t step = warp; step < steps; step += kWarps) {
+        const uint32_t block0 = step * kStepBlocks;
+        uint4 b[kGroups][COLS][TERMS];
+#pragma unroll
+        for (int s = 0; s < kGroups; ++s)
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                for (int k = 0; k < TERMS; ++k)
+                    b[s][c][k] = live[c] && block0 + s * SPREAD + sub < blocks
+                                     ? __ldg(reinterpret_cast<const uint4*>(x[c] + (block0 + s * SPREAD) * mx::kBlock + k * p.k))
+                                     : make_uint4(0, 0, 0, 0);
+        wait_copies(p.depth - 1);
+        __syncwarp();
+        const uint32_t tile = mine + slot * kStage + g * kStepBytes + t * 4;
+        static_for<kGroups>([&](auto which) {
+            constexpr int s = decltype(which)::value;
+            float d[TILES][COLS][4];
+#pragma unroll
+            for (int in = 0; in < SPREAD; ++in) {
+                const uint32_t at = ((s * SPREAD + in) ^ swizzle(g)) << 4;  // (rows 8 apart are swizzled alike)
 #pragma unroll
                 for (int u = 0; u < TILES; ++u) {
-                    acc[u][n][0] *= c0;
-                    acc[u][n][1] *= c1;
-                    acc[u][n][2] *= c0;
-                    acc[u][n][3] *= c1;
+                    uint32_t lo[4], hi[4];
+                    e2m1_f16(lds32(tile + at + u * 16 * kStepBytes), lo);
+                    e2m1_f16(lds32(tile + at + (u * 16 + 8) * kStepBytes), hi);
+#pragma unroll
+                    for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                        for (int k = 0; k < TERMS; ++k) {
+                            const bool take = SPREAD == 1 || sub == static_cast<uint32_t>(in);
+                            const uint32_t x0 = take ? b[s][c][k].x : 0u, x1 = take ? b[s][c][k].y : 0u, x2 = take ? b[s][c][k].z : 0u, x3 = take ? b[s][c][k].w : 0u;
+                            if (in == 0 && k == 0) mma_f16<true>(d[u][c], lo[0], hi[0], lo[1], hi[1], x0, x1);
+                            else mma_f16<false>(d[u][c], lo[0], hi[0], lo[1], hi[1], x0, x1);
+                            mma_f16<false>(d[u][c], lo[2], hi[2], lo[3], hi[3], x2, x3);
+                        }
                 }
             }
-            return factor[n] == 0.0f ? 1.0f : factor[n];
-        };
-        constexpr int kHeld = COLS == 1 ? kGroups : kStep;
-        Raw8<XT> raw[COLS][kHeld], later[kAhead - 1 + (kAhead == 1)][kHeld];  // (`later`: of the steps behind the next, COLS 1)
-        auto load_x = [&](uint32_t block) {
-#pragma unroll
-            for (int n = 0; n < COLS; ++n)
-#pragma unroll
-                for (int s = 0; s < kHeld; ++s) raw[n][s].load(x_of[n] + (block + s * SPREAD) * mx::kBlock, live[n] && block + s * SPREAD + sub < blocks);
-        };
-        // this warp's chunks of the pass are first, first + warps, ..; its step q lies at block_at(q) of K (behind the last at or past `blocks`)
-        const uint32_t chunk0 = pass * p.chunks, first = (warp + p.warps - chunk0 % p.warps) % p.warps;
-        auto block_at = [&](uint32_t q) { return (first + q / kSteps * p.warps) * kChunkBlocks + q % kSteps * kStepBlocks; };
-        auto load_later = [&](Raw8<XT>(&to)[kHeld], uint32_t q) {
-            const uint32_t block = block_at(q);
-#pragma unroll
-            for (int s = 0; s < kHeld; ++s) to[s].load(x_of[0] + (block + s * SPREAD) * mx::kBlock, live[0] && block + s * SPREAD + sub < blocks);
-        };
-        load_x(block_at(0));
-        if constexpr (COLS == 1) {
-#pragma unroll
-            for (int a = 0; a + 1 < kAhead; ++a) load_later(later[a], a + 1);
-        }
-        if (ok && !umma::mbar_wait(&scales_full[pass & 1], (pass >> 1) & 1, abort_flag, p.status, umma::kTimeoutFull)) ok = false;
-        const uint32_t pass_scales = scales_addr + (pass & 1) * scale_bytes + g * p.pitch;
-        for (uint32_t q = 0; ok && first + q / kSteps * p.warps < p.chunks; ++q) {
-            const uint32_t i = chunk0 + first + q / kSteps * p.warps, slot = slot_of(i);
-            const uint32_t block0 = block_at(q);
-            const uint32_t tile = ring_addr + slot * slot_bytes(TILES) + g * kChunkBytes + t * 4, half = q % kSteps * kStepBlocks;
-            auto arrive = [&] {
-                ok = __all_sync(kFull, umma::mbar_wait(&full[slot], phase_of(i), abort_flag, p.status, umma::kTimeoutFull));
-                return ok;
-            };
-            // block `in` of the step: rows of tile u as f16
-            auto weights = [&](uint32_t in, int u, uint32_t (&lo)[4], uint32_t (&hi)[4]) {
-                const uint32_t at = tile + (((half + in) ^ g) << 4);
-                e2m1_f16(lds32(at + u * 16 * kChunkBytes), lo);
-                e2m1_f16(lds32(at + (u * 16 + 8) * kChunkBytes), hi);
-            };
-            if constexpr (COLS == 1) {
-                float amax = 0.0f;
-#pragma unroll
-                for (int s = 0; s < kHeld; ++s) amax = fmaxf(amax, raw[0][s].amax());
-                const float f = rescale(0, amax, [&] {
-                    float m = 0.0f;
-#pragma unroll
-                    for (int s = 0; s < kHeld; ++s) m = fmaxf(m, raw[0][s].finite());
-                    return m;
-                });
-                uint32_t b[kHeld][kTerms][4];
-#pragma unroll
-                for (int s = 0; s < kHeld; ++s) {
-                    if constexpr (SPLIT_TERMS) {
-                        uint32_t both[2][4];
-                        raw[0][s].terms(f, both);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) b[s][0][e] = (g / SPREAD) & 1 ? both[1][e] : both[0][e];
-                    } else {
-                        raw[0][s].terms(f, b[s]);
-                    }
-                }
-                if constexpr (kAhead == 1) {
-                    load_later(raw[0], q + 1);
-                } else {
-#pragma unroll
-                    for (int s = 0; s < kHeld; ++s) raw[0][s] = later[0][s];
-#pragma unroll
-                    for (int a = 0; a + 2 < kAhead; ++a)
-#pragma unroll
-                        for (int s = 0; s < kHeld; ++s) later[a][s] = later[a + 1][s];
-                    load_later(later[kAhead - 2], q + kAhead);
-                }
-                if (!arrive()) break;
-                [[maybe_unused]] uint32_t lo4[TILES], hi4[TILES];
-                if constexpr (SPREAD == 1) {
-#pragma unroll
-                    for (int u = 0; u < TILES; ++u) {
-                        lo4[u] = lds32(pass_scales + block0 + u * 16 * p.pitch);
-                        hi4[u] = lds32(pass_scales + block0 + (u * 16 + 8) * p.pitch);
-                    }
-                }
-                static_for<kGroups>([&](auto which) {
-                    constexpr int s = decltype(which)::value;
-                    float d[TILES][4];
-#pragma unroll
-                    for (int in = 0; in < SPREAD; ++in) {
-                        uint32_t m[kTerms][4];
-#pragma unroll
-                        for (int q = 0; q < kTerms; ++q)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) m[q][e] = SPREAD == 1 || sub == static_cast<uint32_t>(in) ? b[s][q][e] : 0u;
-#pragma unroll
-                        for (int u = 0; u < TILES; ++u) {
-                            uint32_t lo[4], hi[4];
-                            weights(s * SPREAD + in, u, lo, hi);
-                            if (in == 0) mma_f16<true>(d[u], lo[0], hi[0], lo[1], hi[1], m[0][0], m[0][1]);
-                            else mma_f16<false>(d[u], lo[0], hi[0], lo[1], hi[1], m[0][0], m[0][1]);
-                            mma_f16<false>(d[u], lo[2], hi[2], lo[3], hi[3], m[0][2], m[0][3]);
-                            if constexpr (kTerms == 2) {
-                                mma_f16<false>(d[u], lo[0], hi[0], lo[1], hi[1], m[kTerms - 1][0], m[kTerms - 1][1]);
-                                mma_f16<false>(d[u], lo[2], hi[2], lo[3], hi[3], m[kTerms - 1][2], m[kTerms - 1][3]);
-                            }
-                        }
-                    }
-                    // this thread's columns 2t and 2t + 1 are neighbouring blocks of a token (or the same block of two)
-#pragma unroll
-                    for (int u = 0; u < TILES; ++u) {
-                        float lo0, lo1, hi0, hi1;
-                        if constexpr (SPREAD == 1) {
-                            lo0 = lo1 = scale_of<s>(lo4[u]);
-                            hi0 = hi1 = scale_of<s>(hi4[u]);
-                        } else {
-                            const uint32_t at = pass_scales + block0 + s * SPREAD + (2 * t) % SPREAD;
-                            const uint32_t lo2 = lds16(at + u * 16 * p.pitch), hi2 = lds16(at + (u * 16 + 8) * p.pitch);
-                            lo0 = scale_of<0>(lo2);
-                            lo1 = scale_of<1>(lo2);
-                            hi0 = scale_of<0>(hi2);
-                            hi1 = scale_of<1>(hi2);
-                        }
-                        acc[u][0][0] = fmaf(d[u][0], lo0, acc[u][0][0]);
-                        acc[u][0][1] = fmaf(d[u][1], lo1, acc[u][0][1]);
-                        acc[u][0][2] = fmaf(d[u][2], hi0, acc[u][0][2]);
-                        acc[u][0][3] = fmaf(d[u][3], hi1, acc[u][0][3]);
-                    }
-                });
-            } else {
-                uint32_t lo4[TILES], hi4[TILES];
-                static_for<kStepBlocks / kStep>([&](auto which) {
-                    constexpr int step = decltype(which)::value * kStep;
-                    if (!ok) return;
-                    // this step's x as f16, then the next step's is requested
-                    uint32_t b[kStep][COLS][kTerms][4];
-#pragma unroll
-                    for (int n = 0; n < COLS; ++n) {
-                        float amax = 0.0f;
-#pragma unroll
-                        for (int s = 0; s < kStep; ++s) amax = fmaxf(amax, raw[n][s].amax());
-                        const float f = rescale(n, amax, [&] {
-                            float m = 0.0f;
-#pragma unroll
-                            for (int s = 0; s < kStep; ++s) m = fmaxf(m, raw[n][s].finite());
-                            return m;
-                        });
-#pragma unroll
-                        for (int s = 0; s < kStep; ++s) raw[n][s].terms(f, b[s][n]);
-                    }
-                    load_x(step + kStep < static_cast<int>(kStepBlocks) ? block0 + step + kStep : block_at(q + 1));
-                    if (step == 0) {
-                        if (!arrive()) return;
-#pragma unroll
-                        for (int u = 0; u < TILES; ++u) {
-                            lo4[u] = lds32(pass_scales + block0 + u * 16 * p.pitch);
-                            hi4[u] = lds32(pass_scales + block0 + (u * 16 + 8) * p.pitch);
-                        }
-                    }
-                    static_for<kStep>([&](auto in_step) {
-                        constexpr int s = decltype(in_step)::value;
-#pragma unroll
-                        for (int u = 0; u < TILES; ++u) {
-                            uint32_t lo[4], hi[4];
-                            weights(step + s, u, lo, hi);
-                            const float s_lo = scale_of<step + s>(lo4[u]), s_hi = scale_of<step + s>(hi4[u]);
-#pragma unroll
-                            for (int n = 0; n < COLS; ++n) {
-                                float d[4];
-                                mma_f16<true>(d, lo[0], hi[0], lo[1], hi[1], b[s][n][0][0], b[s][n][0][1]);
-                                mma_f16<false>(d, lo[2], hi[2], lo[3], hi[3], b[s][n][0][2], b[s][n][0][3]);
-                                if constexpr (kTerms == 2) {
-                                    mma_f16<false>(d, lo[0], hi[0], lo[1], hi[1], b[s][n][kTerms - 1][0], b[s][n][kTerms - 1][1]);
-                                    mma_f16<false>(d, lo[2], hi[2], lo[3], hi[3], b[s][n][kTerms - 1][2], b[s][n][kTerms - 1][3]);
-                                }
-                                acc[u][n][0] = fmaf(d[0], s_lo, acc[u][n][0]);
-                                acc[u][n][1] = fmaf(d[1], s_lo, acc[u][n][1]);
-                                acc[u][n][2] = fmaf(d[2], s_hi, acc[u][n][2]);
-                                acc[u][n][3] = fmaf(d[3], s_hi, acc[u][n][3]);
-                            }
-                        }
-                    });
-                });
-                if (!ok) break;
-            }
-            __syncwarp();
-            if (ok && lane == 0 && q % kSteps == kSteps - 1) umma::mbar_arrive(&empty[slot]);
-        }
-        if (lane == 0) umma::mbar_arrive(&scales_empty[pass & 1]);
-
-        // ------------------------------------------------------------------ the warps' sums meet, eight tokens at a time
-#pragma unroll
-        for (int n = 0; n < COLS; ++n) {
-            if (n * 8 >= p.tokens * kSpan) break;
-            // (1 / factor, exact: 2^-127 is subnormal)
-            const uint32_t field = __float_as_uint(factor[n]) >> 23;
-            const float back = factor[n] == 0.0f ? 1.0f : __uint_as_float(field == 254 ? 0x00400000u : (254u - field) << 23);
-            const float b0 = __shfl_sync(kFull, back, t * 8), b1 = __shfl_sync(kFull, back, t * 8 + 4);
-            float* mine = sums + warp * kTokens * reduce_pitch(TILES);
+            // this thread's columns 2t and 2t + 1 are neighbouring blocks of a token (or the same block of two)
+            const uint32_t scale_at = scale_row + block0 + s * SPREAD + (2 * t) % SPREAD;
 #pragma unroll
             for (int u = 0; u < TILES; ++u) {
-                if constexpr (kSpan == 1) {
-                    mine[(2 * t) * reduce_pitch(TILES) + u * 16 + g] = acc[u][n][0] * b0;
-                    mine[(2 * t + 1) * reduce_pitch(TILES) + u * 16 + g] = acc[u][n][1] * b1;
-                    mine[(2 * t) * reduce_pitch(TILES) + u * 16 + g + 8] = acc[u][n][2] * b0;
-                    mine[(2 * t + 1) * reduce_pitch(TILES) + u * 16 + g + 8] = acc[u][n][3] * b1;
-                } else {  // a token's columns
-                    float lo = acc[u][n][0] * b0 + acc[u][n][1] * b1, hi = acc[u][n][2] * b0 + acc[u][n][3] * b1;
+                const uint32_t lo = SPREAD == 1 ? lds8(scale_at + u * 16 * p.pitch) : lds16(scale_at + u * 16 * p.pitch);
+                const uint32_t hi = SPREAD == 1 ? lds8(scale_at + (u * 16 + 8) * p.pitch) : lds16(scale_at + (u * 16 + 8) * p.pitch);
+                const float lo0 = scale_of<0>(lo), hi0 = scale_of<0>(hi);
+                const float lo1 = SPREAD == 1 ? lo0 : scale_of<1>(lo), hi1 = SPREAD == 1 ? hi0 : scale_of<1>(hi);
 #pragma unroll
-                    for (int o = 1; o < kSpan / 2; o *= 2) {
-                        lo += __shfl_xor_sync(kFull, lo, o);
-                        hi += __shfl_xor_sync(kFull, hi, o);
-                    }
-                    if ((2 * t) % kSpan == 0) {
-                        mine[2 * t / kSpan * reduce_pitch(TILES) + u * 16 + g] = lo;
-                        mine[2 * t / kSpan * reduce_pitch(TILES) + u * 16 + g + 8] = hi;
-                    }
+                for (int c = 0; c < COLS; ++c) {
+                    acc[u][c][0] = fmaf(d[u][c][0], lo0, acc[u][c][0]);
+                    acc[u][c][1] = fmaf(d[u][c][1], lo1, acc[u][c][1]);
+                    acc[u][c][2] = fmaf(d[u][c][2], hi0, acc[u][c][2]);
+                    acc[u][c][3] = fmaf(d[u][c][3], hi1, acc[u][c][3]);
                 }
             }
-            asm volatile("bar.sync 1, %0;" ::"r"(p.warps * 32) : "memory");
-            const uint32_t tokens = min(kTokens, p.tokens - n * 8), rows = min(p.rows, p.n - row0);
-            auto warps_sum = [&](uint32_t token, uint32_t row) {
-                float sum = 0.0f;
-                for (uint32_t w = 0; w < p.warps; ++w) sum += sums[(w * kTokens + token) * reduce_pitch(TILES) + row];
-                return sum;
-            };
-            for (uint32_t i = threadIdx.x; i < tokens * rows; i += p.warps * 32) {
-                const uint32_t token = i / rows, row = i - token * rows;
-                float sum = warps_sum(token, row);
-                if (!(fabsf(sum) < INFINITY)) {  // a NaN scale among the row's?
-                    const uint8_t* s = p.scales + static_cast<size_t>(row0 + row) * p.pitch;
-                    for (uint32_t q = 0; q < blocks; ++q)
-                        if (s[q] == mx::kNanCode) sum = NAN;
+        });
+        __syncwarp();  // the slot has been read
+        fetch(step + p.depth * kWarps, slot);
+        slot = slot + 1 == p.depth ? 0 : slot + 1;
+    }
+
+    // ---------------------------------------------------------------------- the warps' sums meet
+    wait_copies(0);
+    __syncthreads();
+    float* here = sums + warp * kTokens * reduce_pitch(TILES);
+#pragma unroll
+    for (int u = 0; u < TILES; ++u)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            if constexpr (kSpan == 1) {
+                float* to = here + (c * 8 + 2 * t) * reduce_pitch(TILES) + u * 16 + g;
+                to[0] = acc[u][c][0];
+                to[reduce_pitch(TILES)] = acc[u][c][1];
+                to[8] = acc[u][c][2];
+                to[reduce_pitch(TILES) + 8] = acc[u][c][3];
+            } else {  // a token's columns
+                float lo = acc[u][c][0] + acc[u][c][1], hi = acc[u][c][2] + acc[u][c][3];
+#pragma unroll
+                for (int o = 1; o < kSpan / 2; o *= 2) {
+                    lo += __shfl_xor_sync(kFull, lo, o);
+                    hi += __shfl_xor_sync(kFull, hi, o);
                 }
-                const size_t index = static_cast<size_t>(n * 8 + token) * p.n + row0 + row;
-                if (p.beta != 0.0f)
-                    sum = fmaf(p.beta, p.out_is_bf16 ? bf16_bits_to_float(static_cast<const uint16_t*>(p.c)[index]) : static_cast<const float*>(p.c)[index], sum);
-                if (p.out_is_bf16) static_cast<uint16_t*>(p.out)[index] = float_to_bf16_bits(sum);
-                else static_cast<float*>(p.out)[index] = sum;
+                if ((2 * t) % kSpan == 0) {
+                    here[2 * t / kSpan * reduce_pitch(TILES) + u * 16 + g] = lo;
+                    here[2 * t / kSpan * reduce_pitch(TILES) + u * 16 + g + 8] = hi;
+                }
             }
-            asm volatile("bar.sync 1, %0;" ::"r"(p.warps * 32) : "memory");
         }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < p.tokens * rows; i += 32 * kWarps) {
+        const uint32_t token = i / rows, row = i - token * rows;
+        float sum = 0.0f;
+#pragma unroll
+        for (uint32_t v = 0; v < kWarps; ++v) sum += sums[(v * kTokens + token) * reduce_pitch(TILES) + row];
+        sum *= __ldg(p.back + token);
+        if (!(fabsf(sum) < INFINITY)) {  // a NaN scale among the row's?
+            for (uint32_t k = 0; k < blocks; ++k)
+                if (scales[row * p.pitch + k] == mx::kNanCode) sum = NAN;
+        }
+        const size_t index = static_cast<size_t>(token) * p.n + row0 + row;
+        if (p.beta != 0.0f)
+            sum = fmaf(p.beta, p.out_is_bf16 ? bf16_bits_to_float(static_cast<const uint16_t*>(p.c)[index]) : static_cast<const float*>(p.c)[index], sum);
+        if (p.out_is_bf16) static_cast<uint16_t*>(p.out)[index] = float_to_bf16_bits(sum);
+        else static_cast<float*>(p.out)[index] = sum;
     }
 }
 
 struct Plan {
     uint32_t max_tokens, n, k;
-    uint32_t* status;
-    gemm::MapCache maps_w;
 };
 
-// How a call is cut: rows of a CTA and pass, MMA tiles they take, consumer warps, ring slots of a warp.
-struct Cut {
-    uint32_t rows, passes, tiles, warps, depth, smem;
-};
-inline Cut cut(uint32_t n, uint32_t k, uint32_t pitch, uint32_t tokens, uint32_t sms) {
-    const uint32_t chunks = (k + 2 * kChunkBytes - 1) / (2 * kChunkBytes);
-    Cut r{};
-    for (uint32_t most = kMaxTiles; most > 0; --most) {
-        r.passes = (n + sms * most * 16 - 1) / (sms * most * 16);
-        r.rows = (n + sms * r.passes - 1) / (sms * r.passes);
-        r.tiles = (r.rows + 15) / 16;
-        // as few warps as leave the one with most chunks no more of them
-        const uint32_t all = chunks * r.passes, rounds = (all + kMaxWarps - 1) / kMaxWarps;
-        r.warps = (all + rounds - 1) / rounds;
-        const uint32_t fixed = fixed_bytes(r.tiles, r.warps, tokens, pitch, r.passes), slot = slot_bytes(r.tiles) * r.warps;
-        if (fixed + slot > kSmemLimit) continue;  // (long rows of scales: fewer of them at a time)
-        r.depth = std::min(std::min(kMaxSlots / r.warps, rounds), (kSmemLimit - fixed) / slot);
-        r.smem = fixed + r.depth * slot;
-        return r;
-    }
-    r.depth = 0;
-    return r;
-}
-
-template <int TILES, int COLS, int SPREAD, bool SPLIT_TERMS, typename XT>
-cudaError_t launch(const CUtensorMap& map, const Params& p, uint32_t ctas, uint32_t smem, cudaStream_t stream) {
-    auto kernel = decode_mxfp4_kernel<TILES, COLS, SPREAD, SPLIT_TERMS, XT>;
+template <int TILES, int SPREAD, int TERMS, bool SPLIT_TERMS, int COLS> cudaError_t launch(Params p, cudaStream_t stream) {
+    auto kernel = decode_mxfp4_kernel<TILES, SPREAD, TERMS, SPLIT_TERMS, COLS>;
+    constexpr uint32_t kRows = TILES * 16, kStage = kRows * kStepBytes * kWarps;
+    constexpr uint32_t kSums = kWarps * (8 * COLS / (SPREAD * (SPLIT_TERMS ? 2 : 1))) * reduce_pitch(TILES) * 4;
+    const uint32_t steps = (p.k + 127) / 128, turns = (steps + kWarps - 1) / kWarps, fixed = kRows * p.pitch;
+    // three CTAs an SM while the scales leave room for two stages, else fewer
+    uint32_t limit = kSmemThird;
+    while (fixed + std::max(2 * kStage, kSums) > limit && limit < kSmemMost) limit = std::min(limit * 2, kSmemMost);
+    if (fixed + std::max(kStage, kSums) > limit) return cudaErrorInvalidValue;
+    p.depth = std::max(1u, std::min(std::min(turns, kMaxDepth), (limit - fixed) / kStage));
     static std::atomic<uint8_t> configured[gemm::kMaxDevices];
-    if (cudaError_t st = gemm::opt_in_smem(configured, kernel, kSmemLimit); st != cudaSuccess) return st;
+    if (cudaError_t st = gemm::opt_in_smem(configured, kernel, kSmemMost); st != cudaSuccess) return st;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(32 * (p.warps + 1));
-    cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3((p.n + kRows - 1) / kRows);
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.dynamicSmemBytes = fixed + std::max(p.depth * kStage, kSums);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, map, p);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
 }
-struct Call {
-    Plan& plan;
-    Params p;
-    const uint8_t* w_values;
-    cudaStream_t stream;
-};
-template <int COLS, int SPREAD, bool SPLIT_TERMS, typename XT> cudaError_t run(Call& call) {
-    Params& p = call.p;
-    const Cut how = cut(p.n, p.k, p.pitch, 8 / (SPREAD * (SPLIT_TERMS ? 2 : 1)), static_cast<uint32_t>(gemm::sm_count()));
-    if (how.depth == 0) return cudaErrorInvalidValue;
-    const CUtensorMap* map;
-    cudaError_t st = call.plan.maps_w.get(&map, call.w_values, p.n, p.k / 2, p.k / 2, how.rows);
-    if (st != cudaSuccess) return st;
-    p.rows = how.rows;
-    p.passes = how.passes;
-    p.chunks = (p.k + 2 * kChunkBytes - 1) / (2 * kChunkBytes);
-    p.depth = how.depth;
-    p.warps = how.warps;
-    const uint32_t ctas = (p.n + how.rows * how.passes - 1) / (how.rows * how.passes);
-    switch (how.tiles) {
-        case 1: return launch<1, COLS, SPREAD, SPLIT_TERMS, XT>(*map, p, ctas, how.smem, call.stream);
-        case 2: return launch<2, COLS, SPREAD, SPLIT_TERMS, XT>(*map, p, ctas, how.smem, call.stream);
-        default: return launch<3, COLS, SPREAD, SPLIT_TERMS, XT>(*map, p, ctas, how.smem, call.stream);
-    }
+template <int SPREAD, int TERMS, bool SPLIT_TERMS, int COLS> cudaError_t run(const Params& p, cudaStream_t stream) {
+    // 32 rows a CTA share an activation's registers; with fewer than two and a half such CTAs an SM, 16
+    return p.n >= 80u * static_cast<uint32_t>(gemm::sm_count()) ? launch<2, SPREAD, TERMS, SPLIT_TERMS, COLS>(p, stream)
+                                                               : launch<1, SPREAD, TERMS, SPLIT_TERMS, COLS>(p, stream);
 }
-cudaError_t run_tokens(Call& call, bool bf16) {
-    const uint32_t tokens = call.p.tokens;
-    if (bf16) {
-        if (tokens == 1) return run<1, 8, false, uint16_t>(call);
-        if (tokens == 2) return run<1, 4, false, uint16_t>(call);
-        if (tokens <= 4) return run<1, 2, false, uint16_t>(call);
-        if (tokens <= 8) return run<1, 1, false, uint16_t>(call);
-        return tokens <= 16 ? run<2, 1, false, uint16_t>(call) : run<4, 1, false, uint16_t>(call);
-    }
-    if (tokens == 1) return run<1, 4, true, float>(call);
-    if (tokens == 2) return run<1, 2, true, float>(call);
-    if (tokens <= 4) return run<1, 1, true, float>(call);
-    if (tokens <= 8) return run<1, 1, false, float>(call);
-    return tokens <= 16 ? run<2, 1, false, float>(call) : run<4, 1, false, float>(call);
+cudaError_t run_tokens(const Params& p, bool bf16, cudaStream_t stream) {
+    const uint32_t tokens = p.tokens;
+    if (bf16)
+        return tokens <= 2   ? run<4, 1, false, 1>(p, stream)
+               : tokens <= 4 ? run<2, 1, false, 1>(p, stream)
+               : tokens <= 8 ? run<1, 1, false, 1>(p, stream)
+                             : run<1, 1, false, 2>(p, stream);
+    return tokens == 1   ? run<4, 1, true, 1>(p, stream)
+           : tokens == 2 ? run<2, 1, true, 1>(p, stream)
+           : tokens <= 4 ? run<1, 1, true, 1>(p, stream)
+           : tokens <= 8 ? run<1, 2, false, 1>(p, stream)
+                         : run<1, 2, false, 2>(p, stream);
 }
+template <typename XT>
+cudaError_t prepare(const void* x, uint16_t* prepared, float* back, uint32_t tokens, uint32_t k, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tokens);
+    cfg.blockDim = dim3(kPrepareThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, prepare_mxfp4_kernel<XT>, static_cast<const XT*>(x), prepared, back, k);
+}
+size_t back_bytes(uint32_t tokens) { return (tokens * sizeof(float) + 127) / 128 * 128; }
 
 }  // namespace decode_mx
 }  // namespace eider
@@ -654,55 +478,47 @@ extern "C" {
 
 void* eider_b200_mxfp4_decode_create(uint32_t max_tokens, uint32_t out_features, uint32_t in_features) {
     if (max_tokens == 0 || max_tokens > 64 || out_features == 0 || in_features == 0 || in_features % mx::kBlock != 0 || in_features > 65536) return nullptr;
-    auto* plan = new (std::nothrow) decode_mx::Plan{max_tokens, out_features, in_features, nullptr, {}};
-    if (!plan) return nullptr;
-    if (cudaMalloc(reinterpret_cast<void**>(&plan->status), sizeof(uint32_t)) != cudaSuccess || cudaMemset(plan->status, 0, sizeof(uint32_t)) != cudaSuccess) {
-        cudaFree(plan->status);
-        delete plan;
-        return nullptr;
-    }
-    return plan;
+    return new (std::nothrow) decode_mx::Plan{max_tokens, out_features, in_features};
 }
 
-void eider_b200_mxfp4_decode_destroy(void* raw) {
-    auto* plan = static_cast<decode_mx::Plan*>(raw);
-    if (!plan) return;
-    cudaFree(plan->status);
-    delete plan;
-}
+void eider_b200_mxfp4_decode_destroy(void* raw) { delete static_cast<decode_mx::Plan*>(raw); }
 
-cudaError_t eider_b200_mxfp4_decode_status(void* raw, uint32_t* host_status) {
-    auto* plan = static_cast<decode_mx::Plan*>(raw);
-    if (!plan || !host_status) return cudaErrorInvalidValue;
-    return cudaMemcpy(host_status, plan->status, sizeof(uint32_t), cudaMemcpyDeviceToHost);
+size_t eider_b200_mxfp4_w4a16_workspace_bytes(uint32_t tokens, uint32_t in_features, int input_is_bf16) {
+    return decode_mx::back_bytes(tokens) + static_cast<size_t>(tokens) * in_features * (input_is_bf16 ? 2 : 4);
 }
 
 cudaError_t eider_b200_mxfp4_w4a16_gemv_on_stream(void* raw, const void* input, int input_is_bf16, uint32_t tokens, const uint8_t* w_values,
                                                   const uint8_t* w_scales_rows, uint32_t scale_pitch, const void* c, void* d, float beta,
-                                                  int out_is_bf16, cudaStream_t stream) {
+                                                  int out_is_bf16, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     using namespace decode_mx;
     auto* plan = static_cast<Plan*>(raw);
     if (!plan || !input || !w_values || !w_scales_rows || !d || tokens == 0 || tokens > plan->max_tokens || (beta != 0.0f && !c)) return cudaErrorInvalidValue;
     if (((reinterpret_cast<uintptr_t>(input) | reinterpret_cast<uintptr_t>(w_values) | reinterpret_cast<uintptr_t>(w_scales_rows)) & 15) != 0 ||
-        scale_pitch % 16 != 0 || scale_pitch < (plan->k / mx::kBlock + 7) / 8 * 8)
+        !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
+        workspace_bytes < eider_b200_mxfp4_w4a16_workspace_bytes(tokens, plan->k, input_is_bf16) || scale_pitch % 16 != 0 || scale_pitch < (plan->k / mx::kBlock + 7) / 8 * 8)
         return cudaErrorInvalidValue;
-    const uint32_t groups = (tokens + 31) / 32, each = (tokens + groups - 1) / groups;
+    float* back = static_cast<float*>(workspace);
+    uint16_t* prepared = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + back_bytes(tokens));
+    cudaError_t st = input_is_bf16 ? prepare<uint16_t>(input, prepared, back, tokens, plan->k, stream)
+                                   : prepare<float>(input, prepared, back, tokens, plan->k, stream);
+    if (st != cudaSuccess) return st;
+    const uint32_t groups = (tokens + 15) / 16, each = (tokens + groups - 1) / groups;
     for (uint32_t first = 0; first < tokens; first += each) {
-        Call call{*plan, {}, w_values, stream};
-        Params& p = call.p;
+        const size_t out_bytes = out_is_bf16 ? 2 : 4;
+        Params p{};
         p.tokens = std::min(each, tokens - first);
-        const size_t x_bytes = input_is_bf16 ? 2 : 4, out_bytes = out_is_bf16 ? 2 : 4;
-        p.x = static_cast<const uint8_t*>(input) + first * x_bytes * plan->k;
+        p.x = prepared + static_cast<size_t>(first) * (input_is_bf16 ? 1 : 2) * plan->k;
+        p.back = back + first;
+        p.w = w_values;
         p.scales = w_scales_rows;
         p.out = static_cast<uint8_t*>(d) + first * out_bytes * plan->n;
         p.c = c ? static_cast<const uint8_t*>(c) + first * out_bytes * plan->n : nullptr;
-        p.status = plan->status;
         p.beta = beta;
         p.out_is_bf16 = out_is_bf16;
         p.n = plan->n;
         p.k = plan->k;
         p.pitch = scale_pitch;
-        const cudaError_t st = run_tokens(call, input_is_bf16);
+        st = run_tokens(p, input_is_bf16, stream);
         if (st != cudaSuccess) return st;
     }
     return cudaSuccess;

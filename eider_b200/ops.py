@@ -631,15 +631,13 @@ class Mxfp4DecodePlan(_DevicePlan):
         x = _aligned16(x)
         _need_device(self.device, x, w.packed)
         out, c = self._output(out, (x.shape[0], self.n), out_dtype, beta, c)
-        _call(self.device, "eider_b200_mxfp4_w4a16_gemv_on_stream", self._plan, x.data_ptr(), int(x.dtype == torch.bfloat16), x.shape[0],
-              w.packed.data_ptr(), w.scales_rows.data_ptr(), w.scales_rows.shape[1], _ptr(c), out.data_ptr(), beta,
-              int(out.dtype == torch.bfloat16))
+        tokens, bf16 = x.shape[0], int(x.dtype == torch.bfloat16)
+        size = (tokens * 4 + 127) // 128 * 128 + tokens * self.k * (2 if bf16 else 4)  # eider_b200_mxfp4_w4a16_workspace_bytes
+        workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
+        _call(self.device, "eider_b200_mxfp4_w4a16_gemv_on_stream", self._plan, x.data_ptr(), bf16, tokens, w.packed.data_ptr(),
+              w.scales_rows.data_ptr(), w.scales_rows.shape[1], _ptr(c), out.data_ptr(), beta, int(out.dtype == torch.bfloat16),
+              workspace.data_ptr(), size)
         return out
-
-    def status(self) -> int:
-        v = C.c_uint32(0)
-        check("eider_b200_mxfp4_decode_status", self._lib.eider_b200_mxfp4_decode_status(self._plan, C.byref(v)))
-        return v.value
 
 
 # ---- FP8 quantizers ---------------------------------------------------------------------------------

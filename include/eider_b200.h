@@ -854,14 +854,15 @@ EIDER_B200_API cudaError_t eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream(void
 
 /* W4A16 product for 1 to 64 tokens, D[t][n] = X . W^T + beta * C, X f32 or bf16 [tokens][in_features], D and C f32 or bf16.  The
  * scales are rows of `scale_pitch` bytes (a multiple of 16, at least in_features / 32 rounded up to 8) with zeros behind the
- * blocks.  X, weights and scales 16-byte aligned.  A plan keeps nothing between calls but the status word: calls on several
- * streams may overlap. */
+ * blocks.  X, weights, scales and workspace 16-byte aligned.  The workspace is one call's, and a plan keeps nothing between
+ * calls: calls on several streams may overlap. */
 EIDER_B200_API void* eider_b200_mxfp4_decode_create(uint32_t max_tokens, uint32_t out_features, uint32_t in_features);
 EIDER_B200_API void eider_b200_mxfp4_decode_destroy(void* plan);
-EIDER_B200_API cudaError_t eider_b200_mxfp4_decode_status(void* plan, uint32_t* host_status);
+EIDER_B200_API size_t eider_b200_mxfp4_w4a16_workspace_bytes(uint32_t tokens, uint32_t in_features, int input_is_bf16);
 EIDER_B200_API cudaError_t eider_b200_mxfp4_w4a16_gemv_on_stream(void* plan, const void* input, int input_is_bf16, uint32_t tokens,
                                                                  const uint8_t* w_values, const uint8_t* w_scales_rows, uint32_t scale_pitch,
-                                                                 const void* c, void* d, float beta, int out_is_bf16, cudaStream_t stream);
+                                                                 const void* c, void* d, float beta, int out_is_bf16, void* workspace,
+                                                                 size_t workspace_bytes, cudaStream_t stream);
 
 /* Routed experts.  Rows are expert-major as for NVFP4: the scales of expert e start at ((offset[e] + 127) / 128 + e) tiles of
  * scale_tile_bytes = 128 * (in_features / 32 rounded up to 4).  The route quantizer writes every route's row and scales; the padding

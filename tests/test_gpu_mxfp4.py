@@ -227,7 +227,6 @@ def test_decode(tokens, dtype):
         c = randn(g, tokens, n)
         y = plan.run(x, w, beta=0.25, c=c, out_dtype=torch.float32)
         assert ((y.double() - want - 0.25 * c.double()).abs() <= bound + 2.0 ** -22 * (want.abs() + c.double().abs())).all()
-        assert plan.status() == 0
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
