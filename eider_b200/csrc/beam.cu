@@ -43,8 +43,9 @@ struct BeamArgs {
     uint32_t beams, vocab, k, pad_token, segments, splits, vectors_per_split;
 };
 
+// (What earlier launches wrote is not read with __ldg: to the compiler a read-only load has no order with griddepcontrol.wait.)
 __device__ __forceinline__ bool row_counts(const BeamArgs& a, uint32_t row) {
-    return isfinite(__ldg(a.beam_scores + row)) && !(a.finished && __ldg(a.finished + row));
+    return isfinite(__ldcg(a.beam_scores + row)) && !(a.finished && __ldcg(a.finished + row));
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -96,18 +97,18 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const BeamArgs 
         const uint4* vectors = reinterpret_cast<const uint4*>(logits - lead) + base + threadIdx.x;
         if (inside) {
 #pragma unroll
-            for (uint32_t j = 0; j < kAhead; ++j) next[j] = __ldg(vectors + j * kScanThreads);
+            for (uint32_t j = 0; j < kAhead; ++j) next[j] = __ldcg(vectors + j * kScanThreads);
             return;
         }
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
             const uint32_t vec = base + j * kScanThreads + threadIdx.x, at = vec * E;
             if (vec < v1 && at >= lead && at + E <= end) {
-                next[j] = __ldg(vectors + j * kScanThreads);
+                next[j] = __ldcg(vectors + j * kScanThreads);
             } else {  // the row's first and last vectors, and none
                 T v[E];
 #pragma unroll
-                for (uint32_t e = 0; e < E; ++e) v[e] = vec < v1 && at + e >= lead && at + e < end ? __ldg(logits + (at + e - lead)) : minus_infinity<T>();
+                for (uint32_t e = 0; e < E; ++e) v[e] = vec < v1 && at + e >= lead && at + e < end ? __ldcg(logits + (at + e - lead)) : minus_infinity<T>();
                 memcpy(&next[j], v, 16);
             }
         }
@@ -286,19 +287,19 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
     // the sum of exponentials of every row from its splits, in 64 bits
     for (uint32_t w = warp; w < a.beams; w += kMergeThreads / 32) {
         const uint32_t row = row0 + w;
-        const bool ended = a.finished && __ldg(a.finished + row) && isfinite(__ldg(a.beam_scores + row));
+        const bool ended = a.finished && __ldcg(a.finished + row) && isfinite(__ldcg(a.beam_scores + row));
         bool counts = row_counts(a, row);
-        double base = __ldg(a.beam_scores + row);
+        double base = __ldcg(a.beam_scores + row);
         float top = 0.0f;
         if (counts) {
             const float2* partial = a.partial + static_cast<size_t>(row) * a.splits;
             top = -INFINITY;
-            for (uint32_t s = lane; s < a.splits; s += 32) top = fmaxf(top, partial[s].x);
+            for (uint32_t s = lane; s < a.splits; s += 32) top = fmaxf(top, __ldcg(partial + s).x);
 #pragma unroll
             for (uint32_t o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
             double sum = 0.0;
             for (uint32_t s = lane; s < a.splits; s += 32) {
-                const float2 p = partial[s];
+                const float2 p = __ldcg(partial + s);
                 if (p.y != 0.0f) sum += p.y * exp(static_cast<double>(p.x) - top);
             }
 #pragma unroll
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             for (uint32_t s = part * per_part + lane; s < last; s += 32 * kFetch) {
                 float x[kFetch];
 #pragma unroll
-                for (uint32_t i = 0; i < kFetch; ++i) x[i] = s + 32 * i < last ? maxima[static_cast<size_t>(w) * a.segments + s + 32 * i] : -INFINITY;
+                for (uint32_t i = 0; i < kFetch; ++i) x[i] = s + 32 * i < last ? __ldcg(maxima + static_cast<size_t>(w) * a.segments + s + 32 * i) : -INFINITY;
 #pragma unroll
                 for (uint32_t i = 0; i < kFetch; ++i) use(Candidate{(x[i] - top) + base, w * a.segments + s + 32 * i});
             }
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
             const T* logits = static_cast<const T*>(a.logits) + (row0 + w) * a.stride;
             const uint32_t position = s * kSegment + j % kSegment, lead = row_lead(logits);
             if (position >= lead && position - lead < a.vocab)
-                use(Candidate{(logit_value(__ldg(logits + (position - lead))) - sh.top[w]) + sh.base[w], w * a.vocab + (position - lead)});
+                use(Candidate{(logit_value(__ldcg(logits + (position - lead))) - sh.top[w]) + sh.base[w], w * a.vocab + (position - lead)});
         }
     });
     for (uint32_t r = threadIdx.x; r < a.k; r += kMergeThreads) {
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(kCopyThreads) beam_reorder_kernel(const Reorde
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t row = blockIdx.x, batch = row / a.beams, beam = row - batch * a.beams;
     const size_t bytes = a.row_bytes[blockIdx.z];
-    const int32_t parent = __ldg(a.parents + batch * a.parent_stride + beam);
+    const int32_t parent = __ldcg(a.parents + batch * a.parent_stride + beam);
     if (parent < 0 || static_cast<uint32_t>(parent) >= a.beams) return;  // (no such beam: the row stays as it is)
     const uint8_t* src = a.src[blockIdx.z] + (static_cast<size_t>(batch) * a.beams + parent) * bytes;
     uint8_t* dst = a.dst[blockIdx.z] + static_cast<size_t>(row) * bytes;
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(kCopyThreads) beam_reorder_kernel(const Reorde
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
                 const size_t o = (j * kCopyThreads + threadIdx.x) * 16;
-                if (o + 16 <= left) q[j] = __ldg(reinterpret_cast<const uint4*>(src + at + o));
+                if (o + 16 <= left) q[j] = __ldcg(reinterpret_cast<const uint4*>(src + at + o));
             }
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(kCopyThreads) beam_reorder_kernel(const Reorde
             }
             done = left / 16 * 16;
         }
-        for (size_t o = done + threadIdx.x; o < left && o < kStretch; o += kCopyThreads) dst[at + o] = __ldg(src + at + o);
+        for (size_t o = done + threadIdx.x; o < left && o < kStretch; o += kCopyThreads) dst[at + o] = __ldcg(src + at + o);
     }
 }
 

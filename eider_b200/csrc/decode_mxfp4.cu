@@ -26,7 +26,9 @@ namespace decode_mx {
 constexpr uint32_t kWarps = 8;
 constexpr uint32_t kStepBytes = 64, kStepBlocks = 4;  // of a row: 128 elements
 constexpr uint32_t kMaxDepth = 8;                     // steps a warp has on their way
-constexpr uint32_t kSmemThird = 75 * 1024, kSmemMost = 227 * 1024;
+constexpr uint32_t kSmemMost = 227 * 1024;
+// Three CTAs an SM (80 registers), two (128) where the activations of a step take 64 of them.
+__host__ __device__ constexpr uint32_t ctas_per_sm(int operands) { return operands > 2 ? 2 : 3; }
 constexpr uint32_t kFull = 0xffffffffu;
 
 struct Params {
@@ -124,11 +126,13 @@ __device__ __forceinline__ uint32_t lds16(uint32_t address) {
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(address));
     return v;
 }
+// (Activations are read with __ldca or __ldcg: to the compiler __ldg has no order with griddepcontrol.wait, and it requested what the launch in
+// front had not written yet: 264 of 3200 calls came out wrong.)
 // Eight consecutive elements of a token, their largest finite magnitude, and f16 terms of x * factor.
 template <typename T> struct Raw8;
 template <> struct Raw8<uint16_t> {
     uint4 q;
-    __device__ __forceinline__ void load(const uint16_t* p, bool live) { q = live ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void load(const uint16_t* p, bool live) { q = live ? __ldcg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w; }
     static __device__ __forceinline__ __nv_bfloat162 pair(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
     __device__ __forceinline__ void values(float (&v)[8]) const {
@@ -159,8 +163,8 @@ template <> struct Raw8<uint16_t> {
 template <> struct Raw8<float> {
     float4 a, b;
     __device__ __forceinline__ void load(const float* p, bool live) {
-        a = live ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
-        b = live ? __ldg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
+        a = live ? __ldcg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
+        b = live ? __ldcg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
     }
     __device__ __forceinline__ void values(float (&v)[8]) const {
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_mxfp4_kernel(const XT
 // scales in one go.  SPLIT_TERMS: the two f16 terms of f32 are columns too (up to four tokens).  Else TERMS 2: MMAs of the same weights.
 // COLS: groups of eight columns.
 template <int TILES, int SPREAD, int TERMS, bool SPLIT_TERMS, int COLS>
-__global__ void __launch_bounds__(32 * kWarps, 3) decode_mxfp4_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode_mxfp4_kernel(const Params p) {
     constexpr int kSpan = SPREAD * (SPLIT_TERMS ? 2 : 1);  // columns of a token
     constexpr int kTokens = 8 * COLS / kSpan;
     constexpr int kGroups = kStepBlocks / SPREAD;
@@ -298,22 +302,32 @@ __global__ void __launch_bounds__(32 * kWarps, 3) decode_mxfp4_kernel(const Para
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[u][c][i] = 0.0f;
     const uint32_t scale_row = umma::smem_u32(scales) + g * p.pitch;
+
+    // x of a step's group of blocks; a group's registers are refilled for the warp's next step as soon as its MMAs are out, unless
+    // they are so many that this spills (5 float32 tokens, K 4064 -> N 6150: 13.7 us with two CTAs an SM, requested at the step's begin 10.2 with three)
+    constexpr bool kRefill = COLS * TERMS == 1;
+    uint4 b[kGroups][COLS][TERMS];
+    auto load_x = [&](uint4(&to)[COLS][TERMS], uint32_t block) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k)
+                to[c][k] = live[c] && block + sub < blocks ? __ldca(reinterpret_cast<const uint4*>(x[c] + block * mx::kBlock + k * p.k)) : make_uint4(0, 0, 0, 0);
+    };
+    if constexpr (kRefill) {
+#pragma unroll
+        for (int s = 0; s < kGroups; ++s) load_x(b[s], warp * kStepBlocks + s * SPREAD);
+    }
+
     wait_copies(p.depth);
     __syncthreads();  // the scales are all warps'
-
     uint32_t slot = 0;
     for (uint32_t step = warp; step < steps; step += kWarps) {
         const uint32_t block0 = step * kStepBlocks;
-        uint4 b[kGroups][COLS][TERMS];
+        if constexpr (!kRefill) {
 #pragma unroll
-        for (int s = 0; s < kGroups; ++s)
-#pragma unroll
-            for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                for (int k = 0; k < TERMS; ++k)
-                    b[s][c][k] = live[c] && block0 + s * SPREAD + sub < blocks
-                                     ? __ldg(reinterpret_cast<const uint4*>(x[c] + (block0 + s * SPREAD) * mx::kBlock + k * p.k))
-                                     : make_uint4(0, 0, 0, 0);
+            for (int s = 0; s < kGroups; ++s) load_x(b[s], block0 + s * SPREAD);
+        }
         wait_copies(p.depth - 1);
         __syncwarp();
         const uint32_t tile = mine + slot * kStage + g * kStepBytes + t * 4;
@@ -340,6 +354,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) decode_mxfp4_kernel(const Para
                         }
                 }
             }
+            if constexpr (kRefill) load_x(b[s], block0 + kWarps * kStepBlocks + s * SPREAD);
             // this thread's columns 2t and 2t + 1 are neighbouring blocks of a token (or the same block of two)
             const uint32_t scale_at = scale_row + block0 + s * SPREAD + (2 * t) % SPREAD;
 #pragma unroll
@@ -395,7 +410,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) decode_mxfp4_kernel(const Para
         float sum = 0.0f;
 #pragma unroll
         for (uint32_t v = 0; v < kWarps; ++v) sum += sums[(v * kTokens + token) * reduce_pitch(TILES) + row];
-        sum *= __ldg(p.back + token);
+        sum *= __ldcg(p.back + token);
         if (!(fabsf(sum) < INFINITY)) {  // a NaN scale among the row's?
             for (uint32_t k = 0; k < blocks; ++k)
                 if (scales[row * p.pitch + k] == mx::kNanCode) sum = NAN;
@@ -417,8 +432,8 @@ template <int TILES, int SPREAD, int TERMS, bool SPLIT_TERMS, int COLS> cudaErro
     constexpr uint32_t kRows = TILES * 16, kStage = kRows * kStepBytes * kWarps;
     constexpr uint32_t kSums = kWarps * (8 * COLS / (SPREAD * (SPLIT_TERMS ? 2 : 1))) * reduce_pitch(TILES) * 4;
     const uint32_t steps = (p.k + 127) / 128, turns = (steps + kWarps - 1) / kWarps, fixed = kRows * p.pitch;
-    // three CTAs an SM while the scales leave room for two stages, else fewer
-    uint32_t limit = kSmemThird;
+    // as many CTAs an SM as the registers allow while the scales leave room for two stages, else fewer
+    uint32_t limit = kSmemMost / ctas_per_sm(TERMS * COLS) - 1024;
     while (fixed + std::max(2 * kStage, kSums) > limit && limit < kSmemMost) limit = std::min(limit * 2, kSmemMost);
     if (fixed + std::max(kStage, kSums) > limit) return cudaErrorInvalidValue;
     p.depth = std::max(1u, std::min(std::min(turns, kMaxDepth), (limit - fixed) / kStage));

@@ -17,7 +17,8 @@ namespace {
 constexpr uint32_t kFull = 0xffffffffu;
 
 // The kernels of the routed layer run one behind the other on small data: each is launched as a programmatic dependent, waits
-// here for the one before it (what it wrote is then visible) and lets the next one be launched.
+// here for the one before it (what it wrote is then visible) and lets the next one be launched.  What it wrote is read with __ldca, not
+// __ldg: to the compiler a read-only load has no order with the wait, and it may request the old value in front of it.
 __device__ __forceinline__ void griddep_begin() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -48,7 +49,7 @@ __global__ void __launch_bounds__(128) moe_topk_kernel(const float* __restrict__
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) {
         const uint32_t e = lane + i * 32;
-        v[i] = e < experts ? sanitize_logit(__ldg(lg + e)) : -INFINITY;
+        v[i] = e < experts ? sanitize_logit(__ldca(lg + e)) : -INFINITY;
         mx = fmaxf(mx, v[i]);
     }
 #pragma unroll
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kSortChunk) moe_chunk_hist_kernel(const uint32
     __syncthreads();
     const uint32_t r = blockIdx.x * kSortChunk + threadIdx.x;
     if (r < routes) {
-        const uint32_t e = __ldg(indices + r);
+        const uint32_t e = __ldca(indices + r);
         if (e < experts) atomicAdd(&hist[e], 1u);
     }
     __syncthreads();
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(kSortChunk) moe_scatter_kernel(const uint32_t*
     __syncthreads();
     const uint32_t r = blockIdx.x * kSortChunk + threadIdx.x;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t e = r < routes ? __ldg(indices + r) : 0xffffffffu;
+    const uint32_t e = r < routes ? __ldca(indices + r) : 0xffffffffu;
     const bool valid = e < experts;
     const uint32_t peers = __match_any_sync(kFull, valid ? e : 0xffffffffu);
     const uint32_t rank = __popc(peers & ((1u << lane) - 1));
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kSortChunk) moe_scatter_kernel(const uint32_t*
     if (!valid) return;
     uint32_t before = 0;
     for (uint32_t w = 0; w < warp; ++w) before += wcount[w * experts + e];
-    const uint32_t sorted = offsets[e] + chunk_base[static_cast<size_t>(blockIdx.x) * experts + e] + before + rank;
+    const uint32_t sorted = __ldca(offsets + e) + __ldca(chunk_base + static_cast<size_t>(blockIdx.x) * experts + e) + before + rank;
     sorted_routes[sorted] = r;
     sorted_experts[sorted] = e;
     route_to_sorted[r] = sorted;
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(1024) moe_sort_one_cta_kernel(const uint32_t* 
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
         const uint32_t r = j * 1024 + threadIdx.x;
-        e[j] = r < routes ? __ldg(indices + r) : 0xffffffffu;
+        e[j] = r < routes ? __ldca(indices + r) : 0xffffffffu;
     }
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
@@ -356,11 +357,11 @@ __global__ void __launch_bounds__(kScatterWarps * 32) moe_scatter_rows_kernel(co
     if (row_bytes % 16 == 0 && ((reinterpret_cast<uintptr_t>(src_packed) | reinterpret_cast<uintptr_t>(packed)) & 15) == 0) {
         const uint4* s4 = reinterpret_cast<const uint4*>(s1);
         uint4* d4 = reinterpret_cast<uint4*>(d1);
-        for (uint32_t i = lane; i < row_bytes / 16; i += 32) d4[i] = __ldg(s4 + i);
+        for (uint32_t i = lane; i < row_bytes / 16; i += 32) d4[i] = __ldca(s4 + i);
     } else {  // rows that do not start on 16-byte boundaries (K % 32 != 0): 8-byte words, K % 16 == 0 guarantees those
         const uint2* s2 = reinterpret_cast<const uint2*>(s1);
         uint2* d2 = reinterpret_cast<uint2*>(d1);
-        for (uint32_t i = lane; i < row_bytes / 8; i += 32) d2[i] = __ldg(s2 + i);
+        for (uint32_t i = lane; i < row_bytes / 8; i += 32) d2[i] = __ldca(s2 + i);
     }
     const size_t base = moe_scale_base(expert, offsets, tile_bytes);
     const uint32_t blocks = k / 16;
@@ -368,9 +369,9 @@ __global__ void __launch_bounds__(kScatterWarps * 32) moe_scatter_rows_kernel(co
     const uint32_t words = aligned4 ? blocks / 4 : 0;  // whole groups of four blocks
     for (uint32_t w = lane; w < words; w += 32)
         *reinterpret_cast<uint32_t*>(scales + base + tiled_scale_offset(col, w * 4, k)) =
-            __ldg(reinterpret_cast<const uint32_t*>(src_scales + tiled_scale_offset(src_row, w * 4, k)));
+            __ldca(reinterpret_cast<const uint32_t*>(src_scales + tiled_scale_offset(src_row, w * 4, k)));
     for (uint32_t b = words * 4 + lane; b < blocks; b += 32)
-        scales[base + tiled_scale_offset(col, b, k)] = __ldg(src_scales + tiled_scale_offset(src_row, b, k));
+        scales[base + tiled_scale_offset(col, b, k)] = __ldca(src_scales + tiled_scale_offset(src_row, b, k));
 }
 
 // Quantize a token's row once and write it to all of its routes (first and second half of non_gemm.cu:2899-2998 in one): one
@@ -396,12 +397,12 @@ __global__ void __launch_bounds__(1024) moe_quantize_routes_kernel(const T* __re
     if (b < blocks) v.load(input + static_cast<size_t>(token) * k + b * 16);
     const uint32_t slot0 = blockIdx.y * slots_per_cta, slots = min(slots_per_cta, routes_per_row - slot0);
     if (threadIdx.x < slots) {
-        const uint32_t route = token * routes_per_row + slot0 + threadIdx.x, sorted = __ldg(route_to_sorted + route);
+        const uint32_t route = token * routes_per_row + slot0 + threadIdx.x, sorted = __ldca(route_to_sorted + route);
         size_t row = ~static_cast<size_t>(0), scale = 0;
-        if (sorted < routes && __ldg(sorted_routes + sorted) == route) {  // (a route to an expert that does not exist has no place)
-            const uint32_t expert = __ldg(sorted_experts + sorted);
+        if (sorted < routes && __ldca(sorted_routes + sorted) == route) {  // (a route to an expert that does not exist has no place)
+            const uint32_t expert = __ldca(sorted_experts + sorted);
             row = static_cast<size_t>(sorted) * (k / 2);
-            scale = moe_scale_base(expert, offsets, tile_bytes) + tiled_scale_offset(sorted - __ldg(offsets + expert), 0, k);
+            scale = moe_scale_base(expert, offsets, tile_bytes) + tiled_scale_offset(sorted - __ldca(offsets + expert), 0, k);
         }
         row_at[threadIdx.x] = row;
         scale_at[threadIdx.x] = scale;
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(256) moe_silu_mul_quantize_kernel(const uint16
     const uint32_t halves = k / 8;
     const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     // (routes_limit: optional device-resident row count below the launch's capacity, for buffers filled by other ranks)
-    const bool live = unit < static_cast<uint64_t>(routes) * halves && (!routes_limit || unit / halves < __ldg(routes_limit));
+    const bool live = unit < static_cast<uint64_t>(routes) * halves && (!routes_limit || unit / halves < __ldca(routes_limit));
     const uint32_t sorted = live ? static_cast<uint32_t>(unit / halves) : 0;
     const uint32_t h = live ? static_cast<uint32_t>(unit % halves) : 0;
     float v[8];
@@ -456,8 +457,8 @@ __global__ void __launch_bounds__(256) moe_silu_mul_quantize_kernel(const uint16
     if (live) {
         const uint16_t* gate = gate_up + static_cast<size_t>(sorted) * k * 2;
         const uint16_t* up = gate + k;
-        const uint4 g4 = __ldg(reinterpret_cast<const uint4*>(gate + h * 8));
-        const uint4 u4 = __ldg(reinterpret_cast<const uint4*>(up + h * 8));
+        const uint4 g4 = __ldca(reinterpret_cast<const uint4*>(gate + h * 8));
+        const uint4 u4 = __ldca(reinterpret_cast<const uint4*>(up + h * 8));
         const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -510,34 +511,34 @@ __global__ void __launch_bounds__(256) moe_quantize_sorted_kernel(const void* __
     const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (unit >= static_cast<uint64_t>(routes) * blocks) return;
     const uint32_t sorted = static_cast<uint32_t>(unit / blocks), b = static_cast<uint32_t>(unit % blocks);
-    const uint32_t expert = __ldg(sorted_experts + sorted);
+    const uint32_t expert = __ldca(sorted_experts + sorted);
     float v[16];
     if (MODE == kPlain || MODE == kCalibrated) {
-        const uint32_t src_row = gather_rows ? __ldg(sorted_routes + sorted) / routes_per_row : sorted;
+        const uint32_t src_row = gather_rows ? __ldca(sorted_routes + sorted) / routes_per_row : sorted;
         const float* src = static_cast<const float*>(input) + static_cast<size_t>(src_row) * k + b * 16;
-        const float inverse = MODE == kCalibrated ? __frcp_rn(__ldg(input_scales + expert)) : 1.0f;
+        const float inverse = MODE == kCalibrated ? __frcp_rn(__ldca(input_scales + expert)) : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = MODE == kCalibrated ? __fmul_rn(__ldg(src + i), inverse) : __ldg(src + i);
+        for (int i = 0; i < 16; ++i) v[i] = MODE == kCalibrated ? __fmul_rn(__ldca(src + i), inverse) : __ldca(src + i);
     } else {
         const uint16_t* src = static_cast<const uint16_t*>(input) + static_cast<size_t>(sorted) * k + b * 16;
         if (MODE == kReluSquared) {
-            const float inverse = __frcp_rn(__ldg(input_scales + expert));
+            const float inverse = __frcp_rn(__ldca(input_scales + expert));
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float x = fmaxf(bf16_bits_to_float(__ldg(src + i)), 0.0f);
+                const float x = fmaxf(bf16_bits_to_float(__ldca(src + i)), 0.0f);
                 v[i] = __fmul_rn(__fmul_rn(x, x), inverse);
             }
         } else {
             const uint16_t* up = static_cast<const uint16_t*>(input2) + static_cast<size_t>(sorted) * k + b * 16;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = rowops::gelu_tanh_mul(bf16_bits_to_float(__ldg(src + i)), bf16_bits_to_float(__ldg(up + i)));
+            for (int i = 0; i < 16; ++i) v[i] = rowops::gelu_tanh_mul(bf16_bits_to_float(__ldca(src + i)), bf16_bits_to_float(__ldca(up + i)));
         }
     }
     uint2 bytes;
     const uint8_t sc = quantize_block16(v, 16, &bytes);
     uint8_t* dst = packed + static_cast<size_t>(sorted) * (k / 2) + b * 8;  // 8-byte aligned when `packed` is (k % 16 == 0)
     *reinterpret_cast<uint2*>(dst) = bytes;
-    scales[moe_scale_base(expert, offsets, tile_bytes) + tiled_scale_offset(sorted - __ldg(offsets + expert), b, k)] = sc;
+    scales[moe_scale_base(expert, offsets, tile_bytes) + tiled_scale_offset(sorted - __ldca(offsets + expert), b, k)] = sc;
 }
 
 // non_gemm.cu:3066-3083
@@ -577,8 +578,8 @@ moe_combine_kernel(const uint32_t* __restrict__ route_to_sorted, const float* __
 #pragma unroll
         for (uint32_t s = 0; s < AHEAD; ++s) {
             const uint32_t route = row * routes_per_row + slot0 + s;
-            w[s] = __ldg(route_weights + route);
-            q[s] = __ldg(reinterpret_cast<const uint4*>(sorted_inputs + static_cast<size_t>(__ldg(route_to_sorted + route)) * len) + v);
+            w[s] = __ldca(route_weights + route);
+            q[s] = __ldca(reinterpret_cast<const uint4*>(sorted_inputs + static_cast<size_t>(__ldca(route_to_sorted + route)) * len) + v);
         }
 #pragma unroll
         for (uint32_t s = 0; s < AHEAD; ++s) {
@@ -617,8 +618,8 @@ __global__ void __launch_bounds__(256) moe_combine_scalar_kernel(const uint32_t*
     float sum = 0.0f;
     for (uint32_t slot = 0; slot < routes_per_row; ++slot) {
         const uint32_t route = row * routes_per_row + slot;
-        sum = fmaf(bf16_bits_to_float(sorted_inputs[static_cast<size_t>(route_to_sorted[route]) * len + col]),
-                   route_weights[route], sum);
+        sum = fmaf(bf16_bits_to_float(__ldca(sorted_inputs + static_cast<size_t>(__ldca(route_to_sorted + route)) * len + col)),
+                   __ldca(route_weights + route), sum);
     }
     if constexpr (sizeof(T) == 4) output[idx] = sum;
     else output[idx] = float_to_bf16_bits(sum);

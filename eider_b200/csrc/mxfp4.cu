@@ -17,19 +17,20 @@ namespace {
 constexpr uint32_t kFullMask = 0xffffffffu;
 constexpr uint32_t kUnit = 128;
 
-// Eight elements at p, from aligned rows in 16-byte loads.
+// Eight elements at p, from aligned rows in 16-byte loads.  (Never with __ldg: to the compiler a read-only load has no order with
+// griddepcontrol.wait.)
 template <bool VEC> __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
     if (VEC) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __ldg(p + i);
+        for (int i = 0; i < 8; ++i) v[i] = __ldcg(p + i);
     }
 }
 template <bool VEC> __device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) {
     if (VEC) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p));
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -38,7 +39,7 @@ template <bool VEC> __device__ __forceinline__ void load8(const uint16_t* p, flo
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = bf16_bits_to_float(__ldg(p + i));
+        for (int i = 0; i < 8; ++i) v[i] = bf16_bits_to_float(__ldcg(p + i));
     }
 }
 
@@ -187,8 +188,8 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_mxfp4_kernel(const u
             live[a] = unit < units && k[a] < inner;
             words[a] = codes[a] = 0;
             if (live[a]) {
-                words[a] = __ldg(reinterpret_cast<const uint32_t*>(packed + static_cast<size_t>(row[a]) * (inner / 2)) + k[a] / 8);
-                codes[a] = __ldg(scales + (static_cast<size_t>(row[a] / 128) * padded_blocks + u * 4) * 128 + (row[a] % 32) * 16 + (row[a] / 32 % 4) * 4 +
+                words[a] = __ldcg(reinterpret_cast<const uint32_t*>(packed + static_cast<size_t>(row[a]) * (inner / 2)) + k[a] / 8);
+                codes[a] = __ldcg(scales + (static_cast<size_t>(row[a] / 128) * padded_blocks + u * 4) * 128 + (row[a] % 32) * 16 + (row[a] / 32 % 4) * 4 +
                                  (lane16 >> 2));
             }
         }
@@ -253,10 +254,10 @@ __global__ void __launch_bounds__(1024) moe_quantize_routes_mxfp4_kernel(const T
     if (first_live) load8<true>(src + threadIdx.x * 8, v);
     const uint32_t slot0 = blockIdx.y * slots_per_cta, slots = min(slots_per_cta, routes_per_row - slot0);
     if (threadIdx.x < slots) {
-        const uint32_t route = token * routes_per_row + slot0 + threadIdx.x, sorted = __ldg(route_to_sorted + route);
+        const uint32_t route = token * routes_per_row + slot0 + threadIdx.x, sorted = __ldcg(route_to_sorted + route);
         size_t row = ~static_cast<size_t>(0), scale = 0;
-        if (sorted < routes && __ldg(sorted_routes + sorted) == route) {  // (a route to an expert that does not exist has no place)
-            const uint32_t expert = __ldg(sorted_experts + sorted), offset = __ldg(offsets + expert);
+        if (sorted < routes && __ldcg(sorted_routes + sorted) == route) {  // (a route to an expert that does not exist has no place)
+            const uint32_t expert = __ldcg(sorted_experts + sorted), offset = __ldcg(offsets + expert);
             row = static_cast<size_t>(sorted) * (inner / 2);
             scale = ((static_cast<size_t>(offset) + 127) / 128 + expert) * tile_bytes + mx::tiled_offset(sorted - offset, 0, inner / mx::kBlock);
         }

@@ -293,6 +293,30 @@ def test_decode_is_the_same_in_every_run_and_order(tokens, dtype):
     assert torch.equal(plan.run(x, w, out_dtype=torch.float32)[0], y[0])
 
 
+def test_calls_in_a_row_read_what_was_just_written():
+    """Calls without a pause between them, on buffers that the allocator hands around and that held NaNs before: every launch reads what the
+    one in front of it wrote, not what was there when it started."""
+    g = gen(14)
+    for n, k, tokens, dtype in ((3001, 8192, 9, torch.float32), (1000, 2912, 8, torch.bfloat16), (256, 512, 3, torch.float32)):
+        w, plan = ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k)), ops.Mxfp4DecodePlan(64, n, k)
+        gemm = ops.Mxfp4MatmulPlan(tokens, n, k)
+        xs = [randn(g, tokens, k, dtype=dtype) for _ in range(2)]
+        want = []
+        for x in xs:
+            want.append((plan.run(x, w), gemm.run(ops.quantize_mxfp4(x), w), ops.quantize_mxfp4(x).dequantize()))
+            torch.cuda.synchronize()
+        wrong = torch.zeros((), device="cuda", dtype=torch.int64)
+        for i in range(100):
+            junk = torch.full((tokens * k // 2,), float("nan"), device="cuda", dtype=torch.float64)
+            junk.sum()
+            del junk
+            x, (decoded, multiplied, values) = xs[i % 2], want[i % 2]
+            wrong += (plan.run(x, w) != decoded).any().long()
+            wrong += (gemm.run(ops.quantize_mxfp4(x), w) != multiplied).any().long()
+            wrong += (ops.quantize_mxfp4(x).dequantize() != values).any().long()
+        assert int(wrong) == 0
+
+
 # ---- routed experts -----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("tokens,experts,top_k,hidden,inter", [(1, 4, 2, 64, 32), (5, 8, 3, 160, 96), (77, 16, 4, 512, 288), (300, 6, 6, 288, 320), (1000, 32, 2, 256, 128)])
