@@ -1,4 +1,5 @@
-// W4A16 product of MXFP4 weights for few tokens: y[t][n] = sum_k x[t][k] * w[n][k] (+ beta * C), the weights streamed once.
+// W4A16 product of MXFP4 weights for few tokens: y[t][n] = sum_k x[t][k] * w[n][k] (+ beta * C), the weights streamed once for 16 tokens.  This
+// is the form for a handful of tokens and for every K that is a multiple of 32; takes_terms says which calls go to the other.
 //
 // Bound: HBM, N * K * 17/32 bytes of weights.  A CTA of eight warps has 16 or 32 rows and their whole K, so nothing leaves a CTA but its
 // results: no partial sums, the same order of additions in every run.
@@ -17,6 +18,7 @@
 #include <new>
 
 #include "gemm_launch.cuh"
+#include "decode_mxfp4.cuh"
 #include "mx_block.cuh"
 #include "eider_b200.h"
 
@@ -241,13 +243,33 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_mxfp4_kernel(const XT
     }
 }
 
+// A result whose sum came out infinite or NaN, added up again block by block with x in its own size: sums of x brought to 2^14 overflow
+// before the result does, and a NaN scale counts as an infinity in the loop.
+__device__ __noinline__ float add_again(const Params& p, uint32_t terms, uint32_t token, uint32_t row, const uint8_t* scales) {
+    const float back = __ldcg(p.back + token);
+    float sum = 0.0f;
+    for (uint32_t block = 0; block < p.k / mx::kBlock; ++block) {
+        if (scales[block] == mx::kNanCode) return NAN;
+        float part = 0.0f;
+        for (uint32_t k = block * mx::kBlock; k < (block + 1) * mx::kBlock; ++k) {
+            float x = 0.0f;
+            for (uint32_t term = 0; term < terms; ++term) x += f16x2_values(__ldcg(p.x + (static_cast<size_t>(token) * terms + term) * p.k + k)).x;
+            const uint32_t code = p.w[static_cast<size_t>(row) * (p.k / 2) + k / 2] >> (k % 2 * 4) & 15, m = code & 7;
+            const float w = m < 4 ? 0.5f * m : m == 7 ? 6.0f : m - 2.0f;
+            part = fmaf(x, code & 8 ? -w : w, part);
+        }
+        sum += part * back * scale_of<0>(scales[block]);
+    }
+    return sum;
+}
+
 // TILES: 16-row MMA tiles of a CTA.
 // SPREAD: consecutive blocks that take an MMA column each.  Few tokens leave most of the eight columns empty, so block j of SPREAD goes
 // through column j of its token alone: the MMAs of SPREAD blocks add up in one accumulator, whose columns then get their block
 // scales in one go.  SPLIT_TERMS: the two f16 terms of f32 are columns too (up to four tokens).  Else TERMS 2: MMAs of the same weights.
 // COLS: groups of eight columns.
 template <int TILES, int SPREAD, int TERMS, bool SPLIT_TERMS, int COLS>
-__global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode_mxfp4_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode_mxfp4_kernel(const __grid_constant__ Params p) {
     constexpr int kSpan = SPREAD * (SPLIT_TERMS ? 2 : 1);  // columns of a token
     constexpr int kTokens = 8 * COLS / kSpan;
     constexpr int kGroups = kStepBlocks / SPREAD;
@@ -411,10 +433,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode
 #pragma unroll
         for (uint32_t v = 0; v < kWarps; ++v) sum += sums[(v * kTokens + token) * reduce_pitch(TILES) + row];
         sum *= __ldcg(p.back + token);
-        if (!(fabsf(sum) < INFINITY)) {  // a NaN scale among the row's?
-            for (uint32_t k = 0; k < blocks; ++k)
-                if (scales[row * p.pitch + k] == mx::kNanCode) sum = NAN;
-        }
+        if (!(fabsf(sum) < INFINITY)) sum = add_again(p, TERMS == 2 || SPLIT_TERMS ? 2 : 1, token, row0 + row, scales + row * p.pitch);
         const size_t index = static_cast<size_t>(token) * p.n + row0 + row;
         if (p.beta != 0.0f)
             sum = fmaf(p.beta, p.out_is_bf16 ? bf16_bits_to_float(static_cast<const uint16_t*>(p.c)[index]) : static_cast<const float*>(p.c)[index], sum);
@@ -425,7 +444,19 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode
 
 struct Plan {
     uint32_t max_tokens, n, k;
+    gemm::FifoCache<CUtensorMap> maps;
 };
+
+// The weights go to the tensor cores as they are (decode_mxfp4_terms.cu) where their layout allows, but for a few tokens and weights that are
+// neither long nor many.  us here / there, bf16: K 5120 -> N 13824 one token 10.8 / 11.6, eight 13.6 / 12.5, sixteen 19.8 / 13.8, 48 in
+// three launches 50.6 / 21.7; K 1024 -> N 2048 one 3.5 / 4.9; K 13824 -> N 5120 one 15.3 / 12.0, 48 73 / 19.4; K 5120 -> N 27648 one 18.2 /
+// 17.0.  f32: K 5120 -> N 13824 one 10.9 / 12.2, five 15.8 / 12.7.
+constexpr uint32_t kFewTokens = 4, kLongK = 8192;
+constexpr uint64_t kManyWeights = 1ull << 27;
+bool takes_terms(uint32_t tokens, uint32_t n, uint32_t k, int input_is_bf16) {
+    const bool few = tokens <= (input_is_bf16 ? kFewTokens : kFewTokens / 2) && k < kLongK && static_cast<uint64_t>(n) * k < kManyWeights;
+    return !few && k % 128 == 0 && n <= 65535u * 128;
+}
 
 template <int TILES, int SPREAD, int TERMS, bool SPLIT_TERMS, int COLS> cudaError_t launch(Params p, cudaStream_t stream) {
     auto kernel = decode_mxfp4_kernel<TILES, SPREAD, TERMS, SPLIT_TERMS, COLS>;
@@ -493,25 +524,30 @@ extern "C" {
 
 void* eider_b200_mxfp4_decode_create(uint32_t max_tokens, uint32_t out_features, uint32_t in_features) {
     if (max_tokens == 0 || max_tokens > 64 || out_features == 0 || in_features == 0 || in_features % mx::kBlock != 0 || in_features > 65536) return nullptr;
-    return new (std::nothrow) decode_mx::Plan{max_tokens, out_features, in_features};
+    return new (std::nothrow) decode_mx::Plan{max_tokens, out_features, in_features, {}};
 }
 
 void eider_b200_mxfp4_decode_destroy(void* raw) { delete static_cast<decode_mx::Plan*>(raw); }
 
 size_t eider_b200_mxfp4_w4a16_workspace_bytes(uint32_t tokens, uint32_t in_features, int input_is_bf16) {
-    return decode_mx::back_bytes(tokens) + static_cast<size_t>(tokens) * in_features * (input_is_bf16 ? 2 : 4);
+    const size_t few = decode_mx::back_bytes(tokens) + static_cast<size_t>(tokens) * in_features * (input_is_bf16 ? 2 : 4);
+    return in_features % 128 == 0 ? std::max(few, decode_mx::terms_workspace_bytes(tokens, in_features, input_is_bf16)) : few;  // (whichever form it takes)
 }
 
 cudaError_t eider_b200_mxfp4_w4a16_gemv_on_stream(void* raw, const void* input, int input_is_bf16, uint32_t tokens, const uint8_t* w_values,
-                                                  const uint8_t* w_scales_rows, uint32_t scale_pitch, const void* c, void* d, float beta,
-                                                  int out_is_bf16, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+                                                  const uint8_t* w_scales_rows, uint32_t scale_pitch, const uint8_t* w_scales_tiled, const void* c,
+                                                  void* d, float beta, int out_is_bf16, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     using namespace decode_mx;
     auto* plan = static_cast<Plan*>(raw);
-    if (!plan || !input || !w_values || !w_scales_rows || !d || tokens == 0 || tokens > plan->max_tokens || (beta != 0.0f && !c)) return cudaErrorInvalidValue;
-    if (((reinterpret_cast<uintptr_t>(input) | reinterpret_cast<uintptr_t>(w_values) | reinterpret_cast<uintptr_t>(w_scales_rows)) & 15) != 0 ||
+    if (!plan || !input || !w_values || !w_scales_rows || !w_scales_tiled || !d || tokens == 0 || tokens > plan->max_tokens || (beta != 0.0f && !c)) return cudaErrorInvalidValue;
+    if (((reinterpret_cast<uintptr_t>(input) | reinterpret_cast<uintptr_t>(w_values) | reinterpret_cast<uintptr_t>(w_scales_rows) |
+          reinterpret_cast<uintptr_t>(w_scales_tiled)) & 15) != 0 ||
         !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
         workspace_bytes < eider_b200_mxfp4_w4a16_workspace_bytes(tokens, plan->k, input_is_bf16) || scale_pitch % 16 != 0 || scale_pitch < (plan->k / mx::kBlock + 7) / 8 * 8)
         return cudaErrorInvalidValue;
+    if (takes_terms(tokens, plan->n, plan->k, input_is_bf16) && (reinterpret_cast<uintptr_t>(w_values) & 31) == 0)
+        return run_terms(plan->maps, input, input_is_bf16, tokens, w_values, w_scales_tiled, c, d, beta, out_is_bf16, plan->n, plan->k,
+                         static_cast<uint8_t*>(workspace), stream);
     float* back = static_cast<float*>(workspace);
     uint16_t* prepared = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + back_bytes(tokens));
     cudaError_t st = input_is_bf16 ? prepare<uint16_t>(input, prepared, back, tokens, plan->k, stream)

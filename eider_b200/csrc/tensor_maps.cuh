@@ -44,6 +44,21 @@ cudaError_t make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// FP4 codes [rows][k], k % 128 == 0, loaded 16 codes to the lower half of 16 bytes: box = 128 codes x box_rows, 128-byte swizzle.
+cudaError_t make_spread_fp4_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t k, uint32_t box_rows) {
+    EncodeTiled enc = encode_fn();
+    if (!enc) return cudaErrorNotSupported;
+    if ((reinterpret_cast<uintptr_t>(base) & 31) != 0 || k % 128 != 0) return cudaErrorInvalidValue;
+    cuuint64_t dims[2] = {k, rows};
+    cuuint64_t strides[1] = {k / 2};
+    cuuint32_t box[2] = {128, box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(base), dims, strides, box, elem,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // Tensor maps a plan has already encoded: encoding costs a driver call of a microsecond or two, which is a visible part of a 9 us
 // decode launch.
 struct MapCache {

@@ -258,15 +258,16 @@ def test_decode_activation_ranges(dtype):
     assert not y[2].any()
 
 
-def test_decode_poison_stays_with_its_token_and_row():
+@pytest.mark.parametrize("k,dtype", [(1024, torch.bfloat16), (1024, torch.float32), (1056, torch.bfloat16), (1056, torch.float32)])
+def test_decode_poison_stays_with_its_token_and_row(k, dtype):
     g = gen(12)
-    n, k = 100, 1024
+    n = 100
     wp, ws = ref.weight(g, n, k)
     ws[7, 3] = 255
     ws[9] = 0
     ws[11, 5] = 254
     w = ops.Mxfp4Weight.from_checkpoint(wp, ws)
-    x = randn(g, 5, k, dtype=torch.bfloat16)
+    x = randn(g, 5, k, dtype=dtype)
     x[1, 100] = float("nan")
     x[3, 700] = float("inf")
     y = ops.Mxfp4DecodePlan(8, n, k).run(x, w, out_dtype=torch.float32)
@@ -275,7 +276,10 @@ def test_decode_poison_stays_with_its_token_and_row():
     assert torch.isnan(y[1]).all() and not torch.isfinite(y[3]).any() and torch.isnan(y[:, 7]).all()
     fine = torch.isfinite(want) & (want.abs() < 3e38)
     fine[:, 7] = False
-    assert fine[0].sum() >= 98 and ((y.double() - want).abs()[fine] <= (decode_bound(x.double().nan_to_num(0, 0, 0), wv.nan_to_num(0), torch.bfloat16) + 1e-38)[fine]).all()
+    assert fine[0].sum() >= 98 and ((y.double() - want).abs()[fine] <= (decode_bound(x.double().nan_to_num(0, 0, 0), wv.nan_to_num(0), dtype) + 1e-38)[fine]).all()
+    # infinities by the weight's sign, NaN where it is zero (row 11 aside: what its scale of 2^127 makes of the finite elements overflows)
+    rest = torch.arange(n, device="cuda") != 11
+    assert torch.equal(y[3, rest].double().nan_to_num(nan=7.0), want[3, rest].nan_to_num(nan=7.0))
 
 
 @pytest.mark.parametrize("tokens,dtype", [(1, torch.bfloat16), (2, torch.float32), (4, torch.bfloat16), (8, torch.float32), (16, torch.bfloat16), (40, torch.bfloat16)])

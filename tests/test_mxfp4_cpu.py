@@ -55,8 +55,9 @@ def test_products_refuse():
     assert lib.eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream(None, SOME, SOME, SOME, SOME, 1.0, SOME, SOME, None) == INVALID
     for shape in ((0, 8, 32), (65, 8, 32), (1, 0, 32), (1, 8, 40), (1, 8, 65568)):
         assert not lib.eider_b200_mxfp4_decode_create(*shape)
-    assert lib.eider_b200_mxfp4_w4a16_gemv_on_stream(None, SOME, 1, 1, SOME, SOME, 16, None, SOME, 0.0, 1, SOME, 1 << 20, None) == INVALID
+    assert lib.eider_b200_mxfp4_w4a16_gemv_on_stream(None, SOME, 1, 1, SOME, SOME, 16, SOME, None, SOME, 0.0, 1, SOME, 1 << 20, None) == INVALID
     assert lib.eider_b200_mxfp4_w4a16_workspace_bytes(5, 64, 1) == 128 + 5 * 64 * 2 and lib.eider_b200_mxfp4_w4a16_workspace_bytes(64, 64, 0) == 256 + 64 * 64 * 4
+    assert lib.eider_b200_mxfp4_w4a16_workspace_bytes(9, 256, 1) == 2 * (2 * 16 * 128 + 512)
     assert lib.eider_b200_mxfp4_grouped_gemm_supported(96, 10, 160, 3) == 1
     for shape in ((48, 10, 64, 3), (96, 10, 80, 3), (96, 0, 64, 3), (96, 10, 64, 0), (1 << 20, 10, 64, 4096)):
         assert lib.eider_b200_mxfp4_grouped_gemm_supported(*shape) == 0
