@@ -10,6 +10,10 @@
 // maximum of every 64 consecutive logits (a segment).  beam_merge_kernel, one CTA per sequence, finds the k best segments by their
 // maxima (the k best elements cannot lie in any others: each of k better segments holds a better element) and then the k best of
 // their elements.  Nothing of the order of vocab is written or sorted; no atomics decide an order.
+//
+// Measured (B200): 64 x 8 x 151936 bf16 56.7 us, the scan 38 (4.1 TB/s; its share of the floor is 23.8) and the merge 21 (four
+// dependent passes over 19 thousand maxima a sequence, 64 CTAs of 148 SMs); 1 x 4 x 32000 f32 14.8 us, latencies of the two launches;
+// reordering 64 x 8 states of 64 KB, twice, 15.8 us.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

@@ -4,6 +4,9 @@
 // Every kernel gives a lane eight consecutive elements (16 bytes of bf16, one 4-byte word of codes), four lanes a block and sixteen
 // lanes a UNIT of four blocks: 128 elements whose four scale bytes are one word of the tiled layout.  The block maximum takes two
 // shuffles, the scale word two more; loads and stores of a warp are contiguous.
+//
+// Bound: HBM, elements in and 17/32 byte an element out.  Measured (B200): 16384 x 13824 bf16 135 us (4.3 TB/s, 0.65 of a copy: the issue
+// slots of the rounding), 4096 x 8192 f32 26.4 us (0.88), 512 x 5120 5.4 us, one row of 5120 1.7 us; the inverse 16384 x 13824 150 us.
 #include <algorithm>
 
 #include "common.cuh"
