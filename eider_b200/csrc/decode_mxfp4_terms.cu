@@ -15,7 +15,8 @@
 //    a single MMA.
 //  * x is prepared by a launch of its own in the operand's layout, a step one contiguous piece that a bulk copy brings, while the first
 //    steps of weights are on their way.  Every CTA reads its part of it from L2: 12 KB a step of 8.5 KB of weights for 48 tokens, which is what
-//    they cost beyond one (K 5120 -> N 13824: 1 token 11.6 us, 16 13.8, 48 21.7, 64 24.4; K 13824 -> N 5120: 12.0, 13.3, 19.4, 21.7).
+//    they cost beyond one (K 5120 -> N 13824: 1 token 11.6 us, 16 13.8, 48 21.7; K 13824 -> N 5120: 12.0, 13.3, 19.4; 64 tokens, whose
+//    tensor memory leaves room for two CTAs an SM, 33.2 and 30.3).
 #include <algorithm>
 #include <atomic>
 
@@ -57,7 +58,7 @@ struct Params {
     const void* c;
     float beta;
     int out_is_bf16, x_is_bf16;
-    uint32_t tokens, padded, terms, columns, n, k, stages, sum_columns;
+    uint32_t tokens, padded, terms, columns, n, k, stages, tmem_columns;
 };
 
 __device__ __forceinline__ float lds_cluster(uint32_t address) {
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
     extern __shared__ uint8_t raw_smem[];
     uint8_t* smem = raw_smem + (1024 - (umma::smem_u32(raw_smem) & 1023)) % 1024;  // (the same offset in every CTA)
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
-    __shared__ uint32_t tmem_sums, tmem_scales;
+    __shared__ uint32_t tmem_base;
     __shared__ volatile uint32_t abort_flag;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t split = blockIdx.x, splits = gridDim.x;  // the cluster is a row of the grid
@@ -193,15 +194,14 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
         umma::fence_barrier_init();
     }
     if (warp == 2) {
-        umma::tmem_alloc(&tmem_sums, p.sum_columns);
-        umma::tmem_alloc(&tmem_scales, kScaleColumns);
+        umma::tmem_alloc(&tmem_base, p.tmem_columns);  // (in one piece: no CTA waits for tensor memory while it holds some)
         umma::tmem_relinquish();
     }
     umma::tc_fence_before();
     __syncthreads();
     umma::tc_fence_after();
     umma::griddep_launch_dependents();  // (not before this CTA has its tensor memory: a dependent's could be in its place)
-    const uint32_t tmem = tmem_sums, scale_columns = tmem_scales;
+    const uint32_t tmem = tmem_base, scale_columns = tmem + p.tmem_columns - kScaleColumns;
 
     if (warp == 0 || warp == 3) {
         // ------------------------------------------------------------------------------------------ copies: weights, and x behind the launch in front
@@ -284,8 +284,7 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
     __syncthreads();
     if (warp == 2) {  // before the cluster meets: no CTA holds tensor memory while it waits for another
         umma::tc_fence_after();
-        umma::tmem_dealloc(tmem, p.sum_columns);
-        umma::tmem_dealloc(scale_columns, kScaleColumns);
+        umma::tmem_dealloc(tmem, p.tmem_columns);
     }
     if (splits > 1) umma::cluster_sync_all();
     umma::griddep_wait();
@@ -385,7 +384,9 @@ cudaError_t run_terms(gemm::FifoCache<CUtensorMap>& maps, const void* x, int inp
         p.padded = padded_of(p.tokens);
         p.terms = terms_of(input_is_bf16);
         p.columns = p.terms * p.padded;
-        p.sum_columns = p.columns <= 32 ? 32 : p.columns <= 64 ? 64 : 128;
+        // (beyond 96 columns two CTAs an SM have their tensor memory at a time, not three.  Sums and scales in pieces of their own
+        // would let three run, 24.4 us instead of 33.2 for 64 tokens, but hold one piece while they wait for the other)
+        p.tmem_columns = p.columns + kScaleColumns <= 64 ? 64 : p.columns + kScaleColumns <= 128 ? 128 : 256;
         p.n = n;
         p.k = k;
         p.stages = std::min(std::min(kMaxStages, (steps + splits - 1) / splits), kRing / stage_bytes(p.columns));
