@@ -1294,6 +1294,8 @@ def moe_weighted_accumulate(routes: MoeSortedRoutes, route_weights: torch.Tensor
         out = torch.empty(tokens, ln, dtype=torch.float32, device=sorted_rows.device)
     if out.dtype == torch.bfloat16:
         _need(out, torch.bfloat16, "output")
+        if out.shape != (tokens, ln) or out.device != sorted_rows.device:
+            raise ShapeError(f"output must be ({tokens}, {ln}) on {sorted_rows.device}, got {tuple(out.shape)} on {out.device}")
         check("eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream",
               lib.eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream(routes.route_to_sorted.data_ptr(), route_weights.data_ptr(),
                                                                               sorted_rows.data_ptr(), out.data_ptr(), tokens, ln, routes_per_row,

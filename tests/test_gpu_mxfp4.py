@@ -418,3 +418,10 @@ def test_refusals():
     moe = ops.GroupedMoe(4, 2, 1, 64, 32, weight_format="mxfp4")
     with pytest.raises(ops.ShapeError):
         moe.run(randn(g, 4, 64), randn(g, 4, 2), None, None)
+
+
+def test_combine_refuses_a_bf16_output_of_another_shape():
+    rows = torch.zeros(8, 64, device="cuda", dtype=torch.bfloat16)
+    weights = torch.zeros(4, 2, device="cuda")
+    with pytest.raises(ops.ShapeError):
+        ops.moe_weighted_accumulate(None, weights, rows, 4, 2, out=torch.zeros(3, 64, device="cuda", dtype=torch.bfloat16))
