@@ -1286,25 +1286,23 @@ def moe_weighted_accumulate(routes: MoeSortedRoutes, route_weights: torch.Tensor
                             tokens: int, routes_per_row: int, out: torch.Tensor | None = None) -> torch.Tensor:
     """moe_weighted_accumulate_sorted_bf16_batch (crates/eider-cuda/src/kernels/non_gemm.rs:3336+): f32 [tokens, len]; a bf16 `out`
     takes the f32 sums rounded once."""
-    lib = _lib.load()
     _need(sorted_rows, torch.bfloat16, "sorted rows")
     _need(route_weights, torch.float32, "route weights")
-    ln = sorted_rows.shape[1]
+    if sorted_rows.dim() != 2 or sorted_rows.shape[0] < tokens * routes_per_row or route_weights.numel() != tokens * routes_per_row:
+        raise ShapeError(f"{tokens} tokens of {routes_per_row} routes want a row and a weight per route, got rows {tuple(sorted_rows.shape)} and "
+                         f"{route_weights.numel()} weights")
+    ln, device = sorted_rows.shape[1], sorted_rows.device
     if out is None:
-        out = torch.empty(tokens, ln, dtype=torch.float32, device=sorted_rows.device)
-    if out.dtype == torch.bfloat16:
-        _need(out, torch.bfloat16, "output")
-        if out.shape != (tokens, ln) or out.device != sorted_rows.device:
-            raise ShapeError(f"output must be ({tokens}, {ln}) on {sorted_rows.device}, got {tuple(out.shape)} on {out.device}")
-        check("eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream",
-              lib.eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream(routes.route_to_sorted.data_ptr(), route_weights.data_ptr(),
-                                                                              sorted_rows.data_ptr(), out.data_ptr(), tokens, ln, routes_per_row,
-                                                                              _stream()))
-        return out
-    check("infer_moe_weighted_accumulate_sorted_bf16_batch_on_stream",
-          lib.infer_moe_weighted_accumulate_sorted_bf16_batch_on_stream(routes.route_to_sorted.data_ptr(),
-                                                                        route_weights.data_ptr(), sorted_rows.data_ptr(),
-                                                                        out.data_ptr(), tokens, ln, routes_per_row, _stream()))
+        out = torch.empty(tokens, ln, dtype=torch.float32, device=device)
+    _need_floats(out, "output")
+    if out.shape != (tokens, ln):
+        raise ShapeError(f"output must be ({tokens}, {ln}), got {tuple(out.shape)}")
+    if routes.route_to_sorted.numel() != tokens * routes_per_row:
+        raise ShapeError(f"the sorted routes are {routes.route_to_sorted.numel()}, not {tokens} x {routes_per_row}")
+    _need_device(device, route_weights, out, routes.route_to_sorted)
+    name = ("eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_stream" if out.dtype == torch.bfloat16
+            else "infer_moe_weighted_accumulate_sorted_bf16_batch_on_stream")
+    _call(device, name, routes.route_to_sorted.data_ptr(), route_weights.data_ptr(), sorted_rows.data_ptr(), out.data_ptr(), tokens, ln, routes_per_row)
     return out
 
 
