@@ -17,6 +17,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <memory>
+#include <new>
 
 #include "common.cuh"
 #include "quant_block.cuh"
@@ -441,6 +443,30 @@ uint32_t splits_of(uint32_t rows, uint32_t vocab, bool bf16) {
     const uint32_t elems = bf16 ? 8 : 4, vectors = (vocab + elems - 1) / elems + 1, per = vectors_per_split(rows, vocab, bf16);
     return (vectors + per - 1) / per;
 }
+// Whether an output lies over a state, any state, or over another output: all are copied at once, and a row would be read or written
+// after another copy had written there.  (States may share memory.)  In the order of addresses each output has to begin behind all
+// that came before it, and each state behind the outputs.
+bool outputs_overlap(const void* const* src, void* const* dst, const size_t* row_bytes, uint32_t count, size_t rows) {
+    struct Span {
+        uintptr_t begin, end;
+        bool written;
+    };
+    std::unique_ptr<Span[]> spans(new (std::nothrow) Span[2 * static_cast<size_t>(count)]);
+    if (!spans) return true;
+    for (uint32_t i = 0; i < count; ++i) {
+        const auto s = reinterpret_cast<uintptr_t>(src[i]), d = reinterpret_cast<uintptr_t>(dst[i]);
+        spans[2 * i] = {s, s + row_bytes[i] * rows, false};
+        spans[2 * i + 1] = {d, d + row_bytes[i] * rows, true};
+    }
+    std::sort(spans.get(), spans.get() + 2 * static_cast<size_t>(count), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    uintptr_t written = 0, read = 0;
+    for (size_t i = 0; i < 2 * static_cast<size_t>(count); ++i) {
+        const Span& s = spans[i];
+        if (s.begin < written || (s.written && s.begin < read)) return true;
+        (s.written ? written : read) = std::max(s.written ? written : read, s.end);
+    }
+    return false;
+}
 bool beam_shape_ok(uint32_t batch, uint32_t beams, uint32_t vocab) {
     return batch != 0 && beams != 0 && beams <= kMaxBeams && vocab != 0 && batch <= 0xffffu / beams && vocab <= 0x7fffffffu / beams - 64;
 }
@@ -498,13 +524,9 @@ cudaError_t eider_b200_beam_reorder_on_stream(const void* const* src, void* cons
     if (!src || !dst || !row_bytes || count == 0 || !parents || batch == 0 || beams == 0 || parent_stride < beams ||
         static_cast<uint64_t>(batch) * beams > 0x7fffffffu)
         return cudaErrorInvalidValue;
-    for (uint32_t i = 0; i < count; ++i) {
+    for (uint32_t i = 0; i < count; ++i)
         if (!src[i] || !dst[i] || row_bytes[i] == 0) return cudaErrorInvalidValue;
-        // (rows are read after others have been written: a state cannot be reordered in place)
-        const auto s = reinterpret_cast<uintptr_t>(src[i]), d = reinterpret_cast<uintptr_t>(dst[i]);
-        const uintptr_t bytes = row_bytes[i] * batch * beams;
-        if (s < d + bytes && d < s + bytes) return cudaErrorInvalidValue;
-    }
+    if (outputs_overlap(src, dst, row_bytes, count, static_cast<size_t>(batch) * beams)) return cudaErrorInvalidValue;
     for (uint32_t first = 0; first < count; first += kStates) {
         ReorderArgs a{};
         const uint32_t states = std::min(kStates, count - first);

@@ -1418,9 +1418,9 @@ def beam_search_select(logits: torch.Tensor, beam_scores: torch.Tensor, k: int, 
 
 def beam_search_reorder(states: list, parents: torch.Tensor, out: list | None = None) -> list:
     """The beams' states behind a selection: out[i][b, j] = states[i][b, parents[b, j]] for tensors [batch, beams, ...] of any type.
-    `parents` [batch, beams] int32 (rows may be apart, as in the first `beams` columns of a selection).  Never in place: `out`
-    takes other tensors of the same shapes, e.g. the second of two sets that a decode loop swaps.  A parent that is no beam leaves its
-    row of `out` as it is."""
+    `parents` [batch, beams] int32 (rows may be apart, as in the first `beams` columns of a selection).  Never in place: all states are
+    copied at once, so `out` takes other tensors of the same shapes that overlap neither a state nor each other, e.g. the second of
+    two sets that a decode loop swaps.  A parent that is no beam leaves its row of `out` as it is."""
     if parents.dim() != 2 or not parents.is_cuda or parents.dtype != torch.int32 or parents.numel() == 0 or parents.stride(1) != 1:
         raise ShapeError("parents must be a CUDA tensor [batch, beams] of int32")
     batch, beams = parents.shape
@@ -1435,11 +1435,17 @@ def beam_search_reorder(states: list, parents: torch.Tensor, out: list | None = 
     for s, o in zip(states, out):
         if s.shape[:2] != (batch, beams) or s.numel() == 0 or o.shape != s.shape or o.dtype != s.dtype or not s.is_contiguous() or not o.is_contiguous():
             raise ShapeError(f"states must be contiguous [{batch}, {beams}, ...], and outputs like them")
-        first, other, size = s.data_ptr(), o.data_ptr(), s.nbytes
-        if first < other + size and other < first + size:
-            raise ShapeError("a state cannot be reordered in place")
-        sizes.append(size // (batch * beams))
+        sizes.append(s.nbytes // (batch * beams))
     _need_device(parents.device, *states, *out)
+    # in the order of addresses, only states may lie over each other
+    written = read = 0  # the end of the outputs and of the states so far
+    for start, size, is_out in sorted([(t.data_ptr(), t.nbytes, False) for t in states] + [(t.data_ptr(), t.nbytes, True) for t in out]):
+        if start < written or (is_out and start < read):
+            raise ShapeError("an output overlaps a state or another output: states cannot be reordered in place")
+        if is_out:
+            written = start + size
+        else:
+            read = max(read, start + size)
     n = len(states)
     pointers = C.c_void_p * n
     _call(parents.device, "eider_b200_beam_reorder_on_stream", pointers(*[s.data_ptr() for s in states]), pointers(*[o.data_ptr() for o in out]),

@@ -911,7 +911,8 @@ EIDER_B200_API cudaError_t eider_b200_beam_select_on_stream(const void* logits, 
                                                             int32_t* out_tokens, uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t k,
                                                             void* workspace, size_t workspace_bytes, cudaStream_t stream);
 /* dst[i][b][j] = src[i][b][parents[b][j]] for `count` states of rows of row_bytes[i] bytes (host arrays of device pointers; read before
- * the call returns).  No state may overlap its destination.  A parent outside 0 .. beams - 1 leaves its row as it is. */
+ * the call returns).  All are copied at once: no destination may overlap a state, its own or another, or another destination.  A parent
+ * outside 0 .. beams - 1 leaves its row as it is. */
 EIDER_B200_API cudaError_t eider_b200_beam_reorder_on_stream(const void* const* src, void* const* dst, const size_t* row_bytes, uint32_t count,
                                                              const int32_t* parents, size_t parent_stride, uint32_t batch, uint32_t beams,
                                                              cudaStream_t stream);

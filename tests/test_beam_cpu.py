@@ -1,10 +1,12 @@
 """Beam search refusals that need no GPU."""
 import ctypes as C
+import types
 
 import pytest
 import torch
 
 from eider_b200 import _lib, ops
+from tests import fakes
 
 INVALID = 1
 SOME = 0x1000
@@ -48,3 +50,31 @@ def test_python_layer_refuses():
         ops.beam_search_select(torch.zeros(1, 2, 8), torch.zeros(1, 2), 2)
     with pytest.raises(ops.ShapeError):
         ops.beam_search_reorder([torch.zeros(1, 2, 8)], torch.zeros(1, 2, dtype=torch.int32))
+
+
+def test_reorder_refuses_outputs_over_any_state():
+    """All states are copied at once, so an output may lie over no state and over no other output; states may share memory."""
+    f = _lib.load().eider_b200_beam_reorder_on_stream
+    ptrs, sizes = (C.c_void_p * 3), (C.c_size_t * 3)
+    rows, size = sizes(64, 64, 64), 64 * 8
+    a, b, c, d = (0x10000 + i * size for i in range(4))  # back to back
+    for src, dst in (((a, b, c), (b, c, d)), ((a, b, c), (d, a, 0x40000)), ((a, b, c), (0x40000, 0x40000 + size - 16, 0x50000)), ((a, b, c), (0x40000, 0x50000, c + 16)),
+                     ((a, a, a), (0x40000, 0x50000, 0x40000)), ((a, b, c), (0x40000, 0x50000, a - size + 1))):
+        assert f(ptrs(*src), ptrs(*dst), rows, 3, SOME, 4, 2, 4, None) == INVALID, (src, dst)
+    # an output that is long enough to reach over what lies behind it
+    assert f(ptrs(a, b, 0x50000), ptrs(c, d, a), sizes(64, 64, 192), 3, SOME, 4, 2, 4, None) == INVALID
+
+
+def test_python_reorder_refuses_outputs_over_any_state(monkeypatch):
+    called = fakes.without_a_device(monkeypatch)
+    parents = types.SimpleNamespace(dim=lambda: 2, is_cuda=True, dtype=torch.int32, numel=lambda: 8, stride=lambda i: (4, 1)[i], shape=(2, 4), device=torch.device("cpu"),
+                                    data_ptr=lambda: SOME)
+    buffer = torch.zeros(4, 2, 4, 16)
+    a, b, c, d = buffer
+    for states, out in (([a, b], [b, c]), ([a, b], [c, a]), ([a, b], [c, c]), ([a], [a]), ([a, b], [c, buffer.flatten()[8:136].view(2, 4, 16)])):
+        with pytest.raises(ops.ShapeError):
+            ops.beam_search_reorder(states, parents, out=out)
+    assert not called
+    ops.beam_search_reorder([a, c], parents, out=[b, d])
+    ops.beam_search_reorder([a, a], parents, out=[b, d])
+    assert called == ["eider_b200_beam_reorder_on_stream"] * 2
