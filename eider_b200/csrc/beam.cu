@@ -4,14 +4,18 @@
 //   score(r, v) = beam_score[r] + logits[r][v] - log sum_u exp(logits[r][u]),   the k largest of a sequence's beams x vocab scores,
 //   equal scores in the order of beam * vocab + v.
 //
-// The scores are compared in 64 bits: log-sum-exps differ from row to row, and f32 would tie what is not equal.
+// The scores are compared in 64 bits: log-sum-exps differ from row to row, and f32 would tie what is not equal.  A row's sum of
+// exponentials itself is of f32: hardware exponentials and partial sums, together within 2^-21 of it on normal logits up to 151936 of
+// them.  So the order within a row is exact, and candidates of different rows whose scores differ by less than that may change places.
+// Rows that are equal have equal sums wherever they lie: the parts of a sum are counted from the row's first element, whatever its
+// address.
 //
 // Two launches.  beam_scan_kernel reads the logits once (bound: HBM): running maximum and sum of exponentials per thread, and the
 // maximum of every 64 consecutive logits (a segment).  beam_merge_kernel, one CTA per sequence, finds the k best segments by their
 // maxima (the k best elements cannot lie in any others: each of k better segments holds a better element) and then the k best of
 // their elements.  Nothing of the order of vocab is written or sorted; no atomics decide an order.
 //
-// Measured (B200): 64 x 8 x 151936 bf16 56.7 us, the scan 38 (4.1 TB/s; its share of the floor is 23.8) and the merge 21 (four
+// Measured (B200): 64 x 8 x 151936 bf16 55.4 us, the scan 37 (4.1 TB/s; its share of the floor is 23.8) and the merge 21 (four
 // dependent passes over 19 thousand maxima a sequence, 64 CTAs of 148 SMs); 1 x 4 x 32000 f32 14.8 us, latencies of the two launches;
 // reordering 64 x 8 states of 64 KB, twice, 15.8 us.
 #include <algorithm>
@@ -78,55 +82,84 @@ __device__ __forceinline__ void vector_values(const uint4& q, float (&v)[8]) {
         v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
-// Rows need not start on 16 bytes: positions count from the 16-byte boundary at or below the row, `lead` elements before it.
-template <typename T> __device__ __forceinline__ uint32_t row_lead(const T* row) {
-    return static_cast<uint32_t>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+// Rows need not start on 16 bytes.  The 16 bytes from byte BYTES of piece v of memory on, in lane v: up to 8 it holds piece v and lacks the begin of the next lane's, beyond
+// it holds piece v + 1 and lacks the end of the lane's in front, two words at most.  `edge`: those two words for the lane at the end of
+// the warp, held by the lane at its other end, whose own words nobody takes.
+template <uint32_t BYTES> __device__ __forceinline__ uint4 shifted_piece(const uint4& piece, const uint2& edge, uint32_t lane) {
+    constexpr bool kForward = BYTES <= 8;
+    constexpr uint32_t kStart = kForward ? BYTES : BYTES - 8, kFirst = kStart / 4;
+    auto taken = [&](uint32_t own, uint32_t at_edge) { return __shfl_sync(kFullMask, lane == (kForward ? 0 : 31) ? at_edge : own, kForward ? lane + 1 : lane - 1); };
+    uint32_t w[6];
+    if constexpr (kForward) {
+        w[0] = piece.x; w[1] = piece.y; w[2] = piece.z; w[3] = piece.w;
+        w[4] = taken(piece.x, edge.x);
+        w[5] = kStart > 4 ? taken(piece.y, edge.y) : 0;
+    } else {
+        w[0] = kStart < 4 ? taken(piece.z, edge.x) : 0;
+        w[1] = taken(piece.w, edge.y);
+        w[2] = piece.x; w[3] = piece.y; w[4] = piece.z; w[5] = piece.w;
+    }
+    if constexpr (kStart % 4 == 0) return make_uint4(w[kFirst], w[kFirst + 1], w[kFirst + 2], w[kFirst + 3]);
+    else return make_uint4(__funnelshift_r(w[kFirst], w[kFirst + 1], 16), __funnelshift_r(w[kFirst + 1], w[kFirst + 2], 16),
+                           __funnelshift_r(w[kFirst + 2], w[kFirst + 3], 16), __funnelshift_r(w[kFirst + 3], w[kFirst + 4], 16));
 }
-
-template <typename T>
-__global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const BeamArgs a) {
-    constexpr uint32_t E = Vec<T>::kElems, kSegLanes = kSegment / E;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint32_t row = blockIdx.y;
-    if (!row_counts(a, row)) return;
-    const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
-    const uint32_t lead = row_lead(logits), end = lead + a.vocab;
-    const uint32_t v1 = min((blockIdx.x + 1) * a.vectors_per_split, (end + E - 1) / E);
-    float* segment_max = a.segment_max + static_cast<size_t>(row) * a.segments;
-    float top = -INFINITY, sum = 0.0f;
+// The running maximum and sum of a CTA's part of a row, and its segments' maxima.  The row begins BYTES behind a 16-byte boundary: if that
+// is not 0, a vector is the end of one piece of memory and the begin of the next.
+template <typename T, uint32_t BYTES> __device__ __forceinline__ void scan_row(const BeamArgs& a, const T* logits, float* segment_max, float& top, float& sum) {
+    constexpr uint32_t E = Vec<T>::kElems, kSegLanes = kSegment / E, kLead = BYTES / sizeof(T);
+    constexpr uint32_t kBehind = BYTES > 8 ? 1 : 0;  // (lanes hold the pieces that their vectors end in)
+    constexpr uint32_t kTurn = kScanThreads * kAhead;
+    const uint32_t lane = threadIdx.x % 32;
+    const uint32_t v1 = min((blockIdx.x + 1) * a.vectors_per_split, (a.vocab + E - 1) / E);
+    const uint4* pieces = reinterpret_cast<const uint4*>(logits - kLead);
+    // Whether the vectors from `first` on, `count` of them, come in pieces that lie in the row
+    auto in_pieces = [&](uint32_t first, uint32_t count) {
+        return kLead == 0 ? (first + count) * E <= a.vocab : first > 0 && (first + count + 1) * E - kLead <= a.vocab;
+    };
     // A turn's vectors, requested while the turn before is worked on.  (Whole warps run the same number of turns: a split is a
     // multiple of the block.)
     uint4 next[kAhead];
+    uint2 next_edge[kAhead] = {};
+    auto fetch_pieces = [&](uint32_t vec, uint32_t j) {
+        next[j] = __ldcg(pieces + vec + kBehind);
+        if (kLead != 0 && lane == (kBehind ? 31 : 0)) next_edge[j] = __ldcg(reinterpret_cast<const uint2*>(pieces + vec - lane + (kBehind ? 0 : 32)) + kBehind);
+    };
     auto fetch = [&](uint32_t base) {
-        const bool inside = base + kScanThreads * kAhead <= v1 && base * E >= lead && (base + kScanThreads * kAhead) * E <= end;
-        const uint4* vectors = reinterpret_cast<const uint4*>(logits - lead) + base + threadIdx.x;
-        if (inside) {
+        if (base + kTurn <= v1 && in_pieces(base, kTurn)) {
 #pragma unroll
-            for (uint32_t j = 0; j < kAhead; ++j) next[j] = __ldcg(vectors + j * kScanThreads);
+            for (uint32_t j = 0; j < kAhead; ++j) fetch_pieces(base + j * kScanThreads + threadIdx.x, j);
             return;
         }
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
             const uint32_t vec = base + j * kScanThreads + threadIdx.x, at = vec * E;
-            if (vec < v1 && at >= lead && at + E <= end) {
-                next[j] = __ldcg(vectors + j * kScanThreads);
-            } else {  // the row's first and last vectors, and none
+            if (vec < v1 && (kLead == 0 ? in_pieces(vec, 1) : in_pieces(vec - lane, 32))) {
+                fetch_pieces(vec, j);
+            } else {  // the row's last vectors (its first ones too, if they are in no whole pieces), and none
                 T v[E];
 #pragma unroll
-                for (uint32_t e = 0; e < E; ++e) v[e] = vec < v1 && at + e >= lead && at + e < end ? __ldcg(logits + (at + e - lead)) : minus_infinity<T>();
+                for (uint32_t e = 0; e < E; ++e) v[e] = vec < v1 && at + e < a.vocab ? __ldcg(logits + (at + e)) : minus_infinity<T>();
                 memcpy(&next[j], v, 16);
             }
         }
     };
     uint32_t base = blockIdx.x * a.vectors_per_split;
-    if (base < v1) fetch(base);
-    for (; base < v1; base += kScanThreads * kAhead) {
+    constexpr bool kPrefetch = kLead == 0;  // (vectors in two pieces take the registers of a turn ahead)
+    if (kPrefetch && base < v1) fetch(base);
+    for (; base < v1; base += kTurn) {
+        if (!kPrefetch) fetch(base);
         uint4 now[kAhead];
         float m[kAhead];
+        const bool whole = base + kTurn <= v1 && in_pieces(base, kTurn);
 #pragma unroll
-        for (uint32_t j = 0; j < kAhead; ++j) now[j] = next[j];
-        if (base + kScanThreads * kAhead < v1) fetch(base + kScanThreads * kAhead);
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            now[j] = next[j];
+            if constexpr (kLead != 0) {
+                const uint32_t first = base + j * kScanThreads + threadIdx.x - lane;  // (the warp's)
+                if (whole || (first < v1 && in_pieces(first, 32))) now[j] = shifted_piece<BYTES>(next[j], next_edge[j], lane);
+            }
+        }
+        if (kPrefetch && base + kTurn < v1) fetch(base + kTurn);
         float new_top = top;
 #pragma unroll
         for (uint32_t j = 0; j < kAhead; ++j) {
@@ -158,6 +191,29 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const BeamArgs 
             if (threadIdx.x % kSegLanes == 0 && vec < v1) segment_max[vec / kSegLanes] = m[j];
         }
     }
+}
+
+template <typename T, bool SHIFTED> __device__ __forceinline__ void scan(const BeamArgs& a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t row = blockIdx.y;
+    if (!row_counts(a, row)) return;
+    const T* logits = static_cast<const T*>(a.logits) + row * a.stride;
+    float* segment_max = a.segment_max + static_cast<size_t>(row) * a.segments;
+    float top = -INFINITY, sum = 0.0f;
+    const uint32_t bytes = SHIFTED ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(logits) & 15) : 0;
+    if (bytes == 0) scan_row<T, 0>(a, logits, segment_max, top, sum);
+    if constexpr (SHIFTED) {
+        if (bytes == 4) scan_row<T, 4>(a, logits, segment_max, top, sum);
+        if (bytes == 8) scan_row<T, 8>(a, logits, segment_max, top, sum);
+        if (bytes == 12) scan_row<T, 12>(a, logits, segment_max, top, sum);
+        if constexpr (sizeof(T) == 2) {
+            if (bytes == 2) scan_row<T, 2>(a, logits, segment_max, top, sum);
+            if (bytes == 6) scan_row<T, 6>(a, logits, segment_max, top, sum);
+            if (bytes == 10) scan_row<T, 10>(a, logits, segment_max, top, sum);
+            if (bytes == 14) scan_row<T, 14>(a, logits, segment_max, top, sum);
+        }
+    }
     __shared__ float tops[kScanThreads / 32], sums[kScanThreads / 32];
     auto join = [](float& t, float& s, float t2, float s2) {
         const float n = fmaxf(t, t2);
@@ -183,6 +239,11 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const BeamArgs 
         a.partial[static_cast<size_t>(row) * a.splits + blockIdx.x] = make_float2(top, sum);
     }
 }
+
+template <typename T> __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const BeamArgs a) { scan<T, false>(a); }
+// ... with rows that start between 16-byte boundaries, 64 registers for four CTAs an SM: 512 rows of 151935 bf16 logits cost 21 us more than
+// of 151936 (with three CTAs and requests a turn ahead 23), 128 rows of f32 5 more.
+template <typename T> __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_shifted_kernel(const BeamArgs a) { scan<T, true>(a); }
 
 struct Candidate {
     double score;
@@ -336,8 +397,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
                 continue;
             }
             const double top = sh.top[w], base = sh.base[w];
-            const uint32_t used = (row_lead(static_cast<const T*>(a.logits) + (row0 + w) * a.stride) + a.vocab + kSegment - 1) / kSegment;
-            const uint32_t last = min((part + 1) * per_part, used);
+            const uint32_t last = min((part + 1) * per_part, a.segments);
             for (uint32_t s = part * per_part + lane; s < last; s += 32 * kFetch) {
                 float x[kFetch];
 #pragma unroll
@@ -356,9 +416,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
                 continue;
             }
             const T* logits = static_cast<const T*>(a.logits) + (row0 + w) * a.stride;
-            const uint32_t position = s * kSegment + j % kSegment, lead = row_lead(logits);
-            if (position >= lead && position - lead < a.vocab)
-                use(Candidate{(logit_value(__ldcg(logits + (position - lead))) - sh.top[w]) + sh.base[w], w * a.vocab + (position - lead)});
+            const uint32_t token = s * kSegment + j % kSegment;
+            if (token < a.vocab) use(Candidate{(logit_value(__ldcg(logits + token)) - sh.top[w]) + sh.base[w], w * a.vocab + token});
         }
     });
     for (uint32_t r = threadIdx.x; r < a.k; r += kMergeThreads) {
@@ -431,17 +490,17 @@ __global__ void __launch_bounds__(kCopyThreads) beam_reorder_kernel(const Reorde
     }
 }
 
-uint32_t segments_of(uint32_t vocab, bool bf16) { return (vocab + (bf16 ? 7 : 3) + kSegment - 1) / kSegment; }
+uint32_t segments_of(uint32_t vocab) { return (vocab + kSegment - 1) / kSegment; }
+uint32_t vectors_of(uint32_t vocab, bool bf16) { return (vocab + (bf16 ? 7 : 3)) / (bf16 ? 8 : 4); }
 // Splits of a row: a dozen CTAs an SM, so that the last ones do not leave most SMs idle, while a split keeps a few thousand logits.
 uint32_t vectors_per_split(uint32_t rows, uint32_t vocab, bool bf16) {
-    const uint32_t elems = bf16 ? 8 : 4, vectors = (vocab + elems - 1) / elems + 1;
     const uint32_t wanted = std::max(1u, (148u * 12u + rows - 1) / rows);
-    const uint32_t per = (vectors + wanted - 1) / wanted;
-    return (std::max(per, 1u) + kScanThreads - 1) / kScanThreads * kScanThreads;
+    const uint32_t per = (vectors_of(vocab, bf16) + wanted - 1) / wanted;
+    return (per + kScanThreads - 1) / kScanThreads * kScanThreads;
 }
 uint32_t splits_of(uint32_t rows, uint32_t vocab, bool bf16) {
-    const uint32_t elems = bf16 ? 8 : 4, vectors = (vocab + elems - 1) / elems + 1, per = vectors_per_split(rows, vocab, bf16);
-    return (vectors + per - 1) / per;
+    const uint32_t per = vectors_per_split(rows, vocab, bf16);
+    return (vectors_of(vocab, bf16) + per - 1) / per;
 }
 // Whether an output lies over a state, any state, or over another output: all are copied at once, and a row would be read or written
 // after another copy had written there.  (States may share memory.)  In the order of addresses each output has to begin behind all
@@ -481,7 +540,7 @@ extern "C" {
 size_t eider_b200_beam_select_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, int logits_are_bf16) {
     if (!beam_shape_ok(batch, beams, vocab)) return 0;
     const size_t rows = static_cast<size_t>(batch) * beams;
-    return rows * (splits_of(batch * beams, vocab, logits_are_bf16) * sizeof(float2) + segments_of(vocab, logits_are_bf16) * sizeof(float));
+    return rows * (splits_of(batch * beams, vocab, logits_are_bf16) * sizeof(float2) + segments_of(vocab) * sizeof(float));
 }
 
 cudaError_t eider_b200_beam_select_on_stream(const void* logits, int logits_are_bf16, size_t row_stride, const float* beam_scores,
@@ -506,14 +565,16 @@ cudaError_t eider_b200_beam_select_on_stream(const void* logits, int logits_are_
     a.vocab = vocab;
     a.k = k;
     a.pad_token = pad_token;
-    a.segments = segments_of(vocab, logits_are_bf16);
+    a.segments = segments_of(vocab);
     a.vectors_per_split = vectors_per_split(rows, vocab, logits_are_bf16);
     a.splits = splits_of(rows, vocab, logits_are_bf16);
     a.partial = static_cast<float2*>(workspace);
     a.segment_max = reinterpret_cast<float*>(a.partial + static_cast<size_t>(rows) * a.splits);
     const dim3 scan(a.splits, rows);
-    cudaError_t st = logits_are_bf16 ? launch_dependent(beam_scan_kernel<uint16_t>, scan, kScanThreads, 0, stream, a)
-                                     : launch_dependent(beam_scan_kernel<float>, scan, kScanThreads, 0, stream, a);
+    const bool shifted = ((reinterpret_cast<uintptr_t>(logits) | row_stride * (logits_are_bf16 ? 2 : 4)) & 15) != 0;
+    const auto scan_kernel = logits_are_bf16 ? (shifted ? beam_scan_shifted_kernel<uint16_t> : beam_scan_kernel<uint16_t>)
+                                             : (shifted ? beam_scan_shifted_kernel<float> : beam_scan_kernel<float>);
+    const cudaError_t st = launch_dependent(scan_kernel, scan, kScanThreads, 0, stream, a);
     if (st != cudaSuccess) return st;
     return logits_are_bf16 ? launch_dependent(beam_merge_kernel<uint16_t>, dim3(batch), kMergeThreads, sizeof(MergeShared), stream, a)
                            : launch_dependent(beam_merge_kernel<float>, dim3(batch), kMergeThreads, sizeof(MergeShared), stream, a);

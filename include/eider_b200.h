@@ -901,7 +901,8 @@ EIDER_B200_API cudaError_t eider_b200_moe_weighted_accumulate_sorted_to_bf16_on_
 /* ---- beam search (beside the lm-head arg-max above; the reference decodes one hypothesis) -------------------
  * score[r][v] = beam_scores[r] + log_softmax(logits[r])[v] for the batch x beams rows of logits (f32 or bf16, `row_stride` elements
  * apart); per sequence the k largest over its beams x vocab scores in descending order, compared in 64 bits, equal ones in the order
- * of beam * vocab + v.  A finished beam (finished may be NULL) has one candidate, pad_token, with its score unchanged.  A row
+ * of beam * vocab + v.  A row's log-sum-exp is of f32 exponentials and partial sums (within about 2^-21), the same for equal rows wherever
+ * they lie, so only candidates of different beams that are nearer than that may stand in another order than the definition's.  A finished beam (finished may be NULL) has one candidate, pad_token, with its score unchanged.  A row
  * whose beam score or log-sum-exp is not finite (a NaN or +infinity among its logits, or nothing above -infinity) has candidates of
  * score -infinity only; where fewer than k scores are finite, candidates of score -infinity follow in the order of their index.
  * beams <= 64, k <= 128 and <= beams * vocab, batch * beams <= 65535.  The workspace (8-byte aligned) is one call's. */

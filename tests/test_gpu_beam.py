@@ -192,3 +192,35 @@ def test_decode_steps_with_beams():
         scores.copy_(best[:, :beams])
         for s, o in zip(states, moved):
             s.copy_(o)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [9, 67, 4099, 9001, 50257, 131071])
+def test_equal_beams_tie_wherever_their_rows_lie(v, dtype):
+    """Rows of an odd length start at every offset from a 16-byte boundary: the same logits give the same scores there, bit for bit, so equal
+    beams come in the order of their index, and one candidate of every beam precedes the next token's."""
+    b, w, k = 2, 16, min(16 * v, 100)
+    logits, scores, g = inputs(v, b, 1, v, dtype)
+    # (one row's scores in 64 bits: sums of w copies of it need not agree to the last bit there)
+    top = logits.double().amax(-1, keepdim=True)
+    total = logits.double() - top - torch.log(torch.exp(logits.double() - top).sum(-1, keepdim=True)) + scores.double().unsqueeze(-1)
+    at = total.expand(b, w, v).reshape(b, w * v).sort(dim=1, descending=True, stable=True)[1][:, :k]
+    logits = logits.expand(b, w, v).contiguous()
+    _, parents, tokens = ops.beam_search_select(logits, scores.expand(b, w).contiguous(), k)
+    assert torch.equal(parents.long(), at // v) and torch.equal(tokens.long(), at % v)
+    got, parents, _ = ops.beam_search_select(logits, scores.expand(b, w).contiguous(), 16)
+    assert torch.equal(parents, torch.arange(16, device="cuda", dtype=torch.int32).expand(b, 16)) and (got == got[:, :1]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [1, 7, 8, 1000, 8196, 32003, 131072])
+def test_scores_do_not_depend_on_alignment(v, dtype):
+    b, w, k = 2, 3, min(3 * v, 64)
+    logits, scores, g = inputs(v, b, w, v, dtype)
+    want = ops.beam_search_select(logits, scores, k)
+    for pitch, first in ((v + 8, 0), (v + 1, 0), (v + 1, 1), (v + 5, 3), (v + 8, 7), (v + 14, 5)):
+        wide = torch.full((b, w, pitch), math.nan, device="cuda", dtype=dtype)
+        copy = wide[:, :, first: first + v]
+        copy.copy_(logits)
+        for x, y in zip(ops.beam_search_select(copy, scores, k), want):
+            assert torch.equal(x, y), (pitch, first)
