@@ -1181,9 +1181,12 @@ class GroupedMxfp4Weights:
     experts: int
     out_features: int
     in_features: int
+    gate_up_interleaved: bool = False  # rows in the order of interleave_gate_up()
 
     @staticmethod
-    def from_checkpoint(packed: torch.Tensor, scales_row_major: torch.Tensor, alpha: torch.Tensor | None = None) -> "GroupedMxfp4Weights":
+    def from_checkpoint(packed: torch.Tensor, scales_row_major: torch.Tensor, alpha: torch.Tensor | None = None,
+                        gate_up_interleaved: bool = False) -> "GroupedMxfp4Weights":
+        """`gate_up_interleaved`: the rows are in the order of interleave_gate_up() already."""
         if packed.dim() != 3 or packed.shape[1] % 32 != 0 or packed.shape[2] % 16 != 0 or packed.numel() == 0:
             raise ShapeError(f"expert weights must be [experts, out, in / 2] with out and in in multiples of 32, got {tuple(packed.shape)}")
         e, n, k = packed.shape[0], packed.shape[1], packed.shape[2] * 2
@@ -1195,7 +1198,7 @@ class GroupedMxfp4Weights:
         if alpha.shape != (e,):
             raise ShapeError("alpha must have one value per expert")
         _need_device(packed.device, scales_row_major, alpha)
-        return GroupedMxfp4Weights(_aligned16(packed), scales_row_major, _mxfp4_tiled(scales_row_major, e, n, k), alpha, e, n, k)
+        return GroupedMxfp4Weights(_aligned16(packed), scales_row_major, _mxfp4_tiled(scales_row_major, e, n, k), alpha, e, n, k, gate_up_interleaved)
 
     def interleave_gate_up(self) -> "GroupedMxfp4Weights":
         """The same gate/up weights with the rows of every expert reordered as [32 gate rows, 32 up rows] per 32 features: 64
@@ -1204,9 +1207,11 @@ class GroupedMxfp4Weights:
         n = self.out_features
         if n % 64 != 0:
             raise ShapeError("gate/up rows must come in multiples of 64")
+        if self.gate_up_interleaved:
+            raise ShapeError("the gate/up rows are interleaved already")
         order = torch.arange(n, device=self.packed.device).reshape(2, -1, 32).transpose(0, 1).reshape(-1)
         return GroupedMxfp4Weights.from_checkpoint(self.packed.index_select(1, order).contiguous(),
-                                                   self.scales_row_major.index_select(1, order).contiguous(), self.alpha)
+                                                   self.scales_row_major.index_select(1, order).contiguous(), self.alpha, gate_up_interleaved=True)
 
     @staticmethod
     def quantize(weights: torch.Tensor) -> "GroupedMxfp4Weights":
@@ -1268,6 +1273,8 @@ class Mxfp4GroupedGemmPlan(_DevicePlan):
         """Gate/up GEMM with SiLU(gate) * up -> MXFP4 in the epilogue: fills `out`, the down projection's input.  `w_interleaved` =
         GroupedMxfp4Weights.interleave_gate_up()."""
         self._operands(rows, w_interleaved, routes)
+        if not w_interleaved.gate_up_interleaved:
+            raise ShapeError("the gate/up weights must have been through interleave_gate_up()")
         if out.k * 2 != self.m or out.routes != rows.routes or out.experts != rows.experts:
             raise ShapeError("operand shapes do not match the plan")
         _need_device(self.device, out.packed)
@@ -1360,8 +1367,9 @@ class GroupedMoe:
         return moe_weighted_accumulate(self.routes, weights.reshape(-1), self.down_out, self.tokens, self.top_k, out=out)
 
     def _run_mxfp4(self, x, router_logits, w_down, norm_topk_prob, w_gate_up_interleaved, out):
-        """The same steps over MXFP4 rows; SiLU * up takes the f32 accumulators of the gate/up GEMM."""
-        if not isinstance(w_gate_up_interleaved, GroupedMxfp4Weights) or not isinstance(w_down, GroupedMxfp4Weights):
+        """The same steps over MXFP4 rows, from the interleaved gate/up weights alone; SiLU * up takes the f32 accumulators of the gate/up GEMM."""
+        if (not isinstance(w_gate_up_interleaved, GroupedMxfp4Weights) or not isinstance(w_down, GroupedMxfp4Weights) or
+                not w_gate_up_interleaved.gate_up_interleaved or w_down.gate_up_interleaved):
             raise ShapeError("an MXFP4 layer takes GroupedMxfp4Weights, the gate/up weights through interleave_gate_up()")
         if router_logits.shape != (self.tokens, self.experts) or x.shape != (self.tokens, self.hidden):
             raise ShapeError("x must be [tokens, hidden] and router_logits [tokens, experts]")

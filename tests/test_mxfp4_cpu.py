@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from eider_b200 import _lib, ops
+from tests import fakes
 
 INVALID = 1
 SOME = 0x1000  # an aligned address that nothing reads
@@ -84,3 +85,34 @@ def test_python_layer_refuses_host_tensors_and_odd_shapes():
         ops.MoeSortedMxfp4Rows(4, 2, 48, device="cpu")
     with pytest.raises(ops.ShapeError):
         ops.GroupedMoe(4, 2, 1, 64, 32, device="cpu", weight_format="mxfp6")
+
+
+def test_gate_up_weights_know_their_order(monkeypatch):
+    """Weights that have not been through interleave_gate_up() have the class and shape of those that have, and would give another layer."""
+    called = fakes.without_a_device(monkeypatch)
+    u8 = torch.uint8
+    gate_up = ops.GroupedMxfp4Weights.from_checkpoint(torch.zeros(2, 128, 32, dtype=u8), torch.zeros(2, 128, 2, dtype=u8))
+    down = ops.GroupedMxfp4Weights.from_checkpoint(torch.zeros(2, 64, 32, dtype=u8), torch.zeros(2, 64, 2, dtype=u8))
+    interleaved = gate_up.interleave_gate_up()
+    assert not gate_up.gate_up_interleaved and interleaved.gate_up_interleaved
+    assert ops.GroupedMxfp4Weights.from_checkpoint(interleaved.packed, interleaved.scales_row_major, gate_up_interleaved=True).gate_up_interleaved
+    with pytest.raises(ops.ShapeError):
+        interleaved.interleave_gate_up()
+
+    plan = object.__new__(ops.Mxfp4GroupedGemmPlan)
+    plan._plan, plan.m, plan.max_n, plan.k, plan.groups, plan.device = None, 128, 4, 64, 2, torch.device("cpu")
+    rows, out, routes = ops.MoeSortedMxfp4Rows(4, 2, 64, "cpu"), ops.MoeSortedMxfp4Rows(4, 2, 64, "cpu"), ops.MoeSortedRoutes(4, 2, "cpu")
+    called.clear()
+    with pytest.raises(ops.ShapeError):
+        plan.run_silu_quantize(rows, gate_up, routes, out)
+    assert not called
+    plan.run_silu_quantize(rows, interleaved, routes, out)
+    assert called == ["eider_b200_mxfp4_grouped_gemm_silu_quantize_on_stream"]
+
+    moe = object.__new__(ops.GroupedMoe)
+    moe.weight_format, moe.tokens, moe.experts, moe.hidden, moe.out = "mxfp4", 4, 2, 64, torch.zeros(4, 64)
+    called.clear()
+    for w_gate_up, w_down in ((gate_up, down), (None, down), (interleaved, interleaved)):
+        with pytest.raises(ops.ShapeError):
+            moe.run(torch.zeros(4, 64), torch.zeros(4, 2), gate_up, w_down, w_gate_up_interleaved=w_gate_up)
+    assert not called
