@@ -186,6 +186,7 @@ SIGNATURES = {
     "eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream": (_I, [_P, _P, _P, _P, _P, _F, _P, _P, _P]),
     "eider_b200_mxfp4_decode_create": (_P, [_U32, _U32, _U32]),
     "eider_b200_mxfp4_decode_destroy": (None, [_P]),
+    "eider_b200_mxfp4_decode_status": (_I, [_P, _P]),
     "eider_b200_mxfp4_w4a16_workspace_bytes": (_SZ, [_U32, _U32, _I]),
     "eider_b200_mxfp4_w4a16_gemv_on_stream": (_I, [_P, _P, _I, _U32, _P, _P, _U32, _P, _P, _P, _F, _I, _P, _SZ, _P]),
     "eider_b200_moe_quantize_routes_mxfp4_on_stream": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _P]),

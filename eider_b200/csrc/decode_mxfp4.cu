@@ -444,6 +444,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode
 
 struct Plan {
     uint32_t max_tokens, n, k;
+    uint32_t* status;
     gemm::FifoCache<CUtensorMap> maps;
 };
 
@@ -524,10 +525,31 @@ extern "C" {
 
 void* eider_b200_mxfp4_decode_create(uint32_t max_tokens, uint32_t out_features, uint32_t in_features) {
     if (max_tokens == 0 || max_tokens > 64 || out_features == 0 || in_features == 0 || in_features % mx::kBlock != 0 || in_features > 65536) return nullptr;
-    return new (std::nothrow) decode_mx::Plan{max_tokens, out_features, in_features, {}};
+    auto* plan = new (std::nothrow) decode_mx::Plan{max_tokens, out_features, in_features, nullptr, {}};
+    if (!plan) return nullptr;
+    if (cudaMalloc(reinterpret_cast<void**>(&plan->status), sizeof(uint32_t)) != cudaSuccess) {
+        delete plan;
+        return nullptr;
+    }
+    if (cudaMemset(plan->status, 0, sizeof(uint32_t)) != cudaSuccess) {
+        eider_b200_mxfp4_decode_destroy(plan);
+        return nullptr;
+    }
+    return plan;
 }
 
-void eider_b200_mxfp4_decode_destroy(void* raw) { delete static_cast<decode_mx::Plan*>(raw); }
+void eider_b200_mxfp4_decode_destroy(void* raw) {
+    auto* plan = static_cast<decode_mx::Plan*>(raw);
+    if (!plan) return;
+    cudaFree(plan->status);
+    delete plan;
+}
+
+cudaError_t eider_b200_mxfp4_decode_status(void* raw, uint32_t* host_status) {
+    auto* plan = static_cast<decode_mx::Plan*>(raw);
+    if (!plan || !host_status) return cudaErrorInvalidValue;
+    return cudaMemcpy(host_status, plan->status, sizeof(uint32_t), cudaMemcpyDeviceToHost);
+}
 
 size_t eider_b200_mxfp4_w4a16_workspace_bytes(uint32_t tokens, uint32_t in_features, int input_is_bf16) {
     const size_t few = decode_mx::back_bytes(tokens) + static_cast<size_t>(tokens) * in_features * (input_is_bf16 ? 2 : 4);
@@ -547,7 +569,7 @@ cudaError_t eider_b200_mxfp4_w4a16_gemv_on_stream(void* raw, const void* input, 
         return cudaErrorInvalidValue;
     if (takes_terms(tokens, plan->n, plan->k, input_is_bf16) && (reinterpret_cast<uintptr_t>(w_values) & 31) == 0)
         return run_terms(plan->maps, input, input_is_bf16, tokens, w_values, w_scales_tiled, c, d, beta, out_is_bf16, plan->n, plan->k,
-                         static_cast<uint8_t*>(workspace), stream);
+                         static_cast<uint8_t*>(workspace), plan->status, stream);
     float* back = static_cast<float*>(workspace);
     uint16_t* prepared = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + back_bytes(tokens));
     cudaError_t st = input_is_bf16 ? prepare<uint16_t>(input, prepared, back, tokens, plan->k, stream)

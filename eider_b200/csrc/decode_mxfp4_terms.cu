@@ -59,6 +59,7 @@ struct Params {
     float beta;
     int out_is_bf16, x_is_bf16;
     uint32_t tokens, padded, terms, columns, n, k, stages, tmem_columns;
+    uint32_t* status;  // of a wait that ran out
 };
 
 __device__ __forceinline__ float lds_cluster(uint32_t address) {
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
             const uint64_t once = umma::policy_evict_first();
             uint32_t slot = 0, phase = 1;
             for (uint32_t i = 0; i < steps; ++i) {
-                if (!umma::mbar_wait(empty + slot, phase, &abort_flag, nullptr, umma::kTimeoutEmpty)) break;
+                if (!umma::mbar_wait(empty + slot, phase, &abort_flag, p.status, umma::kTimeoutEmpty)) break;
                 uint8_t* to = smem + slot * stage;
                 if (weights) {
                     umma::mbar_arrive_expect_tx(full + slot, kTileBytes / 2 + kScaleTile);  // (the barrier counts the bytes read, not those spread)
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
             const uint32_t wide = (p.columns + 15) / 16 * 16;  // (what lies behind x goes to columns that nobody reads)
             uint32_t slot = 0, phase = 0;
             for (uint32_t i = 0; i < steps; ++i) {
-                if (!umma::mbar_wait(full + slot, phase, &abort_flag, nullptr, umma::kTimeoutFull)) break;
+                if (!umma::mbar_wait(full + slot, phase, &abort_flag, p.status, umma::kTimeoutFull)) break;
                 umma::tc_fence_after();
                 const uint32_t at = umma::smem_u32(smem) + slot * stage;
                 // scale columns are a slot's own: its MMAs are done before it is filled again
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
 
     // ------------------------------------------------------------------------------------------ the cluster's sums meet
     float* sums = reinterpret_cast<float*>(smem);  // [tokens][kSumPitch]: the ring is done with
-    bool good = umma::mbar_wait(&done, 0, &abort_flag, nullptr, umma::kTimeoutTmemFull);
+    bool good = umma::mbar_wait(&done, 0, &abort_flag, p.status, umma::kTimeoutTmemFull);
     good = __all_sync(kFull, good && abort_flag == 0);
     umma::tc_fence_after();
     for (uint32_t c = 0; c < p.padded; c += 8) {
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
         }
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i)
-            if (c + i < p.tokens) sums[(c + i) * kSumPitch + warp * 32 + lane] = good ? v[i] : NAN;  // (a wait ran out: no result)
+            if (c + i < p.tokens) sums[(c + i) * kSumPitch + warp * 32 + lane] = good ? v[i] : NAN;  // (a wait ran out: no result, and the plan's status says so)
     }
     umma::tc_fence_before();
     __syncthreads();
@@ -350,7 +351,8 @@ size_t terms_workspace_bytes(uint32_t tokens, uint32_t k, int input_is_bf16) {
 }
 
 cudaError_t run_terms(gemm::FifoCache<CUtensorMap>& maps, const void* x, int input_is_bf16, uint32_t tokens, const uint8_t* w, const uint8_t* scales,
-                      const void* c, void* d, float beta, int out_is_bf16, uint32_t n, uint32_t k, uint8_t* workspace, cudaStream_t stream) {
+                      const void* c, void* d, float beta, int out_is_bf16, uint32_t n, uint32_t k, uint8_t* workspace, uint32_t* status,
+                      cudaStream_t stream) {
     const CUtensorMap* map = nullptr;
     cudaError_t st = maps.get(&map, gemm::MapKey{w, n, k, k / 2, kRows}, [&](CUtensorMap* to) { return gemm::make_spread_fp4_map(to, w, n, k, kRows); });
     if (st != cudaSuccess) return st;
@@ -380,6 +382,7 @@ cudaError_t run_terms(gemm::FifoCache<CUtensorMap>& maps, const void* x, int inp
         p.beta = beta;
         p.out_is_bf16 = out_is_bf16;
         p.x_is_bf16 = input_is_bf16;
+        p.status = status;
         p.tokens = std::min(each, tokens - first);
         p.padded = padded_of(p.tokens);
         p.terms = terms_of(input_is_bf16);

@@ -640,6 +640,11 @@ class Mxfp4DecodePlan(_DevicePlan):
               workspace.data_ptr(), size)
         return out
 
+    def status(self) -> int:
+        v = C.c_uint32(0)
+        check("eider_b200_mxfp4_decode_status", self._lib.eider_b200_mxfp4_decode_status(self._plan, C.byref(v)))
+        return v.value
+
 
 # ---- FP8 quantizers ---------------------------------------------------------------------------------
 def quantize_fp8_dynamic(x: torch.Tensor):

@@ -425,3 +425,14 @@ def test_combine_refuses_a_bf16_output_of_another_shape():
     weights = torch.zeros(4, 2, device="cuda")
     with pytest.raises(ops.ShapeError):
         ops.moe_weighted_accumulate(None, weights, rows, 4, 2, out=torch.zeros(3, 64, device="cuda", dtype=torch.bfloat16))
+
+
+def test_decode_plans_report_their_status():
+    """Poisoned activations give NaN with a status of 0: only a wait that ran out sets it."""
+    g = gen(23)
+    for tokens, k in ((1, 96), (9, 512)):  # one of each form
+        plan, w = ops.Mxfp4DecodePlan(16, 200, k), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, 200, k))
+        assert plan.status() == 0
+        x = randn(g, tokens, k)
+        x[0, 3] = float("nan")
+        assert torch.isnan(plan.run(x, w)[0]).all() and plan.status() == 0

@@ -116,3 +116,9 @@ def test_gate_up_weights_know_their_order(monkeypatch):
         with pytest.raises(ops.ShapeError):
             moe.run(torch.zeros(4, 64), torch.zeros(4, 2), gate_up, w_down, w_gate_up_interleaved=w_gate_up)
     assert not called
+
+
+def test_decode_status_refuses():
+    import ctypes as C
+    lib = _lib.load()
+    assert lib.eider_b200_mxfp4_decode_status(None, C.byref(C.c_uint32(0))) == INVALID and lib.eider_b200_mxfp4_decode_status(SOME, None) == INVALID
