@@ -52,7 +52,7 @@ struct Params {
 
 template <typename XT> __device__ __forceinline__ void load8(const XT* p, float (&v)[8]);
 template <> __device__ __forceinline__ void load8<uint16_t>(const uint16_t* p, float (&v)[8]) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 u = __ldca(reinterpret_cast<const uint4*>(p));
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -61,7 +61,7 @@ template <> __device__ __forceinline__ void load8<uint16_t>(const uint16_t* p, f
     }
 }
 template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float4 a = __ldca(reinterpret_cast<const float4*>(p)), b = __ldca(reinterpret_cast<const float4*>(p) + 1);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_quantized_kernel(const
             const float rs = p.alpha * ((p.channel_scale && row_ok) ? p.channel_scale[row] : 1.0f);
             auto emit = [&](uint32_t m, float sum) {
                 const size_t index = static_cast<size_t>(m) * p.ld_out + row;
-                const float v = sum * __ldg(p.x_scale + m) * rs;
+                const float v = sum * __ldca(p.x_scale + m) * rs;
                 if (p.out_is_bf16) static_cast<uint16_t*>(p.out)[index] = float_to_bf16_bits(v);
                 else static_cast<float*>(p.out)[index] = v;
             };
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(256) splitk_reduce_kernel(const Params p) {
 #pragma unroll
         for (uint32_t u = 0; u < 8; ++u) sum += part[u];
     }
-    const float v = sum * __ldg(p.x_scale + m) * p.alpha * (p.channel_scale ? p.channel_scale[row] : 1.0f);
+    const float v = sum * __ldca(p.x_scale + m) * p.alpha * (p.channel_scale ? p.channel_scale[row] : 1.0f);
     const size_t index = static_cast<size_t>(m) * p.ld_out + row;
     if (p.out_is_bf16) static_cast<uint16_t*>(p.out)[index] = float_to_bf16_bits(v);
     else static_cast<float*>(p.out)[index] = v;

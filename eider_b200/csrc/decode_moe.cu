@@ -274,7 +274,7 @@ __device__ __forceinline__ void warp_select(const MoeStepArgs& a, StepRouting& r
     const int lowest = order_key(-INFINITY);
     int key[PER_LANE];
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) key[i] = lane + 32 * i < a.experts ? order_key(router_logit(__ldg(a.logits + lane + 32 * i))) : lowest;
+    for (int i = 0; i < PER_LANE; ++i) key[i] = lane + 32 * i < a.experts ? order_key(router_logit(__ldca(a.logits + lane + 32 * i))) : lowest;
     uint32_t expert = 0;
     float logit = -INFINITY;
     for (uint32_t slot = 0; slot < a.top_k; ++slot) {
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kStepThreads, 4) moe_step_gate_up_kernel(const
         select_experts(a, routing);
     } else {
         for (uint32_t i = threadIdx.x - 32; i < a.hidden / 8; i += kStepThreads - 32) {
-            const float4 lo = __ldg(reinterpret_cast<const float4*>(a.x) + 2 * i), hi = __ldg(reinterpret_cast<const float4*>(a.x) + 2 * i + 1);
+            const float4 lo = __ldca(reinterpret_cast<const float4*>(a.x) + 2 * i), hi = __ldca(reinterpret_cast<const float4*>(a.x) + 2 * i + 1);
             uint32_t t[4][3];
             bf16_terms(lo.x, hi.x, t[0]);
             bf16_terms(lo.y, hi.y, t[1]);

@@ -69,7 +69,7 @@ struct Params {
 
 template <typename XT> __device__ __forceinline__ void load8(const XT* p, float (&v)[8]);
 template <> __device__ __forceinline__ void load8<uint16_t>(const uint16_t* p, float (&v)[8]) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 u = __ldca(reinterpret_cast<const uint4*>(p));
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -80,7 +80,7 @@ template <> __device__ __forceinline__ void load8<uint16_t>(const uint16_t* p, f
 template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(p) + h);
+        const float4 f = __ldca(reinterpret_cast<const float4*>(p) + h);
         v[4 * h] = f.x; v[4 * h + 1] = f.y; v[4 * h + 2] = f.z; v[4 * h + 3] = f.w;
     }
 }
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(PREPARED ? 192 : 64 + kMaxExpandThreads, PREPA
         umma::griddep_wait();  // x may be the previous kernel's output; scratch, counters and the output are shared with it
         if constexpr (PREPARED) {
             // (the producer warp requests the operand stages; the epilogue only needs the row scales)
-            if (te < COLS) col_scale[te] = __ldg(p.x_col_scale + te);
+            if (te < COLS) col_scale[te] = __ldca(p.x_col_scale + te);
             asm volatile("bar.sync 1, %0;" ::"r"(p.expand_threads) : "memory");
         } else {
         // (operand tiles were cleared before the setup barrier: rows past tokens * TERMS and the K tail stay zero)

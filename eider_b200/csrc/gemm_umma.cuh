@@ -282,7 +282,7 @@ __device__ __forceinline__ void convert_bf16x64_scaled(const uint32_t* raw, floa
     if (col_scale) {
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-            const float4 c = __ldg(reinterpret_cast<const float4*>(col_scale) + q);
+            const float4 c = __ldca(reinterpret_cast<const float4*>(col_scale) + q);
             __nv_bfloat162 h0 = __floats2bfloat162_rn(__uint_as_float(raw[4 * q]) * scale * c.x, __uint_as_float(raw[4 * q + 1]) * scale * c.y);
             __nv_bfloat162 h1 = __floats2bfloat162_rn(__uint_as_float(raw[4 * q + 2]) * scale * c.z, __uint_as_float(raw[4 * q + 3]) * scale * c.w);
             w[2 * q] = *reinterpret_cast<uint32_t*>(&h0);
@@ -361,7 +361,7 @@ __device__ __forceinline__ void store_row64(const Params& p, size_t offset, uint
         if (col_scale) {
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
-                const float4 c = __ldg(reinterpret_cast<const float4*>(col_scale + 16 * g) + i);
+                const float4 c = __ldca(reinterpret_cast<const float4*>(col_scale + 16 * g) + i);
                 x[4 * i] *= c.x; x[4 * i + 1] *= c.y; x[4 * i + 2] *= c.z; x[4 * i + 3] *= c.w;
             }
         }

@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(1024) moe_sort_one_cta_kernel(const uint32_t* 
 
 // non_gemm.cu:2554-2557: one spare 128-row scale tile per expert around the sorted prefix
 __device__ __forceinline__ size_t moe_scale_base(uint32_t expert, const uint32_t* offsets, uint32_t tile_bytes) {
-    return ((static_cast<size_t>(offsets[expert]) + 127) / 128 + expert) * tile_bytes;
+    return ((static_cast<size_t>(__ldca(offsets + expert)) + 127) / 128 + expert) * tile_bytes;
 }
 
 // Scatter already quantized token rows into expert-major order (second half of non_gemm.cu:2899-2998).  One warp per
@@ -485,8 +485,8 @@ __global__ void __launch_bounds__(256) moe_silu_mul_quantize_kernel(const uint16
     }
     *reinterpret_cast<uint32_t*>(packed + static_cast<size_t>(sorted) * (k / 2) + h * 4) = w;
     if ((h & 1) == 0) {
-        const uint32_t expert = sorted_experts[sorted];
-        scales[moe_scale_base(expert, offsets, tile_bytes) + tiled_scale_offset(sorted - offsets[expert], h >> 1, k)] = sc;
+        const uint32_t expert = __ldca(sorted_experts + sorted);
+        scales[moe_scale_base(expert, offsets, tile_bytes) + tiled_scale_offset(sorted - __ldca(offsets + expert), h >> 1, k)] = sc;
     }
 }
 

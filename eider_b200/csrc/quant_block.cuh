@@ -61,8 +61,8 @@ template <typename T> struct Block16;
 template <> struct Block16<uint16_t> {
     uint4 q[2];
     __device__ __forceinline__ void load(const uint16_t* p) {
-        q[0] = __ldg(reinterpret_cast<const uint4*>(p));
-        q[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+        q[0] = __ldca(reinterpret_cast<const uint4*>(p));
+        q[1] = __ldca(reinterpret_cast<const uint4*>(p) + 1);
     }
     __device__ __forceinline__ uint32_t word(int j) const {
         const uint4& w = q[j / 4];
@@ -91,7 +91,7 @@ template <> struct Block16<float> {
     float4 q[4];
     __device__ __forceinline__ void load(const float* p) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = __ldg(reinterpret_cast<const float4*>(p) + j);
+        for (int j = 0; j < 4; ++j) q[j] = __ldca(reinterpret_cast<const float4*>(p) + j);
     }
     __device__ __forceinline__ float get(int i) const {
         const float4& f = q[i / 4];
@@ -160,7 +160,9 @@ __device__ __forceinline__ void zero_padding_rows(uint8_t* scales, uint32_t rows
     }
 }
 
-// A kernel that starts with griddepcontrol.wait, launched so that its prologue overlaps the kernel before it.
+// A kernel that starts with griddepcontrol.wait, launched so that its prologue overlaps the kernel before it.  What that kernel wrote is
+// read with __ldca or __ldcg, never with __ldg: to the compiler a read-only load has no order with the wait, and the old value may be
+// requested in front of it (264 of 3200 calls of a decode kernel).
 template <typename Kernel, typename... Args>
 cudaError_t launch_dependent(Kernel kernel, dim3 grid, uint32_t threads, size_t smem, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};

@@ -23,18 +23,18 @@ template <> struct Loader<float> {
         const float4* q = reinterpret_cast<const float4*>(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float4 f = __ldg(q + i);
+            float4 f = __ldca(q + i);
             v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
         }
     }
-    static __device__ __forceinline__ float load1(const float* p) { return __ldg(p); }
+    static __device__ __forceinline__ float load1(const float* p) { return __ldca(p); }
 };
 template <> struct Loader<uint16_t> {
     static __device__ __forceinline__ void load16(const uint16_t* p, float (&v)[16]) {
         const uint4* q = reinterpret_cast<const uint4*>(p);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            uint4 u = __ldg(q + i);
+            uint4 u = __ldca(q + i);
             uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -43,7 +43,7 @@ template <> struct Loader<uint16_t> {
             }
         }
     }
-    static __device__ __forceinline__ float load1(const uint16_t* p) { return bf16_bits_to_float(__ldg(p)); }
+    static __device__ __forceinline__ float load1(const uint16_t* p) { return bf16_bits_to_float(__ldca(p)); }
 };
 
 template <typename T>
@@ -77,14 +77,14 @@ enum ScaleMode { kStatic = 0, kPerRow = 1 };
 template <typename T> struct Half8;
 template <> struct Half8<float> {
     static __device__ __forceinline__ void load(const float* p, float (&v)[8]) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-        const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        const float4 a = __ldca(reinterpret_cast<const float4*>(p));
+        const float4 b = __ldca(reinterpret_cast<const float4*>(p) + 1);
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     }
 };
 template <> struct Half8<uint16_t> {
     static __device__ __forceinline__ void load(const uint16_t* p, float (&v)[8]) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint4 u = __ldca(reinterpret_cast<const uint4*>(p));
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -550,8 +550,8 @@ __global__ void __launch_bounds__(256) silu_mul_quantize_nvfp4_kernel(const floa
     float v[16];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        const float4 g4 = __ldg(reinterpret_cast<const float4*>(gate) + q);
-        const float4 u4 = __ldg(reinterpret_cast<const float4*>(up) + q);
+        const float4 g4 = __ldca(reinterpret_cast<const float4*>(gate) + q);
+        const float4 u4 = __ldca(reinterpret_cast<const float4*>(up) + q);
         const float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -590,8 +590,8 @@ __global__ void __launch_bounds__(256) rms_norm_quantize_nvfp4_kernel(const floa
         float v[16];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float4 x4 = __ldg(reinterpret_cast<const float4*>(x + b * 16) + q);
-            const float4 w4 = __ldg(reinterpret_cast<const float4*>(weight + b * 16) + q);
+            const float4 x4 = __ldca(reinterpret_cast<const float4*>(x + b * 16) + q);
+            const float4 w4 = __ldca(reinterpret_cast<const float4*>(weight + b * 16) + q);
             v[4 * q + 0] = div_rn(rowops::normed(x4.x, inv, w4.x), di);
             v[4 * q + 1] = div_rn(rowops::normed(x4.y, inv, w4.y), di);
             v[4 * q + 2] = div_rn(rowops::normed(x4.z, inv, w4.z), di);
@@ -632,9 +632,9 @@ __global__ void __launch_bounds__(256) rms_norm_add_rms_norm_quantize_nvfp4_kern
     const float inv0 = rowops::inverse_rms(rowops::block_sum_ordered(rowops::thread_sum_squares_f4(input + off, cols), red), cols, input_eps);
     float ss2 = 0.0f;
     for (uint32_t i = threadIdx.x; i < cols / 4; i += blockDim.x) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(input + off) + i);
-        const float4 w = __ldg(reinterpret_cast<const float4*>(input_weight) + i);
-        const float4 r = __ldg(reinterpret_cast<const float4*>(residual + off) + i);
+        const float4 v = __ldca(reinterpret_cast<const float4*>(input + off) + i);
+        const float4 w = __ldca(reinterpret_cast<const float4*>(input_weight) + i);
+        const float4 r = __ldca(reinterpret_cast<const float4*>(residual + off) + i);
         float4 h;
         h.x = rowops::normed_add(v.x, inv0, w.x, r.x);
         h.y = rowops::normed_add(v.y, inv0, w.y, r.y);
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(256) rms_norm_add_rms_norm_quantize_nvfp4_kern
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float4 h4 = reinterpret_cast<const float4*>(staged + b * 16)[q];
-            const float4 w4 = __ldg(reinterpret_cast<const float4*>(quant_weight + b * 16) + q);
+            const float4 w4 = __ldca(reinterpret_cast<const float4*>(quant_weight + b * 16) + q);
             v[4 * q + 0] = div_rn(rowops::normed(h4.x, inv1, w4.x), di);
             v[4 * q + 1] = div_rn(rowops::normed(h4.y, inv1, w4.y), di);
             v[4 * q + 2] = div_rn(rowops::normed(h4.z, inv1, w4.z), di);
