@@ -7,7 +7,7 @@
 //    wait for each other.  Scales and the first steps are requested before the launch in front is awaited; three CTAs an SM have
 //    up to 190 KB on their way.
 //  * 16 rows x 32 elements (a block) at a time go through mma.m16n8k16 with the tokens as the eight columns.  E2M1 codes become f16 by
-//    one conversion per pair (exact), the sum of a block (two MMAs) is taken in f32 and then added times its block scale in f32, so
+//    one conversion per pair (exact), the sum of a block (two MMAs) is taken in f32 and then added times its two block scales in f32, so
 //    the weights are never multiplied out and no MMA chain is longer than a block.
 //  * x is made f16 by a launch of its own (prepare_mxfp4_kernel), which runs while the weights are on their way.  Made in the loop, with a
 //    maximum, two shuffles and a vote a step in front of the MMAs, the product took 13.2 us for one token and 16.6 for eight
@@ -20,6 +20,7 @@
 #include "gemm_launch.cuh"
 #include "decode_mxfp4.cuh"
 #include "mx_block.cuh"
+#include "quant_block.cuh"
 #include "eider_b200.h"
 
 namespace eider {
@@ -34,15 +35,15 @@ __host__ __device__ constexpr uint32_t ctas_per_sm(int operands) { return operan
 constexpr uint32_t kFull = 0xffffffffu;
 
 struct Params {
-    const uint16_t* x;      // prepared: f16 [tokens * terms][k]
-    const float* back;      // [tokens]: what a token's sums are multiplied by
-    const uint8_t* w;       // [n][k / 2]
-    const uint8_t* scales;  // [n][pitch]
+    const uint16_t* x;         // prepared: f16 [tokens * terms][k]
+    const uint32_t* x_scales;  // [steps][x_scale_tokens]: a step's four scale bytes, of this launch's tokens
+    const uint8_t* w;          // [n][k / 2]
+    const uint8_t* scales;     // [n][pitch]
     void* out;
     const void* c;
     float beta;
     int out_is_bf16;
-    uint32_t tokens, n, k, pitch, depth;
+    uint32_t tokens, n, k, pitch, depth, x_scale_tokens;
 };
 
 __host__ __device__ constexpr uint32_t reduce_pitch(uint32_t tiles) { return tiles * 16 + 4; }  // (rows of a token; + 4: the fragments' stores meet no bank twice)
@@ -110,6 +111,11 @@ __device__ __forceinline__ uint32_t lds32(uint32_t address) {
 template <int I> __device__ __forceinline__ float scale_of(uint32_t word) {
     const uint32_t field = (I < 3 ? word << (23 - 8 * I) : word >> 1) & 0x7f800000u;
     return __uint_as_float(max(field, 0x00400000u));
+}
+
+// ... of an activation's byte, which is 1 to 240
+template <int I> __device__ __forceinline__ float x_scale_of(uint32_t word) {
+    return __uint_as_float((I < 3 ? word << (23 - 8 * I) : word >> 1) & 0x7f800000u);
 }
 
 template <int N, typename F> __device__ __forceinline__ void static_for(F f) {
@@ -192,61 +198,41 @@ template <> struct Raw8<float> {
     }
 };
 
-// x as f16: every token times the power of two that brings its largest finite element to 2^14..2^15 (bf16's eight bits fit, f32 goes as
-// two terms, row 2 * token and the next), and the inverse.  What is lost lies 2^-38 below the largest element.  One CTA per token.
-constexpr uint32_t kPrepareThreads = 512;
-constexpr uint32_t kHeld = 4;  // groups of eight elements that a thread keeps between the two passes: rows up to 16384
+// x as f16: every block of 32 times the power of two that brings its largest finite element to 2^14..2^15 (bf16's eight bits fit, f32 goes
+// as two terms, row 2 * token and the next), and the inverse as a scale byte.  bf16 elements keep all their bits within 2^31 of the largest
+// of their block, and 2^-39 of that one else.  Sixteen lanes a step of 128 elements, whose four scale bytes are a word, 1 behind the blocks.
+constexpr uint32_t kPrepareThreads = 256;
 template <typename XT>
-__global__ void __launch_bounds__(kPrepareThreads) prepare_mxfp4_kernel(const XT* __restrict__ x, uint16_t* __restrict__ prepared, float* __restrict__ back,
-                                                                        uint32_t k) {
+__global__ void __launch_bounds__(kPrepareThreads) prepare_mxfp4_kernel(const XT* __restrict__ x, uint16_t* __restrict__ prepared, uint32_t* __restrict__ x_scales,
+                                                                        uint32_t k, uint32_t steps, uint32_t x_scale_tokens) {
     constexpr uint32_t kTerms = sizeof(XT) == 4 ? 2 : 1;
-    __shared__ uint32_t largest;
     umma::griddep_launch_dependents();
-    if (threadIdx.x == 0) largest = 0;
-    __syncthreads();
+    const uint32_t token = blockIdx.y, lane16 = threadIdx.x % 16, step = blockIdx.x * (kPrepareThreads / 16) + threadIdx.x / 16;
+    const uint32_t at = step * 128 + lane16 * 8;
     umma::griddep_wait();
-    const XT* row = x + static_cast<size_t>(blockIdx.x) * k;
-    const uint32_t groups = k / 8;
-    Raw8<XT> held[kHeld];
-    float amax = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < kHeld; ++i) held[i].load(row + (threadIdx.x + i * kPrepareThreads) * 8, threadIdx.x + i * kPrepareThreads < groups);
-#pragma unroll
-    for (uint32_t i = 0; i < kHeld; ++i) amax = fmaxf(amax, held[i].finite());
-    for (uint32_t q = threadIdx.x + kHeld * kPrepareThreads; q < groups; q += kPrepareThreads) {
-        Raw8<XT> r;
-        r.load(row + q * 8, true);
-        amax = fmaxf(amax, r.finite());
-    }
-    const uint32_t warp_max = __reduce_max_sync(kFull, __float_as_uint(amax));
-    if (threadIdx.x % 32 == 0) atomicMax(&largest, warp_max);
-    __syncthreads();
-    const uint32_t e = largest >> 23;
-    // 2^(14 - floor(log2 amax)), and its inverse (2^-127 is subnormal); an all-zero row keeps 1
-    const uint32_t field = largest == 0 ? 127u : min(254u, 268u - e);
-    const float factor = __uint_as_float(field << 23);
-    if (threadIdx.x == 0) back[blockIdx.x] = __uint_as_float(field == 254 ? 0x00400000u : (254u - field) << 23);
-    uint16_t* out = prepared + static_cast<size_t>(blockIdx.x) * kTerms * k;
-    auto store = [&](const Raw8<XT>& r, uint32_t q) {
+    Raw8<XT> v;
+    v.load(x + static_cast<size_t>(token) * k + at, at < k);
+    uint32_t largest = __float_as_uint(v.finite());
+    largest = max(largest, __shfl_xor_sync(kFull, largest, 1));
+    largest = max(largest, __shfl_xor_sync(kFull, largest, 2));
+    // 2^(14 - floor(log2 amax)), at most 2^126, and its inverse's byte, 1 at least; an all-zero block keeps 1
+    const uint32_t field = largest == 0 ? 127u : min(253u, 268u - (largest >> 23));
+    uint32_t word = (at < k ? 254u - field : 1u) << (lane16 / 4 * 8);
+    word |= __shfl_xor_sync(kFull, word, 4);
+    word |= __shfl_xor_sync(kFull, word, 8);
+    if (lane16 == 0 && step < steps) x_scales[step * x_scale_tokens + token] = word;
+    if (at < k) {
         uint32_t t[kTerms][4];
-        r.terms(factor, t);
+        v.terms(__uint_as_float(field << 23), t);
+        uint16_t* out = prepared + static_cast<size_t>(token) * kTerms * k + at;
 #pragma unroll
-        for (uint32_t i = 0; i < kTerms; ++i) reinterpret_cast<uint4*>(out + i * k)[q] = make_uint4(t[i][0], t[i][1], t[i][2], t[i][3]);
-    };
-#pragma unroll
-    for (uint32_t i = 0; i < kHeld; ++i)
-        if (threadIdx.x + i * kPrepareThreads < groups) store(held[i], threadIdx.x + i * kPrepareThreads);
-    for (uint32_t q = threadIdx.x + kHeld * kPrepareThreads; q < groups; q += kPrepareThreads) {
-        Raw8<XT> r;
-        r.load(row + q * 8, true);
-        store(r, q);
+        for (uint32_t i = 0; i < kTerms; ++i) *reinterpret_cast<uint4*>(out + i * k) = make_uint4(t[i][0], t[i][1], t[i][2], t[i][3]);
     }
 }
 
-// A result whose sum came out infinite or NaN, added up again block by block with x in its own size: sums of x brought to 2^14 overflow
-// before the result does, and a NaN scale counts as an infinity in the loop.
+// A result whose sum came out infinite or NaN, added up again block by block with one scaling a block: the product of an activation's and a
+// weight's scale overflows where what it is multiplied by is small, and a NaN scale counts as an infinity in the loop.
 __device__ __noinline__ float add_again(const Params& p, uint32_t terms, uint32_t token, uint32_t row, const uint8_t* scales) {
-    const float back = __ldcg(p.back + token);
     float sum = 0.0f;
     for (uint32_t block = 0; block < p.k / mx::kBlock; ++block) {
         if (scales[block] == mx::kNanCode) return NAN;
@@ -258,7 +244,8 @@ __device__ __noinline__ float add_again(const Params& p, uint32_t terms, uint32_
             const float w = m < 4 ? 0.5f * m : m == 7 ? 6.0f : m - 2.0f;
             part = fmaf(x, code & 8 ? -w : w, part);
         }
-        sum += part * back * scale_of<0>(scales[block]);
+        const uint32_t x_scale = __ldcg(p.x_scales + block / kStepBlocks * p.x_scale_tokens + token) >> (block % kStepBlocks * 8) & 255;
+        sum += ldexpf(part, static_cast<int>(x_scale + scales[block]) - 254);
     }
     return sum;
 }
@@ -316,13 +303,11 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode
         live[c] = column / kSpan < p.tokens;
         x[c] = p.x + (live[c] ? static_cast<size_t>(TERMS == 2 ? 2 * column : column / SPREAD) * p.k : 0) + sub * mx::kBlock + t * 8;
     }
-    float acc[TILES][COLS][4];
+    f32x2 acc[TILES][COLS][2];
 #pragma unroll
     for (int u = 0; u < TILES; ++u)
 #pragma unroll
-        for (int c = 0; c < COLS; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[u][c][i] = 0.0f;
+        for (int c = 0; c < COLS; ++c) acc[u][c][0] = acc[u][c][1] = pack2(0.0f, 0.0f);
     const uint32_t scale_row = umma::smem_u32(scales) + g * p.pitch;
 
     // x of a step's group of blocks; a group's registers are refilled for the warp's next step as soon as its MMAs are out, unless
@@ -336,9 +321,28 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode
             for (int k = 0; k < TERMS; ++k)
                 to[c][k] = live[c] && block + sub < blocks ? __ldca(reinterpret_cast<const uint4*>(x[c] + block * mx::kBlock + k * p.k)) : make_uint4(0, 0, 0, 0);
     };
+    // scale bytes of a step for this thread's columns 2t and 2t + 1, from the first of its blocks on
+    constexpr int kScaleWords = kSpan == 1 ? 2 : 1;
+    uint32_t xs[COLS][kScaleWords];
+    auto load_scales = [&](uint32_t step) {
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            const uint32_t token = kSpan == 1 ? c * 8 + 2 * t : 2 * t / kSpan;
+            const bool some = token < p.tokens && step < steps;
+            const uint32_t* at = p.x_scales + step * p.x_scale_tokens + token;
+            if constexpr (kSpan == 1) {  // (pairs of tokens are 8-byte aligned; one behind the last is nobody's)
+                const uint2 pair = some ? __ldca(reinterpret_cast<const uint2*>(at)) : make_uint2(0x01010101u, 0x01010101u);
+                xs[c][0] = pair.x;
+                xs[c][1] = pair.y;
+            } else {
+                xs[c][0] = (some ? __ldca(at) : 0x01010101u) >> (2 * t % SPREAD * 8);
+            }
+        }
+    };
     if constexpr (kRefill) {
 #pragma unroll
         for (int s = 0; s < kGroups; ++s) load_x(b[s], warp * kStepBlocks + s * SPREAD);
+        load_scales(warp);
     }
 
     wait_copies(p.depth);
@@ -349,6 +353,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode
         if constexpr (!kRefill) {
 #pragma unroll
             for (int s = 0; s < kGroups; ++s) load_x(b[s], block0 + s * SPREAD);
+            load_scales(step);
         }
         wait_copies(p.depth - 1);
         __syncwarp();
@@ -383,17 +388,19 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode
             for (int u = 0; u < TILES; ++u) {
                 const uint32_t lo = SPREAD == 1 ? lds8(scale_at + u * 16 * p.pitch) : lds16(scale_at + u * 16 * p.pitch);
                 const uint32_t hi = SPREAD == 1 ? lds8(scale_at + (u * 16 + 8) * p.pitch) : lds16(scale_at + (u * 16 + 8) * p.pitch);
-                const float lo0 = scale_of<0>(lo), hi0 = scale_of<0>(hi);
-                const float lo1 = SPREAD == 1 ? lo0 : scale_of<1>(lo), hi1 = SPREAD == 1 ? hi0 : scale_of<1>(hi);
+                const f32x2 low = pack2(scale_of<0>(lo), SPREAD == 1 ? scale_of<0>(lo) : scale_of<1>(lo));
+                const f32x2 high = pack2(scale_of<0>(hi), SPREAD == 1 ? scale_of<0>(hi) : scale_of<1>(hi));
 #pragma unroll
                 for (int c = 0; c < COLS; ++c) {
-                    acc[u][c][0] = fmaf(d[u][c][0], lo0, acc[u][c][0]);
-                    acc[u][c][1] = fmaf(d[u][c][1], lo1, acc[u][c][1]);
-                    acc[u][c][2] = fmaf(d[u][c][2], hi0, acc[u][c][2]);
-                    acc[u][c][3] = fmaf(d[u][c][3], hi1, acc[u][c][3]);
+                    // (scales first: their product is exact but beyond f32's range, and d is 2^24 at most)
+                    constexpr int kSecond = SPREAD == 1 ? s : s * SPREAD + 1;
+                    const f32x2 x = pack2(x_scale_of<s * SPREAD>(xs[c][0]), x_scale_of<kSecond>(xs[c][kScaleWords - 1]));
+                    acc[u][c][0] = fma2(pack2(d[u][c][0], d[u][c][1]), mul2(low, x), acc[u][c][0]);
+                    acc[u][c][1] = fma2(pack2(d[u][c][2], d[u][c][3]), mul2(high, x), acc[u][c][1]);
                 }
             }
         });
+        if constexpr (kRefill) load_scales(step + kWarps);
         __syncwarp();  // the slot has been read
         fetch(step + p.depth * kWarps, slot);
         slot = slot + 1 == p.depth ? 0 : slot + 1;
@@ -407,14 +414,15 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode
     for (int u = 0; u < TILES; ++u)
 #pragma unroll
         for (int c = 0; c < COLS; ++c) {
+            const float2 row = unpack2(acc[u][c][0]), below = unpack2(acc[u][c][1]);  // rows g and g + 8
             if constexpr (kSpan == 1) {
                 float* to = here + (c * 8 + 2 * t) * reduce_pitch(TILES) + u * 16 + g;
-                to[0] = acc[u][c][0];
-                to[reduce_pitch(TILES)] = acc[u][c][1];
-                to[8] = acc[u][c][2];
-                to[reduce_pitch(TILES) + 8] = acc[u][c][3];
+                to[0] = row.x;
+                to[reduce_pitch(TILES)] = row.y;
+                to[8] = below.x;
+                to[reduce_pitch(TILES) + 8] = below.y;
             } else {  // a token's columns
-                float lo = acc[u][c][0] + acc[u][c][1], hi = acc[u][c][2] + acc[u][c][3];
+                float lo = row.x + row.y, hi = below.x + below.y;
 #pragma unroll
                 for (int o = 1; o < kSpan / 2; o *= 2) {
                     lo += __shfl_xor_sync(kFull, lo, o);
@@ -432,7 +440,6 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(TERMS * COLS)) decode
         float sum = 0.0f;
 #pragma unroll
         for (uint32_t v = 0; v < kWarps; ++v) sum += sums[(v * kTokens + token) * reduce_pitch(TILES) + row];
-        sum *= __ldcg(p.back + token);
         if (!(fabsf(sum) < INFINITY)) sum = add_again(p, TERMS == 2 || SPLIT_TERMS ? 2 : 1, token, row0 + row, scales + row * p.pitch);
         const size_t index = static_cast<size_t>(token) * p.n + row0 + row;
         if (p.beta != 0.0f)
@@ -501,10 +508,14 @@ cudaError_t run_tokens(const Params& p, bool bf16, cudaStream_t stream) {
            : tokens <= 8 ? run<1, 2, false, 1>(p, stream)
                          : run<1, 2, false, 2>(p, stream);
 }
+uint32_t steps_of(uint32_t k) { return (k + 127) / 128; }
+uint32_t x_scale_tokens(uint32_t tokens) { return (tokens + 1) / 2 * 2; }
+size_t x_scale_bytes(uint32_t tokens, uint32_t k) { return (static_cast<size_t>(x_scale_tokens(tokens)) * steps_of(k) * sizeof(uint32_t) + 127) / 128 * 128; }
 template <typename XT>
-cudaError_t prepare(const void* x, uint16_t* prepared, float* back, uint32_t tokens, uint32_t k, cudaStream_t stream) {
+cudaError_t prepare(const void* x, uint16_t* prepared, uint32_t* x_scales, uint32_t tokens, uint32_t k, cudaStream_t stream) {
+    const uint32_t steps = steps_of(k);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tokens);
+    cfg.gridDim = dim3((steps + kPrepareThreads / 16 - 1) / (kPrepareThreads / 16), tokens);
     cfg.blockDim = dim3(kPrepareThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -512,9 +523,8 @@ cudaError_t prepare(const void* x, uint16_t* prepared, float* back, uint32_t tok
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, prepare_mxfp4_kernel<XT>, static_cast<const XT*>(x), prepared, back, k);
+    return cudaLaunchKernelEx(&cfg, prepare_mxfp4_kernel<XT>, static_cast<const XT*>(x), prepared, x_scales, k, steps, x_scale_tokens(tokens));
 }
-size_t back_bytes(uint32_t tokens) { return (tokens * sizeof(float) + 127) / 128 * 128; }
 
 }  // namespace decode_mx
 }  // namespace eider
@@ -552,7 +562,7 @@ cudaError_t eider_b200_mxfp4_decode_status(void* raw, uint32_t* host_status) {
 }
 
 size_t eider_b200_mxfp4_w4a16_workspace_bytes(uint32_t tokens, uint32_t in_features, int input_is_bf16) {
-    const size_t few = decode_mx::back_bytes(tokens) + static_cast<size_t>(tokens) * in_features * (input_is_bf16 ? 2 : 4);
+    const size_t few = decode_mx::x_scale_bytes(tokens, in_features) + static_cast<size_t>(tokens) * in_features * (input_is_bf16 ? 2 : 4);
     return in_features % 128 == 0 ? std::max(few, decode_mx::terms_workspace_bytes(tokens, in_features, input_is_bf16)) : few;  // (whichever form it takes)
 }
 
@@ -570,18 +580,20 @@ cudaError_t eider_b200_mxfp4_w4a16_gemv_on_stream(void* raw, const void* input, 
     if (takes_terms(tokens, plan->n, plan->k, input_is_bf16) && (reinterpret_cast<uintptr_t>(w_values) & 31) == 0)
         return run_terms(plan->maps, input, input_is_bf16, tokens, w_values, w_scales_tiled, c, d, beta, out_is_bf16, plan->n, plan->k,
                          static_cast<uint8_t*>(workspace), plan->status, stream);
-    float* back = static_cast<float*>(workspace);
-    uint16_t* prepared = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + back_bytes(tokens));
-    cudaError_t st = input_is_bf16 ? prepare<uint16_t>(input, prepared, back, tokens, plan->k, stream)
-                                   : prepare<float>(input, prepared, back, tokens, plan->k, stream);
+    uint32_t* x_scales = static_cast<uint32_t*>(workspace);
+    uint16_t* prepared = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + x_scale_bytes(tokens, plan->k));
+    cudaError_t st = input_is_bf16 ? prepare<uint16_t>(input, prepared, x_scales, tokens, plan->k, stream)
+                                   : prepare<float>(input, prepared, x_scales, tokens, plan->k, stream);
     if (st != cudaSuccess) return st;
-    const uint32_t groups = (tokens + 15) / 16, each = (tokens + groups - 1) / groups;
+    // (an even number: the scales of a launch's tokens come in aligned pairs)
+    const uint32_t groups = (tokens + 15) / 16, each = groups == 1 ? tokens : ((tokens + groups - 1) / groups + 1) / 2 * 2;
     for (uint32_t first = 0; first < tokens; first += each) {
         const size_t out_bytes = out_is_bf16 ? 2 : 4;
         Params p{};
         p.tokens = std::min(each, tokens - first);
         p.x = prepared + static_cast<size_t>(first) * (input_is_bf16 ? 1 : 2) * plan->k;
-        p.back = back + first;
+        p.x_scales = x_scales + first;
+        p.x_scale_tokens = x_scale_tokens(tokens);
         p.w = w_values;
         p.scales = w_scales_rows;
         p.out = static_cast<uint8_t*>(d) + first * out_bytes * plan->n;

@@ -612,8 +612,9 @@ class Mxfp4MatmulPlan(_DevicePlan):
 
 
 class Mxfp4DecodePlan(_DevicePlan):
-    """W4A16 decode linear over MXFP4 weights: y[t] = W . x[t] for up to 64 tokens, the weights streamed once, x as it is (bf16 or
-    f32).  The plan keeps nothing of a call but tensor maps: calls on several streams and captured graphs may overlap, from one thread."""
+    """W4A16 decode linear over MXFP4 weights: y[t] = W . x[t] for up to 64 tokens, the weights streamed once.  x is bf16 or f32 and not
+    quantized: bf16 elements count exactly within 2^14 of the largest of their block of 32, to 2^-22 of that one else, f32 elements to
+    2^-23 of themselves or 2^-37 of the largest of their block.  The plan keeps nothing of a call but tensor maps: calls on several streams and captured graphs may overlap, from one thread."""
     _destroy = "eider_b200_mxfp4_decode_destroy"
 
     def __init__(self, max_tokens: int, out_features: int, in_features: int):
@@ -633,7 +634,7 @@ class Mxfp4DecodePlan(_DevicePlan):
         out, c = self._output(out, (x.shape[0], self.n), out_dtype, beta, c)
         tokens, bf16 = x.shape[0], int(x.dtype == torch.bfloat16)
         # eider_b200_mxfp4_w4a16_workspace_bytes, bounded from above
-        size = (tokens * 4 + 127) // 128 * 128 + (tokens + 7) // 8 * 8 * self.k * (2 if bf16 else 5) + (self.k + 127) // 128 * 512
+        size = 128 + (tokens + 7) // 8 * 8 * self.k * (2 if bf16 else 5) + (self.k + 127) // 128 * 512
         workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
         _call(self.device, "eider_b200_mxfp4_w4a16_gemv_on_stream", self._plan, x.data_ptr(), bf16, tokens, w.packed.data_ptr(),
               w.scales_rows.data_ptr(), w.scales_rows.shape[1], w.scales_tiled.data_ptr(), _ptr(c), out.data_ptr(), beta, int(out.dtype == torch.bfloat16),

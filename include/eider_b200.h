@@ -854,9 +854,9 @@ EIDER_B200_API cudaError_t eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream(void
 
 /* W4A16 product for 1 to 64 tokens, D[t][n] = X . W^T + beta * C, X f32 or bf16 [tokens][in_features], D and C f32 or bf16.  The
  * scales come twice: as rows of `scale_pitch` bytes (a multiple of 16, at least in_features / 32 rounded up to 8) with zeros behind the
- * blocks, and in tiles as for the GEMM.  A plan reads one or the other, and the sums' order, by the call's sizes and types alone.
- * bf16 elements of X enter the products exactly where they lie within 2^14 of the largest element of their block of 32, with 2^-22 of that
- * one else; f32 elements with 2^-23 of themselves or 2^-37 of the largest of their token or block.  X, weights, scales and workspace
+ * blocks, and in tiles as for the GEMM.  Which of the two a call reads, and the order of its sums, follow from its sizes and types and from
+ * whether w_values is 32-byte aligned.  bf16 elements of X enter the products exactly where they lie within 2^14 of the largest element of
+ * their block of 32, with 2^-22 of that one else; f32 elements with 2^-23 of themselves or 2^-37 of the largest of their block.  X, weights, scales and workspace
  * 16-byte aligned.  The workspace is one call's; a plan keeps tensor maps between calls, so one host thread drives it, on any number of
  * streams. */
 EIDER_B200_API void* eider_b200_mxfp4_decode_create(uint32_t max_tokens, uint32_t out_features, uint32_t in_features);

@@ -436,3 +436,72 @@ def test_decode_plans_report_their_status():
         x = randn(g, tokens, k)
         x[0, 3] = float("nan")
         assert torch.isnan(plan.run(x, w)[0]).all() and plan.status() == 0
+
+
+def block_bound(x, w, dtype):
+    """decode_bound without its allowance for the token's largest element: what an element loses is at most 2^-22 (bf16, beyond 2^14 below) or
+    2^-37 (f32) of the largest of its own block of 32."""
+    steps = x.shape[1] // 32 + 16 + (1 if dtype == torch.float32 else 0)
+    largest = x.abs().reshape(x.shape[0], -1, 32).amax(-1)
+    lost = 2.0 ** -22 if dtype == torch.bfloat16 else 2.0 ** -37
+    return steps * 2.0 ** -23 * (x.abs() @ w.abs().t()) + lost * largest @ w.abs().reshape(w.shape[0], -1, 32).sum(-1).t()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,k", [(1, 1024), (2, 1024), (3, 96), (4, 1024), (5, 1056), (9, 2912), (16, 544), (33, 1056), (9, 1024), (24, 2048), (64, 1024)])
+def test_decode_keeps_blocks_far_below_an_outlier(tokens, k, dtype):
+    """An activation with one huge element that the weights do not look at (zero codes in its block): what is left of the results are blocks
+    2^41 to 2^100 below it, in either form of the product."""
+    g = gen(tokens + k)
+    n = 300
+    wp, ws = ref.weight(g, n, k)
+    codes = ref.unpack(wp)
+    codes[:, :32] = 0
+    w = ref.pack(codes).contiguous()
+    wd, wv = ops.Mxfp4Weight.from_checkpoint(w, ws), ref.values(codes, ws)
+    for below in (20, 41, 60, 100):
+        x = torch.randn(tokens, k, generator=g, device="cuda")
+        x[:, 32:] *= 2.0 ** -below
+        x[:, 1:32] = 0
+        x[:, 0] = 1.0
+        x = x.to(dtype)
+        xv = x.double()
+        want = xv @ wv.t()
+        y = ops.Mxfp4DecodePlan(64, n, k).run(x, wd, out_dtype=torch.float32).double()
+        assert want[:, :8].abs().amax() >= 2.0 ** (-below - 12)
+        assert ((y - want).abs() <= block_bound(xv, wv, dtype)).all(), below
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,k", [(1, 1024), (2, 1056), (4, 1024), (8, 1056), (16, 1056), (12, 1024)])
+def test_decode_scales_at_the_ends_of_the_range(tokens, k, dtype):
+    """Activations and weight scales that are huge on one side and tiny on the other: the products lie in f32's range, the scales' do not."""
+    g = gen(tokens)
+    n = 64
+    codes = torch.randint(0, 16, (n, k), generator=g, device="cuda", dtype=torch.uint8)
+    for x_exponent, w_exponent in ((120, -100), (-120, 100), (100, -127), (-100, 127), (60, 50), (-60, -50)):
+        x = (torch.randn(tokens, k, generator=g, device="cuda") * 2.0 ** x_exponent).to(dtype)
+        ws = torch.full((n, k // 32), 127 + w_exponent, dtype=torch.uint8, device="cuda")
+        w = ops.Mxfp4Weight.from_checkpoint(ref.pack(codes).contiguous(), ws)
+        xv, wv = x.double(), ref.values(codes, ws)
+        y = ops.Mxfp4DecodePlan(64, n, k).run(x, w, out_dtype=torch.float32).double()
+        assert ((y - xv @ wv.t()).abs() <= block_bound(xv, wv, dtype) + 2.0 ** -125 * (k // 32)).all(), (x_exponent, w_exponent)
+
+
+@pytest.mark.parametrize("tokens,k,dtype", [(9, 1024, torch.bfloat16), (64, 1024, torch.bfloat16), (5, 1024, torch.float32), (1, 8192, torch.bfloat16)])
+def test_decode_weights_aligned_to_16_bytes_only(tokens, k, dtype):
+    """They take the other form of the product: other sums, the same bounds."""
+    g = gen(24)
+    n = 200
+    wp, ws = ref.weight(g, n, k)
+    buffer = torch.zeros(wp.numel() + 16, device="cuda", dtype=torch.uint8)
+    odd = buffer[16:].view(n, k // 2)
+    odd.copy_(wp)
+    w = ops.Mxfp4Weight.from_checkpoint(odd, ws)
+    assert w.packed.data_ptr() % 32 == 16
+    x = randn(g, tokens, k, dtype=dtype)
+    xv, wv = x.double(), ref.values(ref.unpack(wp), ws)
+    plan = ops.Mxfp4DecodePlan(64, n, k)
+    for weight in (w, ops.Mxfp4Weight.from_checkpoint(wp, ws)):
+        y = plan.run(x, weight, out_dtype=torch.float32).double()
+        assert ((y - xv @ wv.t()).abs() <= block_bound(xv, wv, dtype)).all()
