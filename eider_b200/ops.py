@@ -531,6 +531,8 @@ class _DevicePlan:
 
     def _output(self, out: torch.Tensor | None, shape, dtype, beta: float, c: torch.Tensor | None):
         """The output and C, checked: C has the output's shape and type, and is the output itself unless given."""
+        if beta != 0.0 and out is None and c is None:
+            raise ShapeError("beta wants C, or an output that holds it")
         if out is None:
             if dtype not in (torch.float32, torch.bfloat16):
                 raise ShapeError(f"output must be f32 or bf16, got {dtype}")

@@ -122,3 +122,22 @@ def test_decode_status_refuses():
     import ctypes as C
     lib = _lib.load()
     assert lib.eider_b200_mxfp4_decode_status(None, C.byref(C.c_uint32(0))) == INVALID and lib.eider_b200_mxfp4_decode_status(SOME, None) == INVALID
+
+
+def test_beta_wants_something_to_add(monkeypatch):
+    """Without C and without an output that holds it, what beta multiplies would be memory that nobody has written."""
+    called = fakes.without_a_device(monkeypatch)
+    u8 = torch.uint8
+    w = ops.Mxfp4Weight.from_checkpoint(torch.zeros(8, 32, dtype=u8), torch.zeros(8, 2, dtype=u8))
+    x = ops.Mxfp4Matrix(torch.zeros(4, 32, dtype=u8), torch.zeros(512, dtype=u8), 4, 64)
+    gemm, decode = object.__new__(ops.Mxfp4MatmulPlan), object.__new__(ops.Mxfp4DecodePlan)
+    gemm._plan, gemm.device, gemm.m, gemm.n, gemm.k = None, torch.device("cpu"), 4, 8, 64
+    decode._plan, decode.device, decode.max_tokens, decode.n, decode.k = None, torch.device("cpu"), 4, 8, 64
+    for plan, a in ((gemm, x), (decode, torch.zeros(4, 64))):
+        called.clear()
+        with pytest.raises(ops.ShapeError):
+            plan.run(a, w, beta=1.0)
+        assert not called
+        plan.run(a, w, beta=1.0, c=torch.zeros(4, 8, dtype=torch.bfloat16))
+        plan.run(a, w, beta=1.0, out=torch.zeros(4, 8))
+        assert len(called) == 2
