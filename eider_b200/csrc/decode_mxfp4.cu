@@ -230,10 +230,10 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_mxfp4_kernel(const XT
     }
 }
 
-// A result whose sum came out infinite or NaN, added up again block by block with one scaling a block: the product of an activation's and a
-// weight's scale overflows where what it is multiplied by is small, and a NaN scale counts as an infinity in the loop.
+// A result whose sum came out infinite or NaN, added up again in 64 bits: parts of a sum, or the product of an activation's and a weight's
+// scale, overflow where the result does not, and a NaN scale counts as an infinity in the loop.
 __device__ __noinline__ float add_again(const Params& p, uint32_t terms, uint32_t token, uint32_t row, const uint8_t* scales) {
-    float sum = 0.0f;
+    double sum = 0.0;
     for (uint32_t block = 0; block < p.k / mx::kBlock; ++block) {
         if (scales[block] == mx::kNanCode) return NAN;
         float part = 0.0f;
@@ -245,9 +245,9 @@ __device__ __noinline__ float add_again(const Params& p, uint32_t terms, uint32_
             part = fmaf(x, code & 8 ? -w : w, part);
         }
         const uint32_t x_scale = __ldcg(p.x_scales + block / kStepBlocks * p.x_scale_tokens + token) >> (block % kStepBlocks * 8) & 255;
-        sum += ldexpf(part, static_cast<int>(x_scale + scales[block]) - 254);
+        sum += ldexp(static_cast<double>(part), static_cast<int>(x_scale + scales[block]) - 254);
     }
-    return sum;
+    return static_cast<float>(sum);
 }
 
 // TILES: 16-row MMA tiles of a CTA.

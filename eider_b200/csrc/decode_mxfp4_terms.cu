@@ -101,7 +101,7 @@ __device__ __forceinline__ void load8(const float* p, bool live, float (&v)[8]) 
 // x as E4M3 terms: one CTA a step of 128 elements and 16 tokens, 16 threads a token of it, four a block.  A block's first scale brings its largest
 // finite element to 2^7 .. 2^8; what a term leaves is at most 2^3 in its scale, so the next term's is 2^-5 of it.  bf16 elements keep all
 // their bits as long as they lie within 2^14 of their block's largest, and 2^-22 of that one else; f32 elements leave at most 2^-24 of
-// themselves, or 2^-37 of the largest.  An infinity or NaN goes in as NaN: the product's last lines tell them apart.
+// themselves, or 2^-37 of the largest.  An infinity or NaN goes in as NaN: resolve tells them apart.
 constexpr uint32_t kPrepareThreads = 256;
 template <typename XT>
 __global__ void __launch_bounds__(kPrepareThreads) prepare_terms_kernel(const XT* __restrict__ x, uint8_t* __restrict__ prepared, uint32_t tokens, uint32_t padded, uint32_t k) {
@@ -156,19 +156,20 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_terms_kernel(const XT
 __device__ __forceinline__ float value_at(const void* x, int is_bf16, size_t i) {
     return is_bf16 ? bf16_bits_to_float(__ldcg(static_cast<const uint16_t*>(x) + i)) : __ldcg(static_cast<const float*>(x) + i);
 }
-// What a row's sum is when it came out infinite or NaN: x's infinities went in as NaNs.
-__device__ __noinline__ float resolve(const Params& p, float sum, uint32_t token, uint32_t row) {
+// What a row's sum is when it came out infinite or NaN: x's infinities went in as NaNs, and parts of a sum, or the term that an element near
+// f32's end is rounded up to, overflow where the result does not.  Added up in 64 bits, in order.
+__device__ __noinline__ float resolve(const Params& p, uint32_t token, uint32_t row) {
     const uint8_t* scales = p.scales + static_cast<size_t>(row / 128) * (p.k / 128) * kScaleTile + row % 32 * 16 + row % 128 / 32 * 4;
-    float special = 0.0f;
+    double total = 0.0;
     for (uint32_t k = 0; k < p.k; ++k) {
-        if (scales[static_cast<size_t>(k / 128) * kScaleTile + k / 32 % 4] == mx::kNanCode) return NAN;
+        const uint32_t scale = scales[static_cast<size_t>(k / 128) * kScaleTile + k / 32 % 4];
+        if (scale == mx::kNanCode) return NAN;
         const float x = value_at(p.raw, p.x_is_bf16, static_cast<size_t>(token) * p.k + k);
-        if (fabsf(x) < INFINITY) continue;
         const uint32_t code = p.w[static_cast<size_t>(row) * (p.k / 2) + k / 2] >> (k % 2 * 4) & 15;
-        special += x * ((code & 7) == 0 ? 0.0f : (code & 8) ? -1.0f : 1.0f);
-        if (isnan(special)) return NAN;
+        total += static_cast<double>(x) * e2m1_value(code) * mx::scale_value(scale);
+        if (isnan(total)) return NAN;
     }
-    return special != 0.0f ? special : sum;
+    return static_cast<float>(total);
 }
 
 __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Params p) {
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
         }
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i)
-            if (c + i < p.tokens) sums[(c + i) * kSumPitch + warp * 32 + lane] = good ? v[i] : NAN;  // (a wait ran out: no result, and the plan's status says so)
+            if (c + i < p.tokens) sums[(c + i) * kSumPitch + warp * 32 + lane] = good ? v[i] : NAN;  // (a wait ran out: no sum, and the plan's status says so)
     }
     umma::tc_fence_before();
     __syncthreads();
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
 #pragma unroll
         for (uint32_t s = 0; s < kMaxSplits; ++s)
             if (s < splits) sum += v[s];
-        if (!(fabsf(sum) < INFINITY)) sum = resolve(p, sum, token, row0 + row);
+        if (!(fabsf(sum) < INFINITY)) sum = resolve(p, token, row0 + row);
         const size_t index = static_cast<size_t>(token) * p.n + row0 + row;
         if (p.beta != 0.0f)
             sum = fmaf(p.beta, p.out_is_bf16 ? bf16_bits_to_float(static_cast<const uint16_t*>(p.c)[index]) : static_cast<const float*>(p.c)[index], sum);

@@ -861,7 +861,7 @@ EIDER_B200_API cudaError_t eider_b200_mxfp4_gemm_tn_silu_quantize_on_stream(void
  * streams. */
 EIDER_B200_API void* eider_b200_mxfp4_decode_create(uint32_t max_tokens, uint32_t out_features, uint32_t in_features);
 EIDER_B200_API void eider_b200_mxfp4_decode_destroy(void* plan);
-/* The plan's kernel status word (0 = ok): a bounded wait that ran out is recorded there, and its results are NaN. */
+/* The plan's kernel status word (0 = ok): a bounded wait that ran out is recorded there.  Results of such a call are not to be used. */
 EIDER_B200_API cudaError_t eider_b200_mxfp4_decode_status(void* plan, uint32_t* host_status);
 EIDER_B200_API size_t eider_b200_mxfp4_w4a16_workspace_bytes(uint32_t tokens, uint32_t in_features, int input_is_bf16);
 EIDER_B200_API cudaError_t eider_b200_mxfp4_w4a16_gemv_on_stream(void* plan, const void* input, int input_is_bf16, uint32_t tokens,

@@ -505,3 +505,30 @@ def test_decode_weights_aligned_to_16_bytes_only(tokens, k, dtype):
     for weight in (w, ops.Mxfp4Weight.from_checkpoint(wp, ws)):
         y = plan.run(x, weight, out_dtype=torch.float32).double()
         assert ((y - xv @ wv.t()).abs() <= block_bound(xv, wv, dtype)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,k", [(1, 1024), (3, 96), (6, 1056), (16, 544), (9, 1024), (24, 256), (64, 1024)])
+def test_decode_results_at_the_end_of_the_range(tokens, k, dtype):
+    """Results that f32 holds although a part of their sum, or an element rounded up, lies beyond it; and results that it does not hold."""
+    g = gen(25)
+    n = 40
+    codes = torch.zeros(n, k, device="cuda", dtype=torch.uint8)
+    codes[0, :3] = torch.tensor([2, 2, 10], device="cuda", dtype=torch.uint8)       # 1, 1, -1
+    codes[1, 0] = 2                                                                # one element by itself
+    codes[2, :2] = 2                                                               # overflows
+    codes[3, :2] = 10
+    codes[4, 0], codes[4, 40], codes[4, 41] = 2, 2, 10                             # over two blocks
+    codes[5, 5:] = torch.randint(0, 16, (k - 5,), generator=g, device="cuda", dtype=torch.uint8)
+    ws = torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda")
+    x = randn(g, tokens, k)
+    x[:, :3] = x[:, 40:42] = torch.finfo(dtype).max
+    x = x.to(dtype)
+    w = ops.Mxfp4Weight.from_checkpoint(ref.pack(codes).contiguous(), ws)
+    xv, wv = x.double(), ref.values(codes, ws)
+    want = (xv @ wv.t()).float()
+    y = ops.Mxfp4DecodePlan(64, n, k).run(x, w, out_dtype=torch.float32)
+    largest = torch.full_like(y[:, 0], float(torch.finfo(dtype).max))
+    assert torch.equal(y[:, 0], largest) and torch.equal(y[:, 1], largest) and torch.equal(y[:, 4], largest)
+    assert torch.equal(y[:, 2], torch.full_like(largest, float("inf"))) and torch.equal(y[:, 3], torch.full_like(largest, -float("inf")))
+    assert not y[:, 6:].any() and torch.isfinite(want[:, 5]).sum() == torch.isfinite(y[:, 5]).sum()
