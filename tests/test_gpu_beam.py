@@ -224,3 +224,15 @@ def test_scores_do_not_depend_on_alignment(v, dtype):
         copy.copy_(logits)
         for x, y in zip(ops.beam_search_select(copy, scores, k), want):
             assert torch.equal(x, y), (pitch, first)
+
+
+@pytest.mark.parametrize("row_bytes", [65536, 65552, 300001, 8 << 20])
+def test_reorder_long_states(row_bytes):
+    """Rows beyond what one CTA copies at a time, as of key and value caches."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    b, w = (1, 4) if row_bytes > 1 << 20 else (3, 5)
+    states = [torch.randint(0, 256, (b, w, row_bytes), generator=g, device="cuda", dtype=torch.uint8) for _ in range(2)]
+    parents = torch.randint(0, w, (b, w), generator=g, device="cuda", dtype=torch.int32)
+    batch = torch.arange(b, device="cuda")[:, None]
+    for s, o in zip(states, ops.beam_search_reorder(states, parents)):
+        assert torch.equal(o, s[batch, parents.long()])

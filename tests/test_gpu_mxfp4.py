@@ -532,3 +532,101 @@ def test_decode_results_at_the_end_of_the_range(tokens, k, dtype):
     assert torch.equal(y[:, 0], largest) and torch.equal(y[:, 1], largest) and torch.equal(y[:, 4], largest)
     assert torch.equal(y[:, 2], torch.full_like(largest, float("inf"))) and torch.equal(y[:, 3], torch.full_like(largest, -float("inf")))
     assert not y[:, 6:].any() and torch.isfinite(want[:, 5]).sum() == torch.isfinite(y[:, 5]).sum()
+
+
+@pytest.mark.parametrize("n,k,tokens,dtype", [(30001, 512, 5, torch.bfloat16), (60000, 512, 48, torch.bfloat16), (60000, 512, 64, torch.bfloat16), (30001, 512, 24, torch.float32),
+                                              (60001, 2304, 1, torch.bfloat16)])
+def test_decode_of_an_lm_head(n, k, tokens, dtype):
+    """More row tiles than the device runs at a time: clusters of one CTA, several rounds of them, tensor memory handed on within an SM."""
+    g = gen(26)
+    x, w = randn(g, tokens, k, dtype=dtype), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k))
+    plan = ops.Mxfp4DecodePlan(64, n, k)
+    y = plan.run(x, w, out_dtype=torch.float32)
+    assert torch.equal(plan.run(x, w, out_dtype=torch.float32), y)
+    xv = x.double()
+    for first in range(0, n, 8192):
+        wv = w.dequantize()[first: first + 8192].double()
+        assert ((y[:, first: first + 8192].double() - xv @ wv.t()).abs() <= block_bound(xv, wv, dtype)).all()
+    assert plan.status() == 0
+
+
+@pytest.mark.parametrize("m,n", [(512, 5001), (1000, 5000), (1200, 1001), (520, 13), (2048, 1032)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_gemm_ragged_outputs_on_cta_pairs(m, n, out):
+    """Rows of the output that are no multiple of 16 elements, with beta * C, at 4, 8, 10, 5 and 16 row tiles."""
+    g = gen(m)
+    k = 544
+    x = randn(g, m, k)
+    xq, w = ops.quantize_mxfp4(x), ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k))
+    xv, wv = ref.values(*ref.quantize(x)), w.dequantize().double()
+    plan = ops.Mxfp4MatmulPlan(m, n, k)
+    c = randn(g, m, n, dtype=out)
+    want = xv @ wv.t() - 0.5 * c.double()
+    bound = rounded(product_bound(xv, wv, 2) + 2.0 ** -23 * c.double().abs(), want, out)
+    codes = [plan.block_n, 384, 512]
+    for code in codes:
+        plan.set_block_n(code)
+        guarded = torch.full((m * n + 64,), 7.0, device="cuda", dtype=out)
+        y = plan.run(xq, w, out=guarded[: m * n].view(m, n), beta=-0.5, c=c)
+        assert ((y.double() - want).abs() <= bound).all(), code
+        assert (guarded[m * n:] == 7.0).all()
+    assert plan.status() == 0
+
+
+def test_more_weights_than_a_plan_remembers():
+    """A model's layers share a plan: twenty weights in turn, twice, and one whose memory is used again."""
+    g = gen(27)
+    n, k = 300, 512
+    x = randn(g, 9, k, dtype=torch.bfloat16)
+    weights = [ops.Mxfp4Weight.from_checkpoint(*ref.weight(g, n, k)) for _ in range(20)]
+    decode, gemm, xq = ops.Mxfp4DecodePlan(16, n, k), ops.Mxfp4MatmulPlan(9, n, k), ops.quantize_mxfp4(x)
+    first = [(ops.Mxfp4DecodePlan(16, n, k).run(x, w), ops.Mxfp4MatmulPlan(9, n, k).run(xq, w)) for w in weights]
+    for _ in range(2):
+        for w, (a, b) in zip(weights, first):
+            assert torch.equal(decode.run(x, w), a) and torch.equal(gemm.run(xq, w), b)
+    for part in ("packed", "scales_row_major", "scales_tiled", "scales_rows"):
+        getattr(weights[0], part).copy_(getattr(weights[1], part))
+    assert torch.equal(decode.run(x, weights[0]), first[1][0]) and torch.equal(gemm.run(xq, weights[0]), first[1][1])
+
+
+def test_silu_quantizer_with_large_gates():
+    """e^-gate is off by |gate| * 2^-23 of itself and vanishes below -87.3: a block of such gates keeps its codes but for boundaries, and
+    what vanishes is below 2^-119 of up."""
+    g = gen(28)
+    rows, k = 256, 512
+    gate = torch.linspace(-85, 85, rows, device="cuda").unsqueeze(1) + torch.randn(rows, k, generator=g, device="cuda")
+    up = torch.randn(rows, k, generator=g, device="cuda")
+    m = ops.silu_mul_halves_quantize_mxfp4(torch.cat([gate, up], 1))
+    act = ref.silu_mul(torch.cat([gate, up], 1).double())
+    codes, scales = ref.quantize(act)
+    got, clean = ref.untile(m.scales, rows, k)
+    assert clean
+    # 95 * 2^-23 of a value, and about seven boundaries over a block's range: under 1e-4 of the codes
+    assert (got != scales).float().mean() <= 1e-3 and (ref.unpack(m.packed) != codes).float().mean() <= 1e-3
+    step = torch.exp2(scales.double() - 127).repeat_interleave(32, 1) * 2
+    assert ((m.dequantize().double() - act).abs() <= step * 1.01).all()
+    far = torch.cat([torch.full((4, 64), -95.0, device="cuda"), torch.full((4, 64), 3.0, device="cuda")], 1)
+    far[1, :64], far[2, :64], far[3, :64] = -300.0, 90.0, 3e38
+    far[3, 64:] = 0.5
+    y = ops.silu_mul_halves_quantize_mxfp4(far).dequantize().double()
+    assert y[:2].abs().max() <= 3 * 2.0 ** -119 and (y[2] == 256.0).all() and torch.isfinite(y[3]).all() and (y[3] >= 1e38).all()
+    far[0, 0], far[1, 40], far[2, 0], far[3, 63] = float("nan"), float("inf"), -float("inf"), float("nan")
+    y = ops.silu_mul_halves_quantize_mxfp4(far).dequantize()
+    bad = torch.isnan(y)
+    assert bad[0, :32].all() and bad[1, 32:].all() and bad[2, :32].all() and bad[3, 32:].all() and int(bad.sum()) == 4 * 32
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_poisoned_tokens_stay_alone_in_the_routed_layer(value):
+    g = gen(29)
+    tokens, experts, top_k, hidden, inter = 70, 8, 3, 160, 96
+    gate_up, down = ([t.reshape(experts, -1, t.shape[1]) for t in ref.weight(g, experts * n, k, std=0.1)] for n, k in ((2 * inter, hidden), (hidden, inter)))
+    gu, dn = ops.GroupedMxfp4Weights.from_checkpoint(*gate_up).interleave_gate_up(), ops.GroupedMxfp4Weights.from_checkpoint(*down)
+    x, logits = randn(g, tokens, hidden), randn(g, tokens, experts)
+    moe = ops.GroupedMoe(tokens, experts, top_k, hidden, inter, weight_format="mxfp4")
+    clean = moe.run(x, logits, None, dn, w_gate_up_interleaved=gu).clone()
+    x[11, 7], x[12, 159] = value, value
+    y = moe.run(x, logits, None, dn, w_gate_up_interleaved=gu)
+    others = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    others[11:13] = False
+    assert torch.isnan(y[11:13]).all() and torch.equal(y[others], clean[others])
