@@ -37,7 +37,7 @@ __host__ __device__ inline size_t tiled_scale_offset(uint32_t outer, uint32_t kb
     return base + (in_tile % 32) * 16 + (in_tile / 32) * 4 + (kb % 4);
 }
 
-// n / d for n < 2^31 by multiplication (d > 0).
+// n / d for n < 2^31 by multiplication (d > 0): Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994.
 struct FastDiv {
     uint32_t d, magic, shift;
     FastDiv() : d(1), magic(1), shift(0) {}

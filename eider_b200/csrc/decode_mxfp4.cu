@@ -456,9 +456,13 @@ struct Plan {
 };
 
 // The weights go to the tensor cores as they are (decode_mxfp4_terms.cu) where their layout allows, but for a few tokens and weights that are
-// neither long nor many.  us here / there, bf16: K 5120 -> N 13824 one token 10.8 / 11.6, eight 13.6 / 12.5, sixteen 19.8 / 13.8, 48 in
-// three launches 50.6 / 21.7; K 1024 -> N 2048 one 3.5 / 4.9; K 13824 -> N 5120 one 15.3 / 12.0, 48 73 / 19.4; K 5120 -> N 27648 one 18.2 /
-// 17.0.  f32: K 5120 -> N 13824 one 10.9 / 12.2, five 15.8 / 12.7.
+// neither long nor many.  us a layer here / there, weights beyond L2 in replayed graphs, bf16 with one, four, five and eight tokens: K 5120 ->
+// N 13824 12.3 / 12.6, 13.4 / 13.0, 14.7 / 13.1, 15.2 / 13.6; K 1024 -> N 2048 2.8 / 4.6, 3.1 / 4.9, 3.3 / 4.9, 3.5 / 5.1; K 2048 -> N 1536 3.4 /
+// 5.2, 3.7 / 5.4, 4.0 / 5.4, 4.2 / 5.5; K 5120 -> N 5120 8.1 / 7.5, 8.7 / 7.7, 9.1 / 7.8, 9.4 / 7.9.  f32 with one, two, three: K 5120 ->
+// N 13824 12.4 / 13.3, 13.5 / 13.2, 14.5 / 13.3; K 1024 -> N 2048 3.0 / 5.2, 3.2 / 5.2, 3.3 / 5.3.  At the other bounds, one and four tokens:
+// K 8064 -> N 5120 11.4 / 9.3, 12.8 / 9.4, K 8192 11.4 / 9.4, 13.0 / 9.6; K 5120 -> N 26112 22.0 / 17.8, 24.1 / 18.5, N 27648 22.2 / 18.0, 24.4 /
+// 18.7.  So the bound on tokens is where the larger layers turn and the small ones have not; layers of 25 million weights and more would
+// turn at one token.  More tokens: K 5120 -> N 13824 sixteen 19.8 / 13.8, 48 in three launches 50.6 / 21.7; K 13824 -> N 5120 48 73 / 19.4.
 constexpr uint32_t kFewTokens = 4, kLongK = 8192;
 constexpr uint64_t kManyWeights = 1ull << 27;
 bool takes_terms(uint32_t tokens, uint32_t n, uint32_t k, int input_is_bf16) {

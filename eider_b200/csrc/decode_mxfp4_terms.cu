@@ -3,12 +3,14 @@
 //
 // Bound: HBM, N * K * 17/32 bytes of weights.  The tensor cores take the weights as they are: E2M1 codes and E8M0 block scales are operands
 // of tcgen05.mma kind::mxf8f6f4, and x goes in as a sum of E4M3 terms with block scales of their own, each the rounding of what the terms
-// before it left.  A code has four significant bits and a sign, so two terms are all of bf16's eight bits and five all of f32's
-// twenty-four; the products are exact.
+// before it left.  A code has four significant bits and a sign, so two terms are all of bf16's eight bits, for elements within 2^14 of their
+// block's largest, and five all of f32's twenty-four near it; what lies below loses bits (prepare_terms_kernel).  The products of terms are
+// exact.
 //  * A CTA has 128 rows (the MMA's M) and a part of K; all terms of all tokens are its columns, up to 128, so an MMA reads the weights from
 //    shared memory once.  A term's MMAs of their own took as long as the copies: 24.8 us for one token (K 5120 -> N 13824), now 11.6.
 //  * The CTAs of a cluster share their rows and split K; their sums meet through distributed shared memory in rank order: no atomics, the
-//    same order of additions in every run.  As many CTAs a cluster as all clusters run at once: of 2 / 3 / 4 / 6 / 8 the product above took
+//    same order of additions in every run.  As many CTAs a cluster as all clusters would run at once with three CTAs an SM (beyond 96
+//    columns, tensor memory lets two, and the third waits for theirs): of 2 / 3 / 4 / 6 / 8 the product above took
 //    16.1 / 13.0 / 19.2 / 17.5 / 22.5 us (nine tokens), K 13824 -> N 5120 with 4 / 6 / 8 18.1 / 14.5 / 12.9.
 //  * The TMA brings 128 rows x 128 elements a step and spreads them: an operand byte holds one code whatever its width, 16 codes in the
 //    lower half of 16 bytes.  This needs K % 128 == 0.  Four warps that copied them there (8 bytes a cp.async) kept it at 15.5 us without
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(kThreads) decode_terms_kernel(const __grid_con
 
 static_assert(kRing >= 2 * stage_bytes(kMaxColumns) && kRing >= 64 * kSumPitch * 4 && columns_of(64, true) <= kMaxColumns && columns_of(24, false) <= kMaxColumns, "ring of the most tokens");
 
-// Clusters of `splits` CTAs that the device runs at a time: those it would run with one CTA an SM (asked for once, with shared memory for
+// Clusters of `splits` CTAs that the device runs at a time with three CTAs an SM: those it would run with one CTA an SM (asked for once, with shared memory for
 // no more), times the CTAs an SM.
 constexpr uint32_t kSmemMost = 226 * 1024;
 uint32_t clusters_at_once(uint32_t splits) {
@@ -360,7 +362,7 @@ cudaError_t run_terms(gemm::FifoCache<CUtensorMap>& maps, const void* x, int inp
     static std::atomic<uint8_t> configured[gemm::kMaxDevices];
     if (st = gemm::opt_in_smem(configured, decode_terms_kernel, kSmemMost); st != cudaSuccess) return st;
     const uint32_t each = group_of(tokens, input_is_bf16), steps = k / 128, tiles = (n + kRows - 1) / kRows;
-    // as many CTAs a cluster as K has steps and as all clusters run at once
+    // as many CTAs a cluster as K has steps and as all clusters run at once (by three CTAs an SM, whatever the columns)
     uint32_t splits = std::min(kMaxSplits, steps);
     while (splits > 1 && tiles > clusters_at_once(splits)) --splits;
     cudaLaunchAttribute attr[2];

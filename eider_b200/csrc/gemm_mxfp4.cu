@@ -4,8 +4,12 @@
 //
 // Measured (B200): 512 x 5120 -> 27648 30.9 us (4.7 PFLOP/s; NVFP4 32), 8192 x 5120 -> 27648 387 us (6.0 PFLOP/s), 2048 x 13824 -> 5120 53.4 us;
 // gate/up 2048 x 5120 -> 2 x 13824 with SiLU * up -> MXFP4 in its epilogue 91 us; the experts' pair of 4096 tokens, 8 of 128 experts, 2048 /
-// 768, 65 + 53 us, of 77 tokens 40 + 22 us (weights at 5 TB/s).  333 x 2912 -> 5000 10.3 us on tiles of one CTA: rows of 10000 bytes do not
-// suit the CTA pairs' wide stores (53 us on them).
+// 768, 65 + 53 us, of 77 tokens 40 + 22 us (weights at 5 TB/s); one token's layer 8.6 + 6.8 us.  K 13824 -> N 5120 with 1 / 16 / 64 / 128 tokens 22.5 / 20.7 / 16.4 / 16.9 us:
+// 80 tiles of 54 stages each, and no split K.
+//
+// Outputs whose N is no multiple of 16 elements, or that are not 32-byte aligned, go out one element an access (kEpiOther), which CTA pairs
+// feel most: 512 x 2912 -> 5000 53.8 us, -> 5008 10.3 us; 2048 x 2912 -> 5000 148, -> 5008 20.4.  333 tokens have an odd number of row
+// tiles and so tiles of one CTA: 10.3 us at N 5000.
 #include "gemm_launch.cuh"
 
 namespace eider {

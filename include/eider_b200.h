@@ -878,7 +878,8 @@ EIDER_B200_API cudaError_t eider_b200_moe_quantize_routes_mxfp4_on_stream(const 
                                                                           uint32_t rows, uint32_t routes_per_row, uint32_t in_features,
                                                                           uint32_t scale_tile_bytes, cudaStream_t stream);
 /* m = out features per expert, a multiple of 32; the weights' scales tiled per expert (eider_b200_mxfp4_scales_to_tiled_on_stream
- * with groups = experts).  Output bf16 [route][m] times alpha[expert]. */
+ * with groups = experts).  Output bf16 [route][m] times alpha[expert], each rounded once from its f32 sum: a layer's weighted sum over
+ * bf16 routes is off by one such rounding (0.0017 of it in the 2-norm) before its own result is rounded. */
 EIDER_B200_API int eider_b200_mxfp4_grouped_gemm_supported(uint32_t m, uint32_t max_n, uint32_t k, uint32_t groups);
 EIDER_B200_API void* eider_b200_mxfp4_grouped_gemm_create(uint32_t m, uint32_t max_n, uint32_t k, uint32_t groups);
 EIDER_B200_API void eider_b200_mxfp4_grouped_gemm_destroy(void* plan);
