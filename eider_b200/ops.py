@@ -1447,29 +1447,32 @@ def beam_search_reorder(states: list, parents: torch.Tensor, out: list | None = 
     stride = parents.stride(0) if batch > 1 else beams
     if stride < beams:
         raise ShapeError("rows of parents overlap")
-    if out is None:
+    given = out is not None
+    if not given:
         out = [torch.empty_like(t) for t in states]
     if not states or len(out) != len(states):
         raise ShapeError("as many outputs as states are wanted, and one at least")
-    sizes = []
+    sources, targets, sizes = [], [], []
     for s, o in zip(states, out):
         if s.shape[:2] != (batch, beams) or s.numel() == 0 or o.shape != s.shape or o.dtype != s.dtype or not s.is_contiguous() or not o.is_contiguous():
             raise ShapeError(f"states must be contiguous [{batch}, {beams}, ...], and outputs like them")
+        sources.append(s.data_ptr())
+        targets.append(o.data_ptr())
         sizes.append(s.nbytes // (batch * beams))
     _need_device(parents.device, *states, *out)
-    # in the order of addresses, only states may lie over each other
-    written = read = 0  # the end of the outputs and of the states so far
-    for start, size, is_out in sorted([(t.data_ptr(), t.nbytes, False) for t in states] + [(t.data_ptr(), t.nbytes, True) for t in out]):
-        if start < written or (is_out and start < read):
-            raise ShapeError("an output overlaps a state or another output: states cannot be reordered in place")
-        if is_out:
-            written = start + size
-        else:
-            read = max(read, start + size)
+    if given:  # in the order of addresses, only states may lie over each other
+        rows, written, read = batch * beams, 0, 0  # (the ends of the outputs and of the states so far)
+        for start, is_out, size in sorted([*zip(sources, [False] * len(sizes), sizes), *zip(targets, [True] * len(sizes), sizes)]):
+            if start < written or (is_out and start < read):
+                raise ShapeError("an output overlaps a state or another output: states cannot be reordered in place")
+            if is_out:
+                written = start + size * rows
+            else:
+                read = max(read, start + size * rows)
     n = len(states)
     pointers = C.c_void_p * n
-    _call(parents.device, "eider_b200_beam_reorder_on_stream", pointers(*[s.data_ptr() for s in states]), pointers(*[o.data_ptr() for o in out]),
-          (C.c_size_t * n)(*sizes), n, parents.data_ptr(), stride, batch, beams)
+    _call(parents.device, "eider_b200_beam_reorder_on_stream", pointers(*sources), pointers(*targets), (C.c_size_t * n)(*sizes), n,
+          parents.data_ptr(), stride, batch, beams)
     return out
 
 
