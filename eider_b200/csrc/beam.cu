@@ -15,8 +15,8 @@
 // maxima (the k best elements cannot lie in any others: each of k better segments holds a better element) and then the k best of
 // their elements.  Nothing of the order of vocab is written or sorted; no atomics decide an order.
 //
-// Measured (B200): 64 x 8 x 151936 bf16 55.4 us, the scan 37 (4.1 TB/s; its share of the floor is 23.8) and the merge 21 (four
-// dependent passes over 19 thousand maxima a sequence, 64 CTAs of 148 SMs); 1 x 4 x 32000 f32 14.8 us, latencies of the two launches;
+// Measured (B200): 64 x 8 x 151936 bf16 55.4 us, the scan 37 (4.2 TB/s; its share of the floor is 23.8) and the merge 18 (four
+// dependent passes over 19 thousand maxima a sequence, 64 CTAs of 148 SMs); 1 x 4 x 32000 f32 16.5 us, dependent passes of one CTA;
 // reordering 64 x 8 states of 64 KB, twice, 15.8 us.
 #include <algorithm>
 #include <cmath>
