@@ -103,6 +103,7 @@ template <uint32_t BYTES> __device__ __forceinline__ uint4 shifted_piece(const u
     else return make_uint4(__funnelshift_r(w[kFirst], w[kFirst + 1], 16), __funnelshift_r(w[kFirst + 1], w[kFirst + 2], 16),
                            __funnelshift_r(w[kFirst + 2], w[kFirst + 3], 16), __funnelshift_r(w[kFirst + 3], w[kFirst + 4], 16));
 }
+
 // The running maximum and sum of a CTA's part of a row, and its segments' maxima.  The row begins BYTES behind a 16-byte boundary: if that
 // is not 0, a vector is the end of one piece of memory and the begin of the next.
 template <typename T, uint32_t BYTES> __device__ __forceinline__ void scan_row(const BeamArgs& a, const T* logits, float* segment_max, float& top, float& sum) {
